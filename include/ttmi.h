@@ -271,6 +271,55 @@ TTMI_API int ttmi_matmul_bfp_static(const void *a, int a_layout, const uint32_t 
  * a, b, c 16-byte aligned; c may alias a or b. */
 TTMI_API int ttmi_eltwise_bf16(int op, const void *a, const void *b, float scalar, void *c, size_t count, void *stream);
 
+/* ---- a key/value cache in pages -------------------------------------------------------------------------------------------
+ * One tensor for the keys and one for the values, [pages, kv_heads, page_size, head_dim] in TILE layout, dtype BFLOAT16 or
+ * BFLOAT8_B; page_size and head_dim are multiples of 32.  Token p of a request lies in slot
+ * table[p / page_size] * page_size + p % page_size, with the request's row of the page table.  Lengths, tables, slots and row
+ * starts are int32 in device memory and never come to the host, so a step can be captured into a graph and replayed on other
+ * lengths.  Whatever they hold, no call reads or writes outside the buffers whose sizes it is told: page numbers outside
+ * [0, pages), -1 among them, mean that there is no page, negative lengths count as 0.  No
+ * counterpart on the reference's block-float path.
+ *
+ * ttmi_paged_tables: what a step needs, from its requests' lengths, one launch.  Request r has cached[r] tokens from before and adds
+ * added[r] (requests at most 4096).
+ *   page_table     [requests, max_pages]; entries that r holds already (the first ceil(cached / page_size)) are kept
+ *   free_pages     page numbers to take from, in this order: requests in their order, each its pages in theirs
+ *   page_table_out as page_table (may be the same memory): old entries, then the pages taken, -1 beyond, and where free_pages ran out
+ *   slots          [tokens]: where every new token goes, request by request; -1 without a page (also past max_pages) and behind the last token
+ *   row_starts     [requests + 1]: the first row of every request's new tokens, and how many there are (never more than `tokens`)
+ *   counts         [2]: pages taken, and pages that were wanted and not there */
+TTMI_API int ttmi_paged_tables(const int32_t *cached, const int32_t *added, uint32_t requests, uint32_t page_size, const int32_t *page_table,
+                      uint32_t max_pages, const int32_t *free_pages, uint32_t free_count, uint32_t tokens, int32_t *page_table_out, int32_t *slots,
+                      int32_t *row_starts, int32_t *counts, void *stream);
+
+/* New keys and values into their slots, both caches in one launch.
+ *   rows      bf16 [tokens, width], layout TTMI_ROW_MAJOR or TTMI_TILE, e.g. the output of a fused qkv projection: the keys of token t
+ *             are columns [key_column, key_column + kv_heads * head_dim) of row t, the values likewise; columns are multiples of 32,
+ *             width is a multiple of 8 (TILE: of 32)
+ *   slots     [tokens]; a token whose slot is negative or past the last page is left out.  A slot may be named once
+ * BFLOAT8_B caches get the codes that ttmi_typecast_tiles gives for the bf16 values (one exponent for 16 neighbours of a
+ * token); no other token of the page changes. */
+TTMI_API int ttmi_paged_write(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t key_column, uint32_t value_column,
+                     const int32_t *slots, void *key_cache, void *value_cache, int cache_dtype, uint32_t pages, uint32_t kv_heads,
+                     uint32_t page_size, uint32_t head_dim, void *stream);
+
+/* Attention of new tokens over the cache that already holds them.  Row row_starts[r] + i of `rows` is token p = cached[r] + i of
+ * request r; its head h, columns [query_column + h * head_dim, + head_dim), attends with key head h / (heads / kv_heads) to the
+ * tokens j of the request with p - window < j <= p (window 0: all j <= p):  out = sum_j softmax_j(scale q . k_j) v_j, in
+ * fp32, probabilities rounded to bf16 for the product with the values, rounded once to bf16.  Tokens without a page are left
+ * out, as is what lies in a page behind the last token, whatever its bits; a row with nothing to attend to, and the rows behind
+ * row_starts[requests], are zeros.  Requests may have any number of new tokens each, none among them: decode steps, chunks of prompts
+ * and mixtures are one call.
+ *   out        bf16 [tokens, heads * head_dim], layout as `rows` (TILE: padding rows are zeros)
+ *   head_dim   64, 96, 128 or 256; heads a multiple of kv_heads
+ *   workspace  NULL (a buffer of the library, see above) or ttmi_paged_attention_workspace_bytes() bytes, 256-byte aligned: fp32
+ *              partial results of rows whose tokens are dealt out to several workgroups */
+TTMI_API size_t ttmi_paged_attention_workspace_bytes(uint32_t tokens, uint32_t requests, uint32_t heads, int cache_dtype, uint32_t kv_heads, uint32_t head_dim);
+TTMI_API int ttmi_paged_attention(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t query_column, const void *key_cache,
+                         const void *value_cache, int cache_dtype, uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim,
+                         const int32_t *page_table, uint32_t requests, uint32_t max_pages, const int32_t *cached, const int32_t *row_starts,
+                         uint32_t heads, float scale, uint32_t window, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

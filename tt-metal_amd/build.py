@@ -23,10 +23,11 @@ LIB = os.path.join(LIB_DIR, "libttmi.so")
 LIB_TEST = os.path.join(LIB_DIR, "libttmi_test.so")
 # translation units that the test hooks change (they are compiled twice); the others are shared by the two libraries
 HOOKED = ["host_state.hip", "bfp_matmul.hip", "bfp_matmul_tile.hip", "bfp_matmul_bf16.hip"]
-SOURCES = ["ttmi_capi.hip", "host_state.hip", "bfp_codec.hip", "bfp_matmul.hip", "bfp_matmul_tile.hip", "bfp_matmul_expanded.hip", "bfp_matmul_bf16.hip", "eltwise.hip"]
+SOURCES = ["ttmi_capi.hip", "host_state.hip", "bfp_codec.hip", "bfp_matmul.hip", "bfp_matmul_tile.hip", "bfp_matmul_expanded.hip", "bfp_matmul_bf16.hip", "eltwise.hip",
+           "paged_cache.hip", "paged_attention.hip"]
 # files whose device assembly is inspected before the object is built, and the check of check_isa.py that applies
 ISA_CHECKED = {"bfp_matmul.hip": "check", "bfp_matmul_tile.hip": "check_ring_operands", "bfp_matmul_bf16.hip": "check_lds_order"}
-HEADERS = [os.path.join(CSRC, "ttmi_internal.h"), os.path.join(CSRC, "bfp_dequant.h"), os.path.join(ROOT, "include", "ttmi.h")]
+HEADERS = [os.path.join(CSRC, "ttmi_internal.h"), os.path.join(CSRC, "bfp_dequant.h"), os.path.join(CSRC, "paged_cache.h"), os.path.join(ROOT, "include", "ttmi.h")]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

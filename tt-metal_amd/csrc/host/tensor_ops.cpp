@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <exception>
@@ -775,6 +776,116 @@ Tensor tilize(const Tensor &t, std::optional<DataType> dtype) {
     Tensor tiles = to_layout(t, Layout::TILE);
     if (!dtype || *dtype == tiles.dtype) return tiles;
     return typecast(tiles, *dtype);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// a key/value cache in pages
+// ---------------------------------------------------------------------------------------------------------------------------
+namespace {
+void need_on_device(const Tensor &t, int device, const std::string &op, const char *name) {
+    if (!t.allocated()) raise("TT_FATAL: " + op + ": " + name + " is not allocated");
+    if (!t.on_device()) raise("TT_FATAL: " + op + ": " + name + " needs to be on device!");
+    if (t.buffer.device != device) raise("TT_FATAL: " + op + ": " + name + " is on another device");
+}
+void need_integers(const Tensor &t, int device, const std::string &op, const char *name) {
+    need_on_device(t, device, op, name);
+    if (t.dtype != DataType::UINT32 || t.layout != Layout::ROW_MAJOR) raise("TT_FATAL: " + op + ": " + name + " must be a UINT32 tensor in ROW_MAJOR layout, got " + name_of(t.dtype) + " " + name_of(t.layout));
+}
+// tokens and width of activations [1, .., 1, tokens, width]
+std::pair<uint32_t, uint32_t> activation_rows(const Tensor &t, const std::string &op) {
+    if (!t.allocated() || !t.on_device()) raise("TT_FATAL: " + op + ": input_tensor needs to be on device!");
+    if (t.dtype != DataType::BFLOAT16) raise("TT_FATAL: " + op + ": input_tensor must be BFLOAT16, got " + name_of(t.dtype));
+    if (t.padded.size() < 2 || product(t.padded, 0, t.padded.size() - 2) != 1) raise("TT_FATAL: " + op + ": input_tensor must be [1, 1, tokens, width], got " + list_of(t.shape));
+    return {t.layout == Layout::TILE ? t.shape[t.shape.size() - 2] : t.padded[t.padded.size() - 2], t.padded.back()};
+}
+struct CacheShape { uint32_t pages, kv_heads, page_size, head_dim; };
+CacheShape cache_shape(const Tensor &keys, const Tensor &values, int device, const std::string &op) {
+    need_on_device(keys, device, op, "key_cache");
+    need_on_device(values, device, op, "value_cache");
+    if (keys.padded.size() != 4 || keys.layout != Layout::TILE || keys.shape != keys.padded)
+        raise("TT_FATAL: " + op + ": a cache must be [pages, kv_heads, page_size, head_dim] in TILE layout without padding, got " + list_of(keys.shape) + " " + name_of(keys.layout));
+    if (values.padded != keys.padded || values.shape != keys.shape || values.dtype != keys.dtype || values.layout != keys.layout)
+        raise("TT_FATAL: " + op + ": key_cache and value_cache must have the same shape, dtype and layout");
+    if (keys.dtype != DataType::BFLOAT16 && keys.dtype != DataType::BFLOAT8_B) raise("TT_FATAL: " + op + ": a cache must be BFLOAT16 or BFLOAT8_B, got " + name_of(keys.dtype));
+    return {keys.padded[0], keys.padded[1], keys.padded[2], keys.padded[3]};
+}
+Tensor integers(const Dims &shape, int device) {
+    Tensor t;
+    t.shape = t.padded = shape;
+    t.dtype = DataType::UINT32;
+    t.layout = Layout::ROW_MAJOR;
+    t.buffer = allocate(product(shape) * 4, device);
+    return t;
+}
+const int32_t *ints(const Tensor &t) { return (const int32_t *)t.buffer.data; }
+int32_t *ints(Tensor &t) { return (int32_t *)t.buffer.data; }
+}  // namespace
+
+Tensor allocate_paged_cache(uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, DataType dtype, int device) {
+    need_gpu();
+    if (dtype != DataType::BFLOAT16 && dtype != DataType::BFLOAT8_B) raise(std::string("TT_FATAL: a cache must be BFLOAT16 or BFLOAT8_B, got ") + name_of(dtype));
+    if (!pages || !kv_heads || !page_size || !head_dim || page_size % 32 || head_dim % 32)
+        raise("TT_FATAL: page size and head dimension must be multiples of 32, got " + list_of({pages, kv_heads, page_size, head_dim}));
+    Tensor t;
+    t.shape = t.padded = {pages, kv_heads, page_size, head_dim};
+    t.dtype = dtype;
+    t.layout = Layout::TILE;
+    t.buffer = allocate(storage_bytes(dtype, t.layout, t.padded), device);
+    return t;
+}
+
+std::vector<Tensor> paged_tables(const Tensor &cached, const Tensor &added, const Tensor &page_table, const Tensor &free_pages, uint32_t page_size, uint32_t tokens,
+                                 const std::string &op) {
+    const int device = cached.buffer.device;
+    need_integers(cached, device, op, "cached_lengths");
+    need_integers(added, device, op, "new_lengths");
+    need_integers(page_table, device, op, "page_table");
+    need_integers(free_pages, device, op, "free_pages");
+    const uint32_t requests = (uint32_t)cached.volume();
+    if (added.volume() != requests) raise("TT_FATAL: " + op + ": cached_lengths and new_lengths must name the same requests");
+    if (page_table.padded.size() < 2 || product(page_table.padded, 0, page_table.padded.size() - 1) != requests)
+        raise("TT_FATAL: " + op + ": page_table must be [requests, pages], got " + list_of(page_table.shape) + " for " + std::to_string(requests) + " requests");
+    if (free_pages.volume() > 0x7fffffffu) raise("TT_FATAL: " + op + ": too many free pages");
+    DeviceGuard guard(device);
+    std::vector<Tensor> out{integers(page_table.padded, device), integers({tokens}, device), integers({requests + 1}, device), integers({2}, device)};
+    check(ttmi_paged_tables(ints(cached), ints(added), requests, page_size, ints(page_table), page_table.padded.back(), ints(free_pages), (uint32_t)free_pages.volume(), tokens,
+                            ints(out[0]), ints(out[1]), ints(out[2]), ints(out[3]), stream_of(device)));
+    return out;
+}
+
+void paged_write(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &slots, uint32_t key_column, uint32_t value_column, const std::string &op) {
+    const auto [tokens, width] = activation_rows(rows, op);
+    const int device = rows.buffer.device;
+    const CacheShape c = cache_shape(key_cache, value_cache, device, op);
+    need_integers(slots, device, op, "slots");
+    if (slots.volume() != tokens) raise("TT_FATAL: " + op + ": " + std::to_string(slots.volume()) + " slots for " + std::to_string(tokens) + " tokens");
+    if (key_cache.buffer.data == value_cache.buffer.data) raise("TT_FATAL: " + op + ": key_cache and value_cache are the same memory");
+    DeviceGuard guard(device);
+    check(ttmi_paged_write(rows.buffer.data, (int)rows.layout, tokens, width, key_column, value_column, ints(slots), key_cache.buffer.data, value_cache.buffer.data, (int)key_cache.dtype,
+                           c.pages, c.kv_heads, c.page_size, c.head_dim, stream_of(device)));
+}
+
+Tensor paged_attention(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &page_table, const Tensor &cached, const Tensor &row_starts,
+                       uint32_t heads, uint32_t query_column, std::optional<float> scale, uint32_t window, const std::string &op) {
+    const auto [tokens, width] = activation_rows(rows, op);
+    const int device = rows.buffer.device;
+    const CacheShape c = cache_shape(key_cache, value_cache, device, op);
+    need_integers(page_table, device, op, "page_table");
+    need_integers(cached, device, op, "cached_lengths");
+    need_integers(row_starts, device, op, "row_starts");
+    const uint32_t requests = (uint32_t)cached.volume();
+    if (row_starts.volume() != (uint64_t)requests + 1) raise("TT_FATAL: " + op + ": row_starts must have one element more than cached_lengths");
+    if (page_table.padded.size() < 2 || product(page_table.padded, 0, page_table.padded.size() - 1) != requests)
+        raise("TT_FATAL: " + op + ": page_table must be [requests, pages], got " + list_of(page_table.shape) + " for " + std::to_string(requests) + " requests");
+    if (!heads || (uint64_t)heads * c.head_dim > width) raise("TT_FATAL: " + op + ": " + std::to_string(heads) + " heads of " + std::to_string(c.head_dim) + " elements do not fit rows of " + std::to_string(width));
+    DeviceGuard guard(device);
+    Tensor out = rows;
+    out.shape.back() = out.padded.back() = heads * c.head_dim;
+    out.buffer = allocate(storage_bytes(out.dtype, out.layout, out.padded), device);
+    check(ttmi_paged_attention(rows.buffer.data, (int)rows.layout, tokens, width, query_column, key_cache.buffer.data, value_cache.buffer.data, (int)key_cache.dtype, c.pages, c.kv_heads,
+                               c.page_size, c.head_dim, ints(page_table), requests, page_table.padded.back(), ints(cached), ints(row_starts), heads,
+                               scale ? *scale : 1.f / std::sqrt((float)c.head_dim), window, out.buffer.data, nullptr, 0, stream_of(device)));
+    return out;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------

@@ -91,6 +91,15 @@ Tensor typecast(const Tensor &t, DataType dtype);                               
 Tensor clone(const Tensor &t, std::optional<DataType> dtype);                                          // copy_op.hpp:42
 Tensor tilize(const Tensor &t, std::optional<DataType> dtype);                                         // tilize_op.hpp:71-73
 
+// ---- a key/value cache in pages (include/ttmi.h: ttmi_paged_*); lengths, tables and slots are UINT32 tensors on the device --------
+Tensor allocate_paged_cache(uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, DataType dtype, int device);     // contents undefined
+// {page table, slots, row starts, counts}
+std::vector<Tensor> paged_tables(const Tensor &cached, const Tensor &added, const Tensor &page_table, const Tensor &free_pages, uint32_t page_size, uint32_t tokens,
+                                 const std::string &op);
+void paged_write(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &slots, uint32_t key_column, uint32_t value_column, const std::string &op);
+Tensor paged_attention(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &page_table, const Tensor &cached, const Tensor &row_starts,
+                       uint32_t heads, uint32_t query_column, std::optional<float> scale, uint32_t window, const std::string &op);
+
 // ---- ttnn.from_torch / to_torch / to_layout / __getitem__ (ttnn/ttnn/operations/core.py) ------------------------------------
 // from_torch for block-float: data is host fp32 or bf16 (src_dtype), logical shape `shape`; one fused pad + tilize + pack.
 Tensor ttnn_from_torch_block_float(const void *data, DataType src_dtype, const Dims &shape, DataType dtype, int device);

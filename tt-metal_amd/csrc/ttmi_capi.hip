@@ -2,6 +2,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include "paged_cache.h"
 #include "ttmi_internal.h"
 
 namespace ttmi {
@@ -47,6 +48,30 @@ int validate_matmul(const void *a, int a_layout, const uint32_t *b, int b_fmt, u
         return fail(TTMI_ERR_INVALID_ARGUMENT, "matmul: a, b and c must be 16-byte aligned");
     return TTMI_OK;
 }
+
+// ---- paged key/value cache: what every entry point asks of its tensors
+static int validate_paged_cache(const PagedCache &c) {
+    if (c.dtype != TTMI_BFLOAT16 && c.dtype != TTMI_BFLOAT8_B) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: dtype must be BFLOAT16 or BFLOAT8_B, got %d", c.dtype);
+    if (!c.pages || !c.kv_heads) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: no pages or no heads");
+    if (!c.page_size || (c.page_size & 31)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: page size (%u) must be a multiple of 32", c.page_size);
+    if (!c.head_dim || (c.head_dim & 31)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: head dimension (%u) must be a multiple of 32", c.head_dim);
+    if ((uint64_t)c.pages * c.page_size > 0x7fffffffull) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: %u pages of %u tokens are more slots than an int32 names", c.pages, c.page_size);
+    if ((uint64_t)c.kv_heads * c.head_dim > 0x7fffffffull / 4) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: %u heads of %u elements are too many", c.kv_heads, c.head_dim);
+    return TTMI_OK;
+}
+// `elements` columns from `column` on, of rows that lie as `r` says
+static int validate_paged_columns(const PagedRows &r, uint32_t column, uint64_t elements, const char *what) {
+    if (column & 31) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: the first %s column (%u) must be a multiple of 32", what, column);
+    if (column + elements > r.width) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: %s columns %u to %llu lie outside rows of %u", what, column, (unsigned long long)(column + elements), r.width);
+    return TTMI_OK;
+}
+static int validate_paged_rows(const PagedRows &r) {
+    if (r.layout != TTMI_ROW_MAJOR && r.layout != TTMI_TILE) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: unknown layout");
+    if (r.width & (r.layout == TTMI_TILE ? 31u : 7u)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: width (%u) must be a multiple of %d", r.width, r.layout == TTMI_TILE ? 32 : 8);
+    if (r.tokens > 0x7fffffe0u) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged cache: too many rows (%u)", r.tokens);
+    return TTMI_OK;
+}
+static bool misaligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) & (to - 1); }
 
 }  // namespace ttmi
 
@@ -224,6 +249,65 @@ int ttmi_eltwise_bf16(int op, const void *a, const void *b, float scalar, void *
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15u)
         return fail(TTMI_ERR_INVALID_ARGUMENT, "eltwise: a, b and c must be 16-byte aligned");
     return eltwise_bf16(op, a, b, scalar, c, count, (hipStream_t)stream);
+}
+
+int ttmi_paged_tables(const int32_t *cached, const int32_t *added, uint32_t requests, uint32_t page_size, const int32_t *page_table, uint32_t max_pages,
+                      const int32_t *free_pages, uint32_t free_count, uint32_t tokens, int32_t *page_table_out, int32_t *slots, int32_t *row_starts,
+                      int32_t *counts, void *stream) {
+    if (!page_size || (page_size & 31)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged tables: page size (%u) must be a multiple of 32", page_size);
+    if (requests > PAGED_MAX_REQUESTS) return fail(TTMI_ERR_UNSUPPORTED, "paged tables: %u requests, at most %u", requests, PAGED_MAX_REQUESTS);
+    if (tokens > 0x7fffffffu || free_count > 0x7fffffffu) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged tables: more than 2^31 - 1 tokens or free pages");
+    const uint64_t entries = (uint64_t)requests * max_pages;
+    if (!row_starts || !counts || (requests && (!cached || !added)) || (entries && (!page_table || !page_table_out)) || (free_count && !free_pages) || (tokens && !slots))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged tables: null pointer");
+    const void *all[] = {cached, added, page_table, free_pages, page_table_out, slots, row_starts, counts};
+    for (const void *p : all)
+        if (misaligned(p, 4)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged tables: pointers must be 4-byte aligned");
+    return paged_tables(cached, added, requests, page_size, page_table, max_pages, free_pages, free_count, tokens, page_table_out, slots, row_starts, counts, (hipStream_t)stream);
+}
+
+int ttmi_paged_write(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t key_column, uint32_t value_column, const int32_t *slots, void *key_cache,
+                     void *value_cache, int cache_dtype, uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, void *stream) {
+    const PagedRows r{rows, layout, tokens, width};
+    const PagedCache c{cache_dtype, pages, kv_heads, page_size, head_dim};
+    if (int rc = validate_paged_cache(c)) return rc;
+    if (int rc = validate_paged_rows(r)) return rc;
+    if (int rc = validate_paged_columns(r, key_column, (uint64_t)kv_heads * head_dim, "key")) return rc;
+    if (int rc = validate_paged_columns(r, value_column, (uint64_t)kv_heads * head_dim, "value")) return rc;
+    if (!key_cache || !value_cache || (tokens && (!rows || !slots))) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged write: null pointer");
+    if (misaligned(rows, 16) || misaligned(key_cache, 16) || misaligned(value_cache, 16) || misaligned(slots, 4))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged write: rows and caches must be 16-byte aligned, slots 4-byte aligned");
+    return paged_write(r, key_column, value_column, slots, key_cache, value_cache, c, (hipStream_t)stream);
+}
+
+size_t ttmi_paged_attention_workspace_bytes(uint32_t tokens, uint32_t requests, uint32_t heads, int cache_dtype, uint32_t kv_heads, uint32_t head_dim) {
+    if (!tokens || !requests || !kv_heads || !heads || heads % kv_heads) return 0;
+    return paged_attention_workspace_bytes(tokens, requests, heads, PagedCache{cache_dtype, 1, kv_heads, 32, head_dim});
+}
+
+int ttmi_paged_attention(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t query_column, const void *key_cache, const void *value_cache, int cache_dtype,
+                         uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, const int32_t *page_table, uint32_t requests, uint32_t max_pages,
+                         const int32_t *cached, const int32_t *row_starts, uint32_t heads, float scale, uint32_t window, void *out, void *workspace, size_t workspace_bytes,
+                         void *stream) {
+    const PagedCache c{cache_dtype, pages, kv_heads, page_size, head_dim};
+    const PagedRows r{rows, layout, tokens, width};
+    if (int rc = validate_paged_cache(c)) return rc;
+    if (int rc = validate_paged_rows(r)) return rc;
+    if (head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 256) return fail(TTMI_ERR_UNSUPPORTED, "paged attention: head dimension %u (64, 96, 128 or 256)", head_dim);
+    if (!heads || heads % kv_heads) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: %u query heads are no multiple of %u key heads", heads, kv_heads);
+    if (heads > 0x7fffffffu / head_dim) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: too many heads (%u)", heads);
+    if (int rc = validate_paged_columns(r, query_column, (uint64_t)heads * head_dim, "query")) return rc;
+    if (requests > PAGED_MAX_REQUESTS) return fail(TTMI_ERR_UNSUPPORTED, "paged attention: %u requests, at most %u", requests, PAGED_MAX_REQUESTS);
+    if ((uint64_t)max_pages * page_size > 0x7fffffffull) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: %u pages of %u tokens are more than an int32 counts", max_pages, page_size);
+    if (!(scale == scale) || scale - scale != 0.f) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: scale must be finite");
+    if (!key_cache || !value_cache || !row_starts || (requests && !cached) || ((uint64_t)requests * max_pages && !page_table) || (tokens && (!rows || !out)))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: null pointer");
+    if (misaligned(rows, 16) || misaligned(key_cache, 16) || misaligned(value_cache, 16) || misaligned(out, 16) || misaligned(page_table, 4) || misaligned(cached, 4) || misaligned(row_starts, 4))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: rows, caches and out must be 16-byte aligned, the rest 4-byte aligned");
+    if (workspace && (misaligned(workspace, 256) || workspace_bytes < ttmi_paged_attention_workspace_bytes(tokens, requests, heads, cache_dtype, kv_heads, head_dim)))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: workspace of %zu bytes, 256-byte aligned, expected", ttmi_paged_attention_workspace_bytes(tokens, requests, heads, cache_dtype, kv_heads, head_dim));
+    const PagedAttentionArgs args{r, query_column, key_cache, value_cache, c, PagedStep{page_table, requests, max_pages, cached, row_starts}, heads, scale, window, out, workspace, workspace_bytes};
+    return paged_attention(args, (hipStream_t)stream);
 }
 
 }  // extern "C"

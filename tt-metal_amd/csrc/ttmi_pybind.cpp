@@ -167,6 +167,12 @@ void bind_tensor_layer(py::module_ &m) {
     m.def("typecast", [](const host::Tensor &t, int dtype) { return host::typecast(t, (host::DataType)dtype); }, no_gil);
     m.def("clone", [](const host::Tensor &t, const py::object &dtype) { const auto d = optional_dtype(dtype); return unlocked([&] { return host::clone(t, d); }); });
     m.def("tilize", [](const host::Tensor &t, const py::object &dtype) { const auto d = optional_dtype(dtype); return unlocked([&] { return host::tilize(t, d); }); });
+    m.def("allocate_paged_cache", [](uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, int dtype, int device) {
+        return unlocked([&] { return host::allocate_paged_cache(pages, kv_heads, page_size, head_dim, (host::DataType)dtype, device); });
+    });
+    m.def("paged_tables", &host::paged_tables, no_gil);
+    m.def("paged_write", &host::paged_write, no_gil);
+    m.def("paged_attention", &host::paged_attention, no_gil);
     m.def("ttnn_from_torch_block_float",
           [](uintptr_t data, int src_dtype, host::Dims shape, int dtype, int device) {
               return unlocked([&] { return host::ttnn_from_torch_block_float(reinterpret_cast<const void *>(data), (host::DataType)src_dtype, shape, (host::DataType)dtype, device); });

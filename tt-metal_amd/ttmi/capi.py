@@ -29,6 +29,7 @@ SYMBOLS = (
     "ttmi_matmul_bfp_gated_workspace_bytes", "ttmi_matmul_bfp_gated", "ttmi_matmul_bf16_workspace_bytes", "ttmi_matmul_bf16",
     "ttmi_release_scratch", "ttmi_matmul_bfp_ab_supported", "ttmi_matmul_bfp_ab", "ttmi_matmul_bfp_plan",
     "ttmi_matmul_bias_tiles", "ttmi_matmul_bias_tiles_supported",
+    "ttmi_paged_tables", "ttmi_paged_write", "ttmi_paged_attention", "ttmi_paged_attention_workspace_bytes",
 )
 
 _lib = None
@@ -114,6 +115,14 @@ def _load(path: str) -> ctypes.CDLL:
         L.ttmi_release_scratch.argtypes = [ctypes.POINTER(ctypes.c_size_t)]
         L.ttmi_eltwise_bf16.restype = i32
         L.ttmi_eltwise_bf16.argtypes = [i32, vp, vp, ctypes.c_float, vp, sz, vp]
+        L.ttmi_paged_tables.restype = i32
+        L.ttmi_paged_tables.argtypes = [vp, vp, u32, u32, vp, u32, vp, u32, u32, vp, vp, vp, vp, vp]
+        L.ttmi_paged_write.restype = i32
+        L.ttmi_paged_write.argtypes = [vp, i32, u32, u32, u32, u32, vp, vp, vp, i32, u32, u32, u32, u32, vp]
+        L.ttmi_paged_attention_workspace_bytes.restype = sz
+        L.ttmi_paged_attention_workspace_bytes.argtypes = [u32, u32, u32, i32, u32, u32]
+        L.ttmi_paged_attention.restype = i32
+        L.ttmi_paged_attention.argtypes = [vp, i32, u32, u32, u32, vp, vp, i32, u32, u32, u32, u32, vp, u32, u32, vp, vp, u32, ctypes.c_float, u32, vp, vp, sz, vp]
         _loaded[path] = L
     return _loaded[path]
 

@@ -2,3 +2,4 @@
 from __future__ import annotations
 
 from .matmul import gated_linear  # noqa: F401
+from .paged import allocate_paged_cache, attend_paged_cache, paged_tables, write_paged_cache  # noqa: F401
