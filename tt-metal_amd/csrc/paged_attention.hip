@@ -3,15 +3,35 @@
 // Request r has cached_r tokens from before and n_r = row_starts[r + 1] - row_starts[r] new ones, all of them in the cache.  Row
 // row_starts[r] + i of the activations is token p = cached_r + i.  For each of its heads, with the key head that its group shares,
 //   out = sum_j softmax_j(scale q . k_j) v_j    over the tokens p - window < j <= p that have a page
-// and zeros where nothing is left.  Slots behind a request's last token hold whatever was there before, infinities and NaN
-// among it, and never count.
+// and zeros where nothing is left.
 //
-// One wavefront per row and query head: 64 keys at a time, one to a lane, the running maximum and sum of the softmax in fp32, then
-// each lane adds up its elements of the 64 values.
+// Common to both kernels
+//   rows       the heads that share a key head are rows of one product: row rho of (request, key head) is token rho / group, head
+//              rho % group of the group, so a decode step of 4 heads per key head is 4 rows, a chunk of 512 tokens 2048
+//   units      (request, key head, tile of ROWS rows).  A unit's tokens are cut into pieces of a common length, which is chosen from the
+//              lengths on the device so that the whole step comes to about `target` pieces: requests of any lengths, one long one among
+//              them, fill the chip evenly.  Every workgroup makes the same prefix sums over the requests and takes pieces
+//              blockIdx, blockIdx + gridDim, ...  A unit of one piece is stored at once; the others leave (maximum, sum, fp32
+//              accumulators) in memory, and whoever comes last joins them, in the order of the pieces
+//   softmax    one pass: running maximum m and sum l per row in fp32, weights exp2(s - m).  m only moves when a score passes it
+//              by more than 2^8 in weight, so that the accumulators are hardly ever rescaled
+//   products   keys times queries and values times weights, both transposed: a lane's accumulators belong to one row, so m, l and the
+//              rescaling are the lane's own, and the weights leave the first product in the very lanes that the second one
+//              wants them in (the tokens of a k step are permuted alike on both sides).  Weights are rounded to bf16 for
+//              the second product, as the values are, and l is the sum of the rounded ones: what a row is divided by is what it
+//              was multiplied with, so a row of one token is that token's value (v_dot2_f32_bf16 adds two at a time).  Rows of
+//              few tokens have no others for the roundings to cancel against: in the block where a row ends what the rounding
+//              took off is a second product
+//   masks      a score that does not count becomes -inf.  Values that no row of the unit sees (behind the last token, before the
+//              window) are zeroed on their way into LDS: 0 x NaN is NaN.  Where rows of a unit see different tokens and one of
+//              them is not finite, the product is made token by token of the unit, each time with the values that it sees
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
+#include <mutex>
+#include <type_traits>
 
 #include "bfp_dequant.h"
 #include "paged_cache.h"
@@ -19,104 +39,1059 @@
 
 namespace ttmi {
 
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+
 struct AttentionDev {
-    const uint8_t *rows;
-    const uint8_t *keys, *values;
+    const uint8_t *rows, *keys, *values;
     const int32_t *table, *cached, *starts;
     uint8_t *out;
-    uint32_t tokens, width, query_column, requests, max_pages;
-    uint32_t pages, kv_heads, page_size, head_dim, heads, group, window;
-    float scale;                           // times log2(e)
-    int tiled, packed;
+    uint32_t tokens, out_rows, width, query_column, requests, max_pages;
+    uint32_t pages, kv_heads, page_blocks, heads, group, window;
+    uint32_t least_rows, most_rows;        // requests of that many rows per key head are this launch's
+    uint32_t target, slots;                // pieces aimed at; partial results that fit
+    uint32_t *counters;                    // pieces of a unit that are done, by the unit's first slot; all zero between launches
+    uint8_t *partial;
+    float scale;                           // |scale| log2(e), and what block floats are too large by
+    uint32_t flip;                         // sign bits of the queries, for a negative scale
+    int tiled, zero_rows;                  // zero_rows: this launch clears the rows of no request
 };
 
-__device__ __forceinline__ float bf16_at(const uint8_t *p) { return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(p) << 16); }
+constexpr uint32_t COUNTERS = 4096;        // at most 2 `target` slots, each could be a unit's first
+constexpr float LAZY = 8.f;                // how far (log2) a score may pass the running maximum
 
-// element d of a token that lies in row `at` of a head's page
-__device__ __forceinline__ float cached_element(const uint8_t *head_page, uint32_t at, uint32_t d, uint32_t head_dim, int packed) {
-    const uint64_t tile = (uint64_t)(at / 32) * (head_dim / 32) + d / 32;
-    const uint32_t face = (at >> 4 & 1) * 2 + (d >> 4 & 1), row = at & 15, e = d & 15;
-    if (!packed) return bf16_at(head_page + tile * 2048 + face * 512 + row * 32 + e * 2);
-    const uint8_t *t = head_page + tile * 1088;
-    const uint32_t code = t[64 + face * 256 + row * 16 + e];
-    const float v = (float)(code & 127u) * row_scale(t[face * 16 + row]) * Wfmt<7>::unscale;
-    return code & 128u ? -v : v;
+// ---- the work of a step ---------------------------------------------------------------------------------------------------------
+struct Request { uint32_t start, added, cached; };
+__device__ __forceinline__ Request request_at(const AttentionDev &p, uint32_t r) {
+    const uint32_t from = min((uint32_t)max(p.starts[r], 0), p.tokens), to = min((uint32_t)max(p.starts[r + 1], 0), p.tokens);
+    return {from, to > from ? to - from : 0u, (uint32_t)max(p.cached[r], 0)};
+}
+// first token that a row at `position` sees
+__device__ __forceinline__ uint32_t first_seen(const AttentionDev &p, uint32_t position) {
+    return p.window && position >= p.window ? position - p.window + 1 : 0u;
 }
 
-__global__ __launch_bounds__(64) void paged_attention_rows_kernel(const AttentionDev p) {
-    const uint32_t lane = threadIdx.x;
-    const uint32_t t = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
-    const uint64_t out_width = p.heads * p.head_dim;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};                       // elements lane, lane + 64, ... of the head
-    float sum = 0.f, top = -INFINITY;
+template <int ROWS> struct Extent {
+    uint32_t units, blocks;                // units of the request; 32-token blocks that one of them has at most
+    __device__ __forceinline__ Extent(const AttentionDev &p, const Request &q) {
+        const uint64_t rows = (uint64_t)q.added * p.group;
+        if (rows < p.least_rows || rows > p.most_rows) { units = blocks = 0; return; }
+        units = (uint32_t)((rows + ROWS - 1) / ROWS) * p.kv_heads;
+        const uint32_t end = min((q.cached + q.added - 1) / 32 + 1, p.max_pages * p.page_blocks), begin = min(first_seen(p, q.cached) / 32, end);
+        blocks = end - begin;
+        if (p.window) blocks = (uint32_t)min((uint64_t)blocks, ((uint64_t)p.window + ROWS / p.group + 2) / 32 + 2);
+        blocks = max(blocks, 1u);
+    }
+};
+
+// Exclusive prefix sum over the workgroup, and the sum of all.
+template <int THREADS> __device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t *wave_sums, uint64_t &all) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t to = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_up(to, d);
+        if (lane >= (uint32_t)d) to += o;
+    }
+    __syncthreads();
+    if (lane == 63) wave_sums[wave] = to;
+    __syncthreads();
+    to -= v;
+    all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < THREADS / 64; ++w) {
+        if (w < wave) to += wave_sums[w];
+        all += wave_sums[w];
+    }
+    return to;
+}
+
+struct Plan { uint32_t piece, pieces; };   // blocks of a piece, pieces of the step
+// first_piece[requests + 1], first_slot[requests]: LDS
+template <int THREADS, int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const AttentionDev &p, uint32_t *first_piece, uint32_t *first_slot, uint64_t *wave_sums) {
+    const uint32_t each = (p.requests + THREADS - 1) / THREADS, r0 = min(threadIdx.x * each, p.requests), r1 = min(r0 + each, p.requests);
+    uint64_t work = 0, all;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const Extent<ROWS> e(p, request_at(p, r));
+        work += (uint64_t)e.units * e.blocks;
+    }
+    scan<THREADS>(work, wave_sums, all);
+    const uint64_t share = (all + p.target - 1) / p.target;
+    const uint32_t piece = (uint32_t)(max(share, (uint64_t)1) + STEP - 1) / STEP * STEP;
+    uint64_t pieces = 0, slots = 0;        // of this lane's requests: pieces, and those of units with more than one, together in one scan
+    for (uint32_t r = r0; r < r1; ++r) {
+        const Extent<ROWS> e(p, request_at(p, r));
+        const uint32_t parts = (e.blocks + piece - 1) / piece;
+        pieces += (uint64_t)e.units * parts;
+        if (parts > 1) slots += (uint64_t)e.units * parts;
+    }
+    uint64_t at = scan<THREADS>(pieces | slots << 32, wave_sums, all);
+    for (uint32_t r = r0; r < r1; ++r) {
+        const Extent<ROWS> e(p, request_at(p, r));
+        const uint32_t parts = (e.blocks + piece - 1) / piece;
+        first_piece[r] = (uint32_t)at;
+        first_slot[r] = (uint32_t)(at >> 32);
+        at += (uint64_t)e.units * parts;
+        if (parts > 1) at += (uint64_t)e.units * parts << 32;
+    }
+    if (threadIdx.x == 0) first_piece[p.requests] = (uint32_t)all;
+    __syncthreads();
+    return {piece, (uint32_t)all};
+}
+
+// One piece: rows [row0, row0 + rows) of a request and key head, blocks [begin, end) of those that the unit sees.
+struct Piece {
+    Request q;
+    uint32_t r, kv, row0, rows, begin, end, parts, part, slot;
+    uint32_t token0, token1;               // first and last token of the unit, counted from the request's first new one
+};
+template <int ROWS> __device__ __forceinline__ Piece piece_at(const AttentionDev &p, const Plan &plan, const uint32_t *first_piece, const uint32_t *first_slot, uint32_t index) {
     uint32_t low = 0, high = p.requests;
-    if (t < p.tokens && t < (uint32_t)max(p.starts[p.requests], 0)) {
-        while (high - low > 1) {
-            const uint32_t mid = (low + high) / 2;
-            if ((uint32_t)max(p.starts[mid], 0) <= t) low = mid; else high = mid;
-        }
-        const uint32_t r = low;
-        const uint64_t position = (uint64_t)max(p.cached[r], 0) + (t - (uint32_t)max(p.starts[r], 0));
-        const uint64_t first = p.window && position + 1 > p.window ? position + 1 - p.window : 0;
-        const uint64_t end = min(position + 1, (uint64_t)p.max_pages * p.page_size);
-        const uint64_t page_bytes = (uint64_t)(p.page_size / 32) * (p.head_dim / 32) * (p.packed ? 1088 : 2048);
-        const uint32_t kv = h / p.group;
-        for (uint64_t j0 = first / 64 * 64; j0 < end; j0 += 64) {
-            const uint64_t j = j0 + lane;
-            int32_t page = -1;
-            if (j >= first && j < end) page = p.table[(uint64_t)r * p.max_pages + j / p.page_size];
-            const bool there = (uint32_t)page < p.pages;
-            const uint32_t at = (uint32_t)(j % p.page_size);
-            const uint64_t head_page = ((uint64_t)page * p.kv_heads + kv) * page_bytes;
-            float score = -INFINITY;
-            if (there) {
-                float dot = 0.f;
-                for (uint32_t d = 0; d < p.head_dim; ++d)
-                    dot += bf16_at(p.rows + row_bytes_at(t, p.width, p.query_column + h * p.head_dim + (d & ~7u), p.tiled) + (d & 7) * 2) *
-                           cached_element(p.keys + head_page, at, d, p.head_dim, p.packed);
-                score = dot * p.scale;
-            }
-            float most = score;
-            for (int s = 32; s; s >>= 1) most = fmaxf(most, __shfl_xor(most, s));
-            most = fmaxf(most, top);
-            const float from = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(top - from);
-            const float weight = there ? __builtin_amdgcn_exp2f(score - from) : 0.f;
-            float all = weight;
-            for (int s = 32; s; s >>= 1) all += __shfl_xor(all, s);
-            sum = sum * shrink + all;
-            top = most;
-            for (int i = 0; i < 4; ++i) acc[i] *= shrink;
-            for (int l = 0; l < 64; ++l) {
-                const float w = __shfl(weight, l);
-                if (!__shfl((int)there, l)) continue;          // the whole wavefront
-                const uint32_t at_l = __shfl(at, l);
-                const uint64_t page_l = ((uint64_t)__shfl(page, l) * p.kv_heads + kv) * page_bytes;
-                for (uint32_t i = 0, d = lane; d < p.head_dim; ++i, d += 64) acc[i] += w * cached_element(p.values + page_l, at_l, d, p.head_dim, p.packed);
-            }
+    while (high - low > 1) {
+        const uint32_t mid = (low + high) / 2;
+        if (first_piece[mid] <= index) low = mid; else high = mid;
+    }
+    Piece x;
+    x.r = __builtin_amdgcn_readfirstlane(low);
+    x.q = request_at(p, x.r);
+    const Extent<ROWS> e(p, x.q);
+    const uint32_t most = (e.blocks + plan.piece - 1) / plan.piece, tiles = e.units / p.kv_heads;
+    uint32_t local = index - first_piece[x.r];
+    x.kv = local % p.kv_heads; local /= p.kv_heads;
+    x.part = local % most;
+    const uint32_t tile = tiles - 1 - local / most;            // the last tile of a chunk sees most: first
+    const uint32_t all_rows = x.q.added * p.group;
+    x.row0 = tile * ROWS;
+    x.rows = min((uint32_t)ROWS, all_rows - x.row0);
+    x.token0 = x.row0 / p.group;
+    x.token1 = (x.row0 + x.rows - 1) / p.group;
+    const uint32_t end = min((x.q.cached + x.token1) / 32 + 1, p.max_pages * p.page_blocks), begin = min(first_seen(p, x.q.cached + x.token0) / 32, end);
+    x.parts = max((end - begin + plan.piece - 1) / plan.piece, 1u);
+    x.begin = min(begin + x.part * plan.piece, end);
+    x.end = min(x.begin + plan.piece, end);
+    x.slot = first_slot[x.r] + (tile * p.kv_heads + x.kv) * most;
+    return x;
+}
+
+// Pages of the blocks first, first + STRIDE, ... of a piece, 64 at a time: lane i has entry i, -1 for what is no page or lies past the end.
+template <int STRIDE> struct Pages {
+    int32_t page;
+    uint32_t within;
+    __device__ __forceinline__ void load(const AttentionDev &p, const Piece &x, uint32_t first) {
+        const uint32_t b = first + (threadIdx.x & 63) * STRIDE;
+        page = -1;
+        within = b % p.page_blocks;
+        if (b < x.end) {
+            page = p.table[(uint64_t)x.r * p.max_pages + b / p.page_blocks];
+            if ((uint32_t)page >= p.pages) page = -1;
         }
     }
-    const float share = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    for (uint32_t i = 0, d = lane; d < p.head_dim; ++i, d += 64) {
-        const uint32_t column = h * p.head_dim + d;
-        *reinterpret_cast<uint16_t *>(p.out + row_bytes_at(t, (uint32_t)out_width, column & ~7u, p.tiled) + (column & 7) * 2) = (uint16_t)f32x2_to_bf16x2_rne(sum == 0.f ? 0.f : acc[i] * share, 0.f);
+    // number of the tile row of `head`, of page 0 where there is none; false there
+    __device__ __forceinline__ bool at(const AttentionDev &p, uint32_t head, uint32_t i, uint64_t &tile_row) const {
+        const int32_t g = __builtin_amdgcn_readlane(page, i);
+        tile_row = ((uint64_t)(uint32_t)max(g, 0) * p.kv_heads + head) * p.page_blocks + (uint32_t)__builtin_amdgcn_readlane(within, i);
+        return g >= 0;
+    }
+};
+
+// ---- softmax ----------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float floor_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ float max_over_halves(float v) {
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+}
+__device__ __forceinline__ float sum_over_halves(float v) {
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(o[0]) + __uint_as_float(o[1]);
+}
+__device__ __forceinline__ float max_over_quarters(float v) {
+    const auto o = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return max_over_halves(fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])));
+}
+__device__ __forceinline__ float sum_over_quarters(float v) {
+    const auto o = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return sum_over_halves(__uint_as_float(o[0]) + __uint_as_float(o[1]));
+}
+
+// sum + both bf16 of a word
+__device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), sum, false);
+}
+
+// ---- partial results: device-coherent accesses, past the L2 of the XCD; a fence over all of it would cost more ----------------------
+__device__ __forceinline__ void put_pair(uint8_t *to, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(to), (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void get_pair(const uint8_t *from, float &a, float &b) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    a = __uint_as_float((uint32_t)v);
+    b = __uint_as_float((uint32_t)(v >> 32));
+}
+// Called by the whole workgroup once its partial result is on its way; true for the one that finds all the others' there.
+__device__ __forceinline__ bool last_of(const AttentionDev &p, const Piece &x, uint32_t *flag) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // this wavefront's stores have arrived
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t *counter = p.counters + x.slot;
+        const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == x.parts - 1;
+        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = last;
+    }
+    __syncthreads();
+    return *flag;
+}
+
+// LDS that lanes of one wavefront hand each other: the hardware keeps a wavefront's accesses in order, this keeps the compiler to it.
+__device__ __forceinline__ void lanes_in_order() {
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ bool not_finite(const u32x4 &v) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+    return bad;
+}
+// Exponent bytes that expand to more than a float holds: 127 x 2^(E - 127) is infinite from 249 on.
+__device__ __forceinline__ bool exponents_not_finite(const u32x4 &v) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad |= (v[i >> 2] >> (8 * (i & 3)) & 0xffu) >= 249u;
+    return bad;
+}
+
+__device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_dim) {
+    const uint32_t width = p.heads * head_dim, pieces = width / 8, from = min((uint32_t)max(p.starts[p.requests], 0), p.out_rows);
+    const uint64_t all = (uint64_t)(p.out_rows - from) * pieces;
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (uint64_t)gridDim.x * blockDim.x)
+        *reinterpret_cast<u32x4 *>(p.out + row_bytes_at(from + (uint32_t)(i / pieces), width, (uint32_t)(i % pieces) * 8, p.tiled)) = u32x4{0, 0, 0, 0};
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Few rows (decode, drafts): bound by reading the cache.  Four wavefronts share a unit of MT x 16 rows and take its 32-token blocks in
+// turn, each with softmax state of its own; they are joined at the end.  v_mfma_f32_16x16x32_bf16.
+//   keys     go from memory into the registers of the MFMA operand (16 bytes per lane, whole tiles); block floats are expanded there
+//   values   go through 32 tokens of LDS that belong to the wavefront (no barriers) for their transposition: ds_read_b64_tr_b16 for
+//            bf16; block floats as words of four columns, of which each of four products takes one byte
+// The next block is on its way, in registers, while one is worked on.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <int D, bool PACKED> struct StreamShape {
+    static constexpr int SLABS = D / 32, TILE_BYTES = PACKED ? 1088 : 2048;
+    static constexpr int COLS = PACKED ? (D + 63) / 64 * 4 : D / 16;               // accumulators of four values
+    // packed tile in LDS: [even tile 0 | odd tile 32] + face column * 528 + face row * 256 + row * 16, exponents at 1088: the words that
+    // 32 lanes read at once (2 tiles, 2 face columns, 2 groups of rows, 4 words) lie in 32 banks
+    static constexpr int STAGE = PACKED ? SLABS * 1152 : D * 64;
+    static constexpr int CHUNKS = SLABS * TILE_BYTES / 16, LOADS = (CHUNKS + 63) / 64;
+};
+template <int D, bool PACKED> struct StreamBlock {
+    using S = StreamShape<D, PACKED>;
+    u32x4 k[2][PACKED ? 1 : S::SLABS];
+    u32x2v codes[2][PACKED ? S::SLABS : 1];
+    uint32_t exps[2][PACKED ? S::SLABS : 1];
+    u32x4 v[S::LOADS];
+    __device__ __forceinline__ void load_values(const uint8_t *base, int lane) {
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i) v[i] = *reinterpret_cast<const u32x4 *>(base + min(i * 64 + lane, S::CHUNKS - 1) * 16);
+    }
+    __device__ __forceinline__ void load(const uint8_t *keys, const uint8_t *values, uint64_t tile_row, int lane) {
+        const uint64_t at = tile_row * (S::SLABS * S::TILE_BYTES);
+        const uint8_t *base = keys + at;
+        const int x = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int th = 0; th < 2; ++th)
+#pragma unroll
+            for (int s = 0; s < S::SLABS; ++s) {
+                if constexpr (PACKED) {
+                    codes[th][s] = *reinterpret_cast<const u32x2v *>(base + s * 1088 + 64 + (th * 2 + (g >> 1)) * 256 + x * 16 + (g & 1) * 8);
+                    exps[th][s] = base[s * 1088 + (th * 2 + (g >> 1)) * 16 + x];
+                } else {
+                    k[th][s] = *reinterpret_cast<const u32x4 *>(base + s * 2048 + th * 1024 + (g >> 1) * 512 + x * 32 + (g & 1) * 16);
+                }
+            }
+        load_values(values + at, lane);
+    }
+};
+
+template <int D, int MT, bool PACKED>
+__global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attention_stream_kernel(const AttentionDev p) {
+    using S = StreamShape<D, PACKED>;
+    constexpr int ROWS = MT * 16, NACC = MT * S::COLS;          // NACC quads of accumulators
+    constexpr int JOIN = 2 * (NACC * 16 + MT * 8) * 64;         // bytes: two wavefronts' state
+    constexpr int LDS = 4 * S::STAGE > JOIN ? 4 * S::STAGE : JOIN;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    __shared__ uint64_t wave_sums[4];
+    __shared__ uint32_t flag;
+    extern __shared__ uint32_t tables[];
+    const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (p.zero_rows) clear_rows(p, D);
+    const Plan plan = make_plan<256, ROWS, 4>(p, tables, tables + p.requests + 1, wave_sums);
+
+    typedef __attribute__((address_space(3))) uint8_t lds_byte;
+    lds_byte *const stage = (lds_byte *)lds + wave * S::STAGE;
+    // where this lane's pieces of a block's values go, and the token that a piece belongs to (exponents: 32 + face row * 16)
+    uint32_t to[S::LOADS], token_of[S::LOADS];
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+        const uint32_t c = i * 64 + lane;
+        if (PACKED) {
+            const uint32_t tile = c / 68, cc = c % 68, f = (cc - 4) >> 4, r = (cc - 4) & 15;
+            to[i] = tile * 1152 + (cc < 4 ? 1088 + cc * 16 : (tile & 1) * 32 + (f & 1) * 528 + (f >> 1) * 256 + r * 16);
+            token_of[i] = cc < 4 ? 32 + (cc >> 1) * 16 : (f >> 1) * 16 + r;
+        } else {
+            to[i] = c * 16;
+            token_of[i] = (c >> 6 & 1) * 16 + (c >> 1 & 15);
+        }
+    }
+    const uint32_t out_width = p.heads * D;
+
+    for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
+        const Piece pc = piece_at<ROWS>(p, plan, tables, tables + p.requests + 1, index);
+        if (pc.part >= pc.parts) continue;
+        bf16x8 q[MT][S::SLABS];
+        uint32_t row_token[MT], head[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const uint32_t rho = pc.row0 + min((uint32_t)(mt * 16 + x), pc.rows - 1);       // rows past the last repeat it
+            row_token[mt] = rho / p.group;
+            head[mt] = pc.kv * p.group + rho % p.group;
+#pragma unroll
+            for (int s = 0; s < S::SLABS; ++s) {
+                u32x4 w = *reinterpret_cast<const u32x4 *>(p.rows + row_bytes_at(pc.q.start + row_token[mt], p.width, p.query_column + head[mt] * D + s * 32 + g * 8, p.tiled));
+                q[mt][s] = __builtin_bit_cast(bf16x8, w ^ u32x4{p.flip, p.flip, p.flip, p.flip});
+            }
+        }
+        f32x4 acc[MT][S::COLS];
+        float m[MT], l[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt] = -INFINITY; l[mt] = 0.f;
+#pragma unroll
+            for (int c = 0; c < S::COLS; ++c) acc[mt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        const uint32_t pos_min = pc.q.cached + pc.token0, pos_max = pc.q.cached + pc.token1;
+        const uint32_t first_min = first_seen(p, pos_min), first_max = first_seen(p, pos_max);
+
+        // values of a block into LDS, zeros for the tokens outside [low, high]; true (wavefront) where one that stays is not finite
+        auto put_values = [&](const u32x4 (&v)[S::LOADS], uint32_t token0, uint32_t low, uint32_t high, bool look) __attribute__((always_inline)) {
+            const bool whole = token0 >= low && token0 + 31 <= high;
+            bool bad = false;
+            lanes_in_order();
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) {
+                u32x4 w = v[i];
+                if (!whole || look) {
+                    if (PACKED && token_of[i] >= 32) {
+#pragma unroll
+                        for (int b = 0; b < 16; ++b) {
+                            const uint32_t t = token0 + token_of[i] - 32 + b;
+                            if (t < low || t > high) w[b >> 2] &= ~(0xffu << (8 * (b & 3)));
+                        }
+                        if (look) bad |= exponents_not_finite(w);
+                    } else {
+                        const uint32_t t = token0 + token_of[i];
+                        if (t < low || t > high) w = u32x4{0, 0, 0, 0};
+                        if (look && !PACKED) bad |= not_finite(w);
+                    }
+                }
+                if (i + 1 < S::LOADS || S::CHUNKS % 64 == 0 || i * 64 + lane < S::CHUNKS) *(__attribute__((address_space(3))) u32x4 *)(stage + to[i]) = w;
+            }
+            lanes_in_order();
+            return look && __ballot(bad) != 0;
+        };
+        // acc += values . weights for the rows with `only`'s token, or all
+        auto add_values = [&](const bf16x8 (&w)[MT], uint32_t only, auto all) __attribute__((always_inline)) {
+            constexpr bool ALL = decltype(all)::value;
+            auto product = [&](const bf16x8 v, int c) __attribute__((always_inline)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[mt], acc[mt][c], 0, 0, 0);
+                    if (ALL || row_token[mt] == only) acc[mt][c] = sum;
+                }
+            };
+            if constexpr (PACKED) {
+#pragma unroll
+                for (int grp = 0; grp < S::COLS / 4; ++grp) {
+                    const int tile = min(grp * 2 + (x >> 3), S::SLABS - 1);                  // columns past the head: any, not stored
+                    lds_byte *const at = stage + tile * 1152, *const face = at + (tile & 1) * 32 + (x >> 2 & 1) * 528 + g * 64 + (x & 3) * 4;
+                    uint32_t words[8], mags[8];
+                    float scale[8];
+#pragma unroll
+                    for (int th = 0; th < 2; ++th) {
+                        const uint32_t e = *(__attribute__((address_space(3))) uint32_t *)(at + 1088 + (th * 2 + (x >> 2 & 1)) * 16 + g * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            words[th * 4 + i] = *(__attribute__((address_space(3))) uint32_t *)(face + th * 256 + i * 16);
+                            mags[th * 4 + i] = words[th * 4 + i] & 0x7f7f7f7fu;
+                            scale[th * 4 + i] = row_scale(e >> (8 * i) & 0xffu);
+                        }
+                    }
+                    product(weights_operand8<0>(words, mags, scale), grp * 4 + 0);
+                    product(weights_operand8<1>(words, mags, scale), grp * 4 + 1);
+                    product(weights_operand8<2>(words, mags, scale), grp * 4 + 2);
+                    product(weights_operand8<3>(words, mags, scale), grp * 4 + 3);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < S::COLS; ++c) {
+                    union { s16x4 half[2]; bf16x8 v; } u;
+#pragma unroll
+                    for (int th = 0; th < 2; ++th)
+                        u.half[th] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(stage + (c >> 1) * 2048 + th * 1024 + (c & 1) * 512 + lane * 8));
+                    product(u.v, c);
+                }
+            }
+        };
+        auto work_on = [&](StreamBlock<D, PACKED> &b, uint32_t block, uint64_t tile_row) __attribute__((always_inline)) {
+            const uint32_t token0 = block * 32;
+            const bool all_seen = token0 >= first_max && token0 + 31 <= pos_min;
+            const bool bad = put_values(b.v, token0, first_min, pos_max, !all_seen && pc.token0 != pc.token1);
+            f32x4 s[2][MT];
+#pragma unroll
+            for (int th = 0; th < 2; ++th) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[th][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int sl = 0; sl < S::SLABS; ++sl) {
+                    bf16x8 k;
+                    if constexpr (PACKED) k = __builtin_bit_cast(bf16x8, activations_operand8(b.codes[th][sl][0], b.codes[th][sl][1], b.exps[th][sl]));
+                    else k = __builtin_bit_cast(bf16x8, b.k[th][sl]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) s[th][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[mt][sl], s[th][mt], 0, 0, 0);
+                }
+            }
+            // weights of a row tile rounded to bf16, or what the rounding took off; their sum goes to l
+            auto weights = [&](int mt, bool rest) __attribute__((always_inline)) {
+                const float base = floor_of(m[mt]);
+                union { uint32_t words[4]; bf16x8 v; } u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float e[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[i >> 1][mt][(i & 1) * 2 + j], p.scale, -base));
+                    uint32_t rounded = f32x2_to_bf16x2_rne(e[0], e[1]);
+                    if (rest) rounded = f32x2_to_bf16x2_rne(e[0] - __uint_as_float(rounded << 16), e[1] - __uint_as_float(rounded & 0xffff0000u));
+                    u.words[i] = rounded;
+                    l[mt] = add_pair(rounded, l[mt]);
+                }
+                return u.v;
+            };
+            bf16x8 w[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                if (!all_seen) {
+                    const uint32_t pos = pc.q.cached + row_token[mt], first = first_seen(p, pos);
+#pragma unroll
+                    for (int th = 0; th < 2; ++th)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t t = token0 + th * 16 + g * 4 + i;
+                            if (t < first || t > pos) s[th][mt][i] = -INFINITY;
+                        }
+                }
+                float top = fmaxf(fmaxf(s[0][mt][0], s[0][mt][1]), fmaxf(s[0][mt][2], s[0][mt][3]));
+                top = fmaxf(top, fmaxf(fmaxf(s[1][mt][0], s[1][mt][1]), fmaxf(s[1][mt][2], s[1][mt][3])));
+                top = max_over_quarters(top) * p.scale;
+                if (__ballot(top > m[mt] + LAZY || (m[mt] == -INFINITY && top > m[mt]))) {
+                    const float next = fmaxf(m[mt], top), shrink = __builtin_amdgcn_exp2f(m[mt] - floor_of(next));
+                    m[mt] = next;
+                    l[mt] *= shrink;
+#pragma unroll
+                    for (int c = 0; c < S::COLS; ++c) acc[mt][c] *= shrink;
+                }
+                w[mt] = weights(mt, false);
+            }
+            if (bad) {
+                for (uint32_t t = pc.token0; t <= pc.token1; ++t) {
+                    b.load_values(p.values + tile_row * (S::SLABS * S::TILE_BYTES), lane);
+                    put_values(b.v, token0, first_seen(p, pc.q.cached + t), pc.q.cached + t, false);
+                    add_values(w, t, std::false_type{});
+                }
+            } else {
+                add_values(w, 0, std::true_type{});
+                if (token0 + 31 >= pos_min) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) w[mt] = weights(mt, true);
+                    add_values(w, 0, std::true_type{});
+                }
+            }
+        };
+
+        // ---- this wavefront's blocks: pc.begin + wave, + 4, ... ------------------------------------------------------------------
+        const uint32_t mine = pc.end > pc.begin + wave ? (pc.end - pc.begin - wave + 3) / 4 : 0;
+        Pages<4> entries;
+        StreamBlock<D, PACKED> b[2];
+        uint64_t tile_row[2];
+        bool there[2];
+        auto request = [&](int which, uint32_t i) __attribute__((always_inline)) {
+            if ((i & 63) == 0) entries.load(p, pc, pc.begin + wave + i * 4);
+            there[which] = entries.at(p, pc.kv, i & 63, tile_row[which]);
+            b[which].load(p.keys, p.values, tile_row[which], lane);
+        };
+        if (mine) request(0, 0);
+        for (uint32_t i = 0; i < mine; i += 2) {
+            if (i + 1 < mine) request(1, i + 1);
+            if (there[0]) work_on(b[0], pc.begin + wave + i * 4, tile_row[0]);
+            if (i + 1 < mine) {
+                if (i + 2 < mine) request(0, i + 2);
+                if (there[1]) work_on(b[1], pc.begin + wave + (i + 1) * 4, tile_row[1]);
+            }
+        }
+
+        // ---- join: wavefronts 2, 3 into 0, 1, then 1 into 0; afterwards wavefront 0 has it all -----------------------------------
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) l[mt] = sum_over_quarters(l[mt]);
+        auto take = [&](int mt, float m2, float l2, auto &&other) __attribute__((always_inline)) {
+            const float next = fmaxf(m[mt], m2), mine_by = __builtin_amdgcn_exp2f(m[mt] - floor_of(next)), other_by = __builtin_amdgcn_exp2f(m2 - floor_of(next));
+            m[mt] = next;
+            l[mt] = l[mt] * mine_by + l2 * other_by;
+#pragma unroll
+            for (int c = 0; c < S::COLS; ++c) acc[mt][c] = acc[mt][c] * mine_by + other(c) * other_by;
+        };
+        auto join_waves = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int half = 2; half >= 1; half >>= 1) {
+                __syncthreads();
+                float *const state = reinterpret_cast<float *>(lds) + (wave % half) * (JOIN / 8);
+                f32x4 *const quads = reinterpret_cast<f32x4 *>(state) + lane;
+                float2 *const ml = reinterpret_cast<float2 *>(state + NACC * 256) + lane;
+                if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        ml[mt * 64] = make_float2(m[mt], l[mt]);
+#pragma unroll
+                        for (int c = 0; c < S::COLS; ++c) quads[(mt * S::COLS + c) * 64] = acc[mt][c];
+                    }
+                }
+                __syncthreads();
+                if (wave < half) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        const float2 o = ml[mt * 64];
+                        take(mt, o.x, o.y, [&](int c) { return quads[(mt * S::COLS + c) * 64]; });
+                    }
+                }
+            }
+        };
+        join_waves();
+        if (pc.parts > 1) {
+            constexpr uint32_t SLOT = (NACC * 16 + MT * 8) * 64;
+            const bool fits = pc.slot + pc.parts <= p.slots;       // always, unless row_starts is out of order
+            if (wave == 0 && fits) {
+                uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + lane * 8;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    put_pair(at + mt * 512, m[mt], l[mt]);
+#pragma unroll
+                    for (int c = 0; c < S::COLS; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) put_pair(at + (MT + (mt * S::COLS + c) * 2 + h) * 512, acc[mt][c][2 * h], acc[mt][c][2 * h + 1]);
+                }
+            }
+            if (!fits || !last_of(p, pc, &flag)) { __syncthreads(); continue; }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                m[mt] = -INFINITY; l[mt] = 0.f;
+#pragma unroll
+                for (int c = 0; c < S::COLS; ++c) acc[mt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            for (uint32_t part = wave; part < pc.parts; part += 4) {
+                const uint8_t *const at = p.partial + (uint64_t)(pc.slot + part) * SLOT + lane * 8;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    float m2, l2;
+                    get_pair(at + mt * 512, m2, l2);
+                    f32x4 other[S::COLS];
+#pragma unroll
+                    for (int c = 0; c < S::COLS; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float a, b2;
+                            get_pair(at + (MT + (mt * S::COLS + c) * 2 + h) * 512, a, b2);
+                            other[c][2 * h] = a;
+                            other[c][2 * h + 1] = b2;
+                        }
+                    take(mt, m2, l2, [&](int c) { return other[c]; });
+                }
+            }
+            join_waves();
+        }
+        if (wave == 0) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                if ((uint32_t)(mt * 16 + x) >= pc.rows) continue;
+                const float by = l[mt] == 0.f ? 0.f : (PACKED ? Wfmt<7>::unscale : 1.f) / l[mt];
+                const uint32_t t = pc.q.start + row_token[mt], column = head[mt] * D;
+                if constexpr (PACKED) {
+#pragma unroll
+                    for (int grp = 0; grp < S::COLS / 4; ++grp) {
+                        const uint32_t d = grp * 64 + g * 16;      // 16 neighbouring columns: 4 i + byte
+                        if (d >= (uint32_t)D) continue;
+                        uint32_t words[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) words[2 * i + h] = f32x2_to_bf16x2_rne(acc[mt][grp * 4 + 2 * h][i] * by, acc[mt][grp * 4 + 2 * h + 1][i] * by);
+                        u32x4 *const o = reinterpret_cast<u32x4 *>(p.out + row_bytes_at(t, out_width, column + d, p.tiled));
+                        o[0] = u32x4{words[0], words[1], words[2], words[3]};
+                        o[1] = u32x4{words[4], words[5], words[6], words[7]};
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < S::COLS; ++c)
+                        *reinterpret_cast<u32x2v *>(p.out + row_bytes_at(t, out_width, column + c * 16 + g * 4, p.tiled)) =
+                            u32x2v{f32x2_to_bf16x2_rne(acc[mt][c][0] * by, acc[mt][c][1] * by), f32x2_to_bf16x2_rne(acc[mt][c][2] * by, acc[mt][c][3] * by)};
+                }
+            }
+        }
+        __syncthreads();                                        // LDS is the next piece's
     }
 }
 
-size_t paged_attention_workspace_bytes(uint32_t, uint32_t, uint32_t, const PagedCache &) { return 0; }
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Many rows (chunks, prompts): bound by the matrix cores.  Eight wavefronts of 32 rows each share a unit of 256 rows and its keys and values,
+// which go through two LDS buffers of 64 tokens (32 where heads have 256 elements) as bf16; block floats are expanded on the way,
+// once for all 256 rows.  v_mfma_f32_32x32x16_bf16.
+//   keys     16-byte chunk (row r, half h) of a face lies at r * 32 + (h ^ (r / 8)) * 16: what a pass of a ds_read_b128 touches lies
+//            in different banks
+//   values   read transposed (ds_read_b64_tr_b16); the 128-byte halves of the row groups are exchanged in the right-hand faces, for the
+//            same reason
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <int D, bool PACKED> struct TileShape {
+    static constexpr int NB = D == 256 ? 1 : 2;                 // blocks of 32 tokens per step
+    static constexpr int BLOCK = D * 64, HALF = NB * BLOCK;     // bytes of a block, and of the keys or the values of a step
+    static constexpr int TILE_BYTES = PACKED ? 1088 : 2048, ROW_BYTES = D / 32 * TILE_BYTES;
+    // pieces of a step's keys, and of its values: 16 bytes of bf16, or a face row of block floats
+    static constexpr int PIECES = PACKED ? NB * 2 * D : NB * D * 4, EACH = (PIECES + 511) / 512;
+};
+
+template <int D, bool PACKED>
+__global__ __launch_bounds__(512) void paged_attention_tile_kernel(const AttentionDev p) {
+    using S = TileShape<D, PACKED>;
+    constexpr int ROWS = 256, NB = S::NB, SLABS = D / 16, DB = D / 32;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * S::HALF];                // [buffer][keys | values]
+    __shared__ uint64_t wave_sums[8];
+    __shared__ uint32_t flag;
+    extern __shared__ uint32_t tables[];
+    const int lane = threadIdx.x & 63, c = lane & 31, kh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    typedef __attribute__((address_space(3))) uint8_t lds_byte;
+    if (p.zero_rows) clear_rows(p, D);
+    const Plan plan = make_plan<512, ROWS, NB>(p, tables, tables + p.requests + 1, wave_sums);
+    const uint32_t out_width = p.heads * D;
+
+    for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
+        const Piece pc = piece_at<ROWS>(p, plan, tables, tables + p.requests + 1, index);
+        if (pc.part >= pc.parts) continue;
+        const bool idle = (uint32_t)wave * 32 >= pc.rows;       // a wavefront without rows only moves keys and values
+        const uint32_t rho = pc.row0 + min((uint32_t)(wave * 32 + c), pc.rows - 1);
+        const uint32_t row_token = rho / p.group, head = pc.kv * p.group + rho % p.group;
+        bf16x8 q[SLABS];
+#pragma unroll
+        for (int s = 0; s < SLABS; ++s) {
+            u32x4 w = *reinterpret_cast<const u32x4 *>(p.rows + row_bytes_at(pc.q.start + row_token, p.width, p.query_column + head * D + s * 16 + kh * 8, p.tiled));
+            q[s] = __builtin_bit_cast(bf16x8, w ^ u32x4{p.flip, p.flip, p.flip, p.flip});
+        }
+        f32x16 acc[DB];
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+        const uint32_t pos = pc.q.cached + row_token, first = first_seen(p, pos);
+        // tokens that some row, and that every row, sees: of the unit and of this wavefront
+        const uint32_t pos_max = pc.q.cached + pc.token1, first_min = first_seen(p, pc.q.cached + pc.token0);
+        const uint32_t unit_pos_min = pc.q.cached + pc.token0, unit_first_max = first_seen(p, pos_max);
+        const uint32_t wave_pos_min = pc.q.cached + (pc.row0 + min((uint32_t)wave * 32, pc.rows - 1)) / p.group, wave_pos_max = pc.q.cached + (pc.row0 + min((uint32_t)wave * 32 + 31, pc.rows - 1)) / p.group;
+        const uint32_t wave_first_min = first_seen(p, wave_pos_min), wave_first_max = first_seen(p, wave_pos_max);
+
+        Pages<1> entries;
+        u32x4 kreg[S::EACH], vreg[S::EACH];
+        uint32_t kexp[S::EACH], vexp[S::EACH];
+        // piece i of this thread: block of the step, byte in the block's tiles (keys and values alike), token of the block
+        auto place = [&](int i, uint32_t &block, uint32_t &from, uint32_t &token, uint32_t &exponent) __attribute__((always_inline)) {
+            const uint32_t n = min(threadIdx.x + i * 512u, (uint32_t)S::PIECES - 1), per_block = S::PIECES / NB;
+            block = n / per_block;
+            const uint32_t within = n % per_block;
+            if (PACKED) {
+                const uint32_t tile = within >> 6, face = within >> 4 & 3, r = within & 15;
+                from = tile * 1088 + 64 + face * 256 + r * 16;
+                exponent = tile * 1088 + face * 16 + r;
+                token = (face >> 1) * 16 + r;
+            } else {
+                from = within * 16;
+                exponent = 0;
+                token = (within >> 6 & 1) * 16 + (within >> 1 & 15);
+            }
+        };
+        uint64_t rows_of[NB];
+        bool there[NB], ready[NB];                              // of the step that is loaded, and of the one that lies in LDS
+        auto load = [&](const uint8_t *tensor, u32x4 (&v)[S::EACH], uint32_t (&e)[S::EACH]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < S::EACH; ++i) {
+                uint32_t block, from, token, exponent;
+                place(i, block, from, token, exponent);
+                const uint8_t *base = tensor + (NB == 2 && block ? rows_of[NB - 1] : rows_of[0]) * S::ROW_BYTES;
+                v[i] = *reinterpret_cast<const u32x4 *>(base + from);
+                e[i] = PACKED ? base[exponent] : 0u;
+            }
+        };
+        auto request = [&](uint32_t step) __attribute__((always_inline)) {
+            const uint32_t i = step * NB;
+            if ((i & 63) == 0) entries.load(p, pc, pc.begin + i);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) there[b] = entries.at(p, pc.kv, (i + b) & 63, rows_of[b]);
+            load(p.keys, kreg, kexp);
+            load(p.values, vreg, vexp);
+        };
+        // Keys and values, or the values alone, of the loaded step into LDS; values outside [low, high], or without a page, as zeros.  True where one
+        // that stays is not finite.
+        auto put = [&](uint32_t buffer, uint32_t token0, uint32_t low, uint32_t high, const bool (&pages)[NB], bool keys, bool look) __attribute__((always_inline)) {
+            lds_byte *const to = (lds_byte *)lds + buffer * 2 * S::HALF;
+            const bool whole = token0 >= low && token0 + NB * 32 - 1 <= high && pages[0] && pages[NB - 1];
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < S::EACH; ++i) {
+                if (S::PIECES % 512 && threadIdx.x + i * 512u >= (uint32_t)S::PIECES) break;
+                uint32_t block, from, token, exponent;
+                place(i, block, from, token, exponent);
+                const uint32_t t = token0 + block * 32 + token;
+                const bool gone = !whole && (t < low || t > high || !(NB == 2 && block ? pages[NB - 1] : pages[0]));
+                const uint32_t within = (threadIdx.x + i * 512u) % (S::PIECES / NB);
+                if constexpr (PACKED) {
+                    const uint32_t tile = within >> 6, face = within >> 4 & 3, r = within & 15;
+                    const uint32_t base = block * S::BLOCK + tile * 2048 + face * 512;
+                    if (look && !gone) bad |= vexp[i] >= 249u;
+                    const uint32_t ve = gone ? 0u : vexp[i];
+                    const u32x4 vc = gone ? u32x4{0, 0, 0, 0} : vreg[i];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (keys) *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + ((h ^ (r >> 3)) * 16)) = activations_operand8(kreg[i][2 * h], kreg[i][2 * h + 1], kexp[i]);
+                        *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + (((r * 2 + h) ^ ((face & 1) * 8)) * 16)) = activations_operand8(vc[2 * h], vc[2 * h + 1], ve);
+                    }
+                } else {
+                    const uint32_t face = within >> 5 & 3, in_face = within & 31, r = in_face >> 1;
+                    const uint32_t base = block * S::BLOCK + (within >> 5) * 512;
+                    const u32x4 v = gone ? u32x4{0, 0, 0, 0} : vreg[i];
+                    if (look) bad |= not_finite(v);
+                    if (keys) *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + (((in_face & 1) ^ (r >> 3)) * 16)) = kreg[i];
+                    *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + ((in_face ^ ((face & 1) * 8)) * 16)) = v;
+                }
+            }
+            return bad;
+        };
+
+        const uint32_t steps = (pc.end - pc.begin + NB - 1) / NB;
+        bool bad = false;
+        // rows of the unit see different parts of the step: values that are not finite have to be looked for
+        auto uneven = [&](uint32_t token0) { return pc.token0 != pc.token1 && !(token0 >= unit_first_max && token0 + NB * 32 - 1 <= unit_pos_min); };
+        auto fill = [&](uint32_t step) __attribute__((always_inline)) {
+            const uint32_t token0 = (pc.begin + step * NB) * 32;
+            const bool look = uneven(token0);
+            const bool mine = put(step & 1, token0, first_min, pos_max, there, true, look);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) ready[b] = there[b];
+            if (look) bad = __syncthreads_or(mine);
+            else { bad = false; __syncthreads(); }
+        };
+        if (steps) {
+            request(0);
+            fill(0);
+        }
+        const uint32_t key_at = (c >> 4) * 1024 + (c & 15) * 32 + ((kh ^ (c >> 3 & 1)) * 16);                     // + slab
+        const uint32_t fc = lane >> 4 & 1, value_at = S::HALF + fc * 512 + ((kh * 128 + (lane & 15) * 8) ^ (fc * 128));
+        for (uint32_t step = 0; step < steps; ++step) {
+            if (step + 1 < steps) request(step + 1);
+            const uint32_t token0 = (pc.begin + step * NB) * 32, last = token0 + NB * 32 - 1;
+            lds_byte *const from = (lds_byte *)lds + (step & 1) * 2 * S::HALF;
+            const bool skip = idle || token0 > wave_pos_max || last < wave_first_min;
+            bf16x8 w[NB][2];
+            f32x16 s[NB];
+            // weights rounded to bf16, or what the rounding took off; their sum goes to l
+            auto weights = [&](bool rest) __attribute__((always_inline)) {
+                const float base = floor_of(m);
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        union { uint32_t words[4]; bf16x8 v; } u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float e[2];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[b][h * 8 + 2 * i + j], p.scale, -base));
+                            uint32_t rounded = f32x2_to_bf16x2_rne(e[0], e[1]);
+                            if (rest) rounded = f32x2_to_bf16x2_rne(e[0] - __uint_as_float(rounded << 16), e[1] - __uint_as_float(rounded & 0xffff0000u));
+                            u.words[i] = rounded;
+                            l = add_pair(rounded, l);
+                        }
+                        w[b][h] = u.v;
+                    }
+            };
+            if (!skip) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+                    for (int sl = 0; sl < SLABS; ++sl) {
+                        const u32x4 k = *(__attribute__((address_space(3))) u32x4 *)(from + key_at + b * S::BLOCK + (sl >> 1) * 2048 + (sl & 1) * 512);
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k), q[sl], s[b], 0, 0, 0);
+                    }
+                }
+                if (!(token0 >= wave_first_max && last <= wave_pos_min && ready[0] && ready[NB - 1])) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint32_t t = token0 + b * 32 + (i >> 2) * 8 + kh * 4 + (i & 3);
+                            if (t < first || t > pos || !ready[b]) s[b][i] = -INFINITY;
+                        }
+                }
+                float top = s[0][0];
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+                top = max_over_halves(top) * p.scale;
+                if (__ballot(top > m + LAZY || (m == -INFINITY && top > m))) {
+                    const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - floor_of(next));
+                    m = next;
+                    l *= shrink;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] *= shrink;
+                }
+                weights(false);
+            }
+            // acc += values . weights for the rows with `only`'s token, or all
+            auto add_values = [&](uint32_t only, auto all) __attribute__((always_inline)) {
+                constexpr bool ALL = decltype(all)::value;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    f32x16 sum = acc[d];
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            union { s16x4 half[2]; bf16x8 v; } u;
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                u.half[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(from + value_at + b * S::BLOCK + d * 2048 + h * 1024 + r * 256));
+                            sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, w[b][h], sum, 0, 0, 0);
+                        }
+                    if (ALL || row_token == only) acc[d] = sum;
+                }
+            };
+            if (!bad) {
+                if (!skip) {
+                    add_values(0, std::true_type{});
+                    if (last >= wave_pos_min) {
+                        weights(true);
+                        add_values(0, std::true_type{});
+                    }
+                }
+            } else {
+                // the step behind this one waits in registers, and is loaded again afterwards
+                bool mine[NB];
+                uint64_t rows_next[NB];
+                bool there_next[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    mine[b] = ready[b]; rows_next[b] = rows_of[b]; there_next[b] = there[b];
+                    const uint32_t block = pc.begin + step * NB + b;
+                    int32_t page = block < pc.end ? p.table[(uint64_t)pc.r * p.max_pages + block / p.page_blocks] : -1;
+                    if ((uint32_t)page >= p.pages) page = 0;
+                    rows_of[b] = ((uint64_t)page * p.kv_heads + pc.kv) * p.page_blocks + block % p.page_blocks;
+                }
+                for (uint32_t t = pc.token0; t <= pc.token1; ++t) {
+                    load(p.values, vreg, vexp);
+                    __syncthreads();
+                    put(step & 1, token0, first_seen(p, pc.q.cached + t), pc.q.cached + t, mine, false, false);
+                    __syncthreads();
+                    if (!skip) add_values(t, std::false_type{});
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) { rows_of[b] = rows_next[b]; there[b] = there_next[b]; }
+                if (step + 1 < steps) load(p.values, vreg, vexp);
+            }
+            if (step + 1 < steps) fill(step + 1);
+        }
+
+        l = sum_over_halves(l);
+        if (pc.parts > 1) {
+            constexpr uint32_t PART = (DB * 8 + 1) * 512, SLOT = 8 * PART;             // of a wavefront, of a workgroup
+            const bool fits = pc.slot + pc.parts <= p.slots;   // always, unless row_starts is out of order
+            if (fits && !idle) {
+                uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + wave * PART + lane * 8;
+                put_pair(at, m, l);
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) put_pair(at + (1 + d * 8 + i) * 512, acc[d][2 * i], acc[d][2 * i + 1]);
+            }
+            if (!fits || !last_of(p, pc, &flag)) { __syncthreads(); continue; }
+            m = -INFINITY; l = 0.f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+            for (uint32_t part = 0; part < (idle ? 0 : pc.parts); ++part) {
+                const uint8_t *const at = p.partial + (uint64_t)(pc.slot + part) * SLOT + wave * PART + lane * 8;
+                float m2, l2;
+                get_pair(at, m2, l2);
+                const float next = fmaxf(m, m2), by = __builtin_amdgcn_exp2f(m - floor_of(next)), by2 = __builtin_amdgcn_exp2f(m2 - floor_of(next));
+                m = next;
+                l = l * by + l2 * by2;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float a, b;
+                        get_pair(at + (1 + d * 8 + i) * 512, a, b);
+                        acc[d][2 * i] = acc[d][2 * i] * by + a * by2;
+                        acc[d][2 * i + 1] = acc[d][2 * i + 1] * by + b * by2;
+                    }
+            }
+        }
+        // columns 8 (i / 4) + 4 kh + i % 4 of 32: the swap leaves columns 8 kh .. 8 kh + 7 of a face row in each lane
+        const float by = l == 0.f ? 0.f : (PACKED ? Wfmt<7>::unscale : 1.f) / l;
+        const bool stored = (uint32_t)(wave * 32 + c) < pc.rows;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int i = f * 8;
+                const auto w0 = __builtin_amdgcn_permlane32_swap(f32x2_to_bf16x2_rne(acc[d][i] * by, acc[d][i + 1] * by), f32x2_to_bf16x2_rne(acc[d][i + 4] * by, acc[d][i + 5] * by), false, false);
+                const auto w1 = __builtin_amdgcn_permlane32_swap(f32x2_to_bf16x2_rne(acc[d][i + 2] * by, acc[d][i + 3] * by), f32x2_to_bf16x2_rne(acc[d][i + 6] * by, acc[d][i + 7] * by), false, false);
+                if (stored) *reinterpret_cast<u32x4 *>(p.out + row_bytes_at(pc.q.start + row_token, out_width, head * D + d * 32 + f * 16 + kh * 8, p.tiled)) = u32x4{w0[0], w1[0], w0[1], w1[1]};
+            }
+        __syncthreads();                                        // LDS is the next piece's
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------
+namespace {
+// Which kernels a step needs: the lengths are on the device, the host knows how many tokens there are for how many requests.
+struct Route {
+    uint32_t mt = 0;                       // row tiles of the kernel for few rows; 0: not launched
+    bool tile = false;
+    uint32_t stream_target = 1024, tile_target = 512;
+    size_t slot_bytes = 0, slots = 0;
+};
+Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCache &c) {
+    Route r;
+    const uint32_t group = heads / c.kv_heads;
+    const uint64_t rows = (uint64_t)((tokens + requests - 1) / std::max(requests, 1u)) * group;       // of an average request
+    const uint32_t most = c.head_dim == 64 ? 5 : c.head_dim == 256 ? 2 : 4;
+    const uint64_t wanted = (std::max<uint64_t>(rows, 1) + 15) / 16;
+    r.mt = wanted <= 1 ? 1 : wanted <= 2 ? 2 : most;
+    const bool few = (uint64_t)tokens <= 8ull * requests || (uint64_t)tokens * group <= r.mt * 16, many = rows >= 256;
+    r.tile = !few;
+    if (many) r.mt = 0;
+    if (requests == 1) {                   // its length is known
+        r.tile = rows > most * 16;
+        if (r.tile) r.mt = 0;
+    }
+    const bool packed = c.dtype == TTMI_BFLOAT8_B;
+    if (r.mt) {
+        const size_t cols = packed ? (c.head_dim + 63) / 64 * 4 : c.head_dim / 16;
+        r.slot_bytes = (r.mt * cols * 16 + r.mt * 8) * 64;
+        r.slots = 2 * (size_t)r.stream_target * r.slot_bytes;
+    }
+    if (r.tile) r.slots = std::max(r.slots, 2 * (size_t)r.tile_target * 8 * ((size_t)c.head_dim / 32 * 8 + 1) * 512);
+    return r;
+}
+
+__global__ void clear_counters_kernel(uint32_t *counters) { counters[blockIdx.x * 256 + threadIdx.x] = 0; }
+int clear_counters(void *at, hipStream_t st) {
+    hipLaunchKernelGGL(clear_counters_kernel, dim3(COUNTERS / 256), dim3(256), 0, st, (uint32_t *)at);
+    return check_launch("clear_counters_kernel");
+}
+
+template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, uint32_t blocks, size_t lds, hipStream_t st) {
+    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(blocks), dim3(256), lds, st, p);
+    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(blocks), dim3(256), lds, st, p);
+}
+template <int D, int MOST> void launch_stream(const AttentionDev &p, uint32_t mt, bool packed, size_t lds, hipStream_t st) {
+    if (mt == 1) launch_stream<D, 1>(p, packed, 512, lds, st);
+    else if (mt == 2) launch_stream<D, 2>(p, packed, 512, lds, st);
+    else launch_stream<D, MOST>(p, packed, 512, lds, st);
+}
+template <int D> void launch_tile(const AttentionDev &p, bool packed, size_t lds, hipStream_t st) {
+    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(256), dim3(512), lds, st, p);
+    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(256), dim3(512), lds, st, p);
+}
+}  // namespace
+
+size_t paged_attention_workspace_bytes(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCache &cache) {
+    return COUNTERS * 4 + route_of(tokens, requests, heads, cache).slots;
+}
 
 int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
-    const uint32_t rows = x.rows.layout == TTMI_TILE ? (x.rows.tokens + 31) / 32 * 32 : x.rows.tokens;
-    if (!rows) return TTMI_OK;
+    const PagedCache &c = x.cache;
     AttentionDev p{};
     p.rows = (const uint8_t *)x.rows.data; p.keys = (const uint8_t *)x.key_cache; p.values = (const uint8_t *)x.value_cache;
     p.table = x.step.page_table; p.cached = x.step.cached; p.starts = x.step.row_starts; p.out = (uint8_t *)x.out;
-    p.tokens = x.rows.tokens; p.width = x.rows.width; p.query_column = x.query_column; p.requests = x.step.requests; p.max_pages = x.step.max_pages;
-    p.pages = x.cache.pages; p.kv_heads = x.cache.kv_heads; p.page_size = x.cache.page_size; p.head_dim = x.cache.head_dim;
-    p.heads = x.heads; p.group = x.heads / x.cache.kv_heads; p.window = x.window;
-    p.scale = x.scale * 1.4426950408889634f;
-    p.tiled = x.rows.layout == TTMI_TILE; p.packed = x.cache.dtype == TTMI_BFLOAT8_B;
-    hipLaunchKernelGGL(paged_attention_rows_kernel, dim3(rows * x.heads), dim3(64), 0, st, p);
-    return check_launch("paged_attention_rows_kernel");
+    p.tiled = x.rows.layout == TTMI_TILE;
+    p.tokens = x.rows.tokens; p.out_rows = p.tiled ? (x.rows.tokens + 31) / 32 * 32 : x.rows.tokens;
+    if (!p.out_rows) return TTMI_OK;
+    p.width = x.rows.width; p.query_column = x.query_column; p.requests = x.step.requests; p.max_pages = x.step.max_pages;
+    p.pages = c.pages; p.kv_heads = c.kv_heads; p.page_blocks = c.page_size / 32;
+    p.heads = x.heads; p.group = x.heads / c.kv_heads; p.window = x.window;
+    const bool packed = c.dtype == TTMI_BFLOAT8_B;
+    // a scale of zero stands for one that no score survives: -inf, what is masked, has to stay -inf
+    p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 1e-30f) * (packed ? Wfmt<7>::unscale : 1.f);
+    p.flip = x.scale < 0.f ? 0x80008000u : 0u;
+
+    const Route route = route_of(p.tokens, p.requests, p.heads, c);
+    const size_t bytes = COUNTERS * 4 + route.slots;
+    uint8_t *memory = (uint8_t *)x.workspace;
+    static std::mutex fresh_guard;         // another thread's launch on this stream stays behind the clearing of a new buffer
+    if (memory) {
+        if (int rc = clear_counters(memory, st)) return rc;
+    } else {
+        std::lock_guard<std::mutex> lock(fresh_guard);
+        if (stream_is_capturing(st) && !scratch_held(SCRATCH_PAGED, st, bytes))
+            return fail(TTMI_ERR_UNSUPPORTED, "paged attention: a captured call cannot allocate its %zu bytes of scratch: make one on this stream before the capture, or bring a workspace", bytes);
+        bool fresh = false;
+        if (int rc = scratch_get(SCRATCH_PAGED, st, bytes, (void **)&memory, &fresh)) return rc;
+        if (fresh)
+            if (int rc = clear_counters(memory, st)) return rc;
+    }
+    p.counters = (uint32_t *)memory;
+    p.partial = memory + COUNTERS * 4;
+    p.zero_rows = 1;
+    const size_t lds = (2 * (size_t)p.requests + 1) * 4;
+    if (route.mt) {
+        p.least_rows = 1;
+        p.most_rows = route.tile ? route.mt * 16 : 0xffffffffu;
+        p.target = route.stream_target; p.slots = 2 * p.target;
+        switch (c.head_dim) {
+            case 64: launch_stream<64, 5>(p, route.mt, packed, lds, st); break;
+            case 96: launch_stream<96, 4>(p, route.mt, packed, lds, st); break;
+            case 128: launch_stream<128, 4>(p, route.mt, packed, lds, st); break;
+            default: launch_stream<256, 2>(p, route.mt, packed, lds, st); break;
+        }
+        if (int rc = check_launch("paged_attention_stream_kernel")) return rc;
+        p.zero_rows = 0;
+    }
+    if (route.tile) {
+        p.least_rows = route.mt ? route.mt * 16 + 1 : 1;
+        p.most_rows = 0xffffffffu;
+        p.target = route.tile_target; p.slots = 2 * p.target;
+        switch (c.head_dim) {
+            case 64: launch_tile<64>(p, packed, lds, st); break;
+            case 96: launch_tile<96>(p, packed, lds, st); break;
+            case 128: launch_tile<128>(p, packed, lds, st); break;
+            default: launch_tile<256>(p, packed, lds, st); break;
+        }
+        if (int rc = check_launch("paged_attention_tile_kernel")) return rc;
+    }
+    return TTMI_OK;
 }
 
 }  // namespace ttmi
