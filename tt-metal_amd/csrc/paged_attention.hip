@@ -22,9 +22,10 @@
 //              was multiplied with, so a row of one token is that token's value (v_dot2_f32_bf16 adds two at a time).  Rows of
 //              few tokens have no others for the roundings to cancel against: in the block where a row ends what the rounding
 //              took off is a second product
-//   masks      a score that does not count becomes -inf.  Values that no row of the unit sees (behind the last token, before the
-//              window) are zeroed on their way into LDS: 0 x NaN is NaN.  Where rows of a unit see different tokens and one of
-//              them is not finite, the product is made token by token of the unit, each time with the values that it sees
+//   masks      a score that does not count becomes -inf, its weight 0.  bf16 values that no row of the unit sees (behind the last token,
+//              before the window) are zeroed on their way into LDS: 0 x NaN is NaN.  Where rows of a unit see different tokens,
+//              values that are not finite are taken out as well, and two products with ones in their places say which rows
+//              see them.  Block floats are always finite here: see block_scale
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -50,10 +51,10 @@ struct AttentionDev {
     uint32_t tokens, out_rows, width, query_column, requests, max_pages;
     uint32_t pages, kv_heads, page_blocks, heads, group, window;
     uint32_t least_rows, most_rows;        // requests of that many rows per key head are this launch's
-    uint32_t target, slots;                // pieces aimed at; partial results that fit
+    uint32_t target, slots;                // workgroups that are resident at once; partial results that fit
     uint32_t *counters;                    // pieces of a unit that are done, by the unit's first slot; all zero between launches
     uint8_t *partial;
-    float scale;                           // |scale| log2(e), and what block floats are too large by
+    float scale;                           // |scale| log2(e)
     uint32_t flip;                         // sign bits of the queries, for a negative scale
     int tiled, zero_rows;                  // zero_rows: this launch clears the rows of no request
 };
@@ -111,13 +112,16 @@ struct Plan { uint32_t piece, pieces; };   // blocks of a piece, pieces of the s
 // first_piece[requests + 1], first_slot[requests]: LDS
 template <int THREADS, int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const AttentionDev &p, uint32_t *first_piece, uint32_t *first_slot, uint64_t *wave_sums) {
     const uint32_t each = (p.requests + THREADS - 1) / THREADS, r0 = min(threadIdx.x * each, p.requests), r1 = min(r0 + each, p.requests);
-    uint64_t work = 0, all;
+    uint64_t work = 0, units = 0, all, all_units;
     for (uint32_t r = r0; r < r1; ++r) {
         const Extent<ROWS> e(p, request_at(p, r));
         work += (uint64_t)e.units * e.blocks;
+        units += e.units;
     }
     scan<THREADS>(work, wave_sums, all);
-    const uint64_t share = (all + p.target - 1) / p.target;
+    scan<THREADS>(units, wave_sums, all_units);
+    // the last piece of a unit is on average half a piece: that many more come to about one for each resident workgroup
+    const uint64_t aim = max((uint64_t)p.target - min(all_units / 2, (uint64_t)p.target), (uint64_t)p.target / 4), share = (all + aim - 1) / aim;
     const uint32_t piece = (uint32_t)(max(share, (uint64_t)1) + STEP - 1) / STEP * STEP;
     uint64_t pieces = 0, slots = 0;        // of this lane's requests: pieces, and those of units with more than one, together in one scan
     for (uint32_t r = r0; r < r1; ++r) {
@@ -250,18 +254,23 @@ __device__ __forceinline__ void lanes_in_order() {
     asm volatile("" ::: "memory");
 }
 
-__device__ __forceinline__ bool not_finite(const u32x4 &v) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
-    return bad;
+// bf16 values that are not finite.  KEEP_FINITE: zeros in their places; ONES_UP, ONES_DOWN: ones where adding the value would add +inf or
+// NaN, or -inf or NaN, zeros elsewhere (a NaN is both: inf - inf).
+enum Pick { KEEP_FINITE, ONES_UP, ONES_DOWN };
+__device__ __forceinline__ uint32_t pick(uint32_t v, Pick how) {            // two values
+    const uint32_t size = v & 0x7fff7fffu, gone = (size + 0x00800080u) & 0x80008000u, nan = size + 0x007f007fu;     // bit 15 of each half
+    if (how == KEEP_FINITE) return v & ~((gone >> 15) * 0xffffu);
+    return ((gone & (nan | (how == ONES_DOWN ? v : ~v))) >> 15) * 0x3f80u;
 }
-// Exponent bytes that expand to more than a float holds: 127 x 2^(E - 127) is infinite from 249 on.
-__device__ __forceinline__ bool exponents_not_finite(const u32x4 &v) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad |= (v[i >> 2] >> (8 * (i & 3)) & 0xffu) >= 249u;
-    return bad;
+__device__ __forceinline__ u32x4 pick(u32x4 v, Pick how) { return u32x4{pick(v[0], how), pick(v[1], how), pick(v[2], how), pick(v[3], how)}; }
+
+// What a mantissa of 1 stands for in a face row of block floats: 2^(E - 133), as a float.  The exponent byte of a row that infinities or
+// NaN were written into, 255, is read as 254, so that every value is finite; below 7 (numbers under 2^-119) it is read as 7.
+__device__ __forceinline__ float block_scale(uint32_t e) { return __uint_as_float((min(max(e, 7u), 254u) - 6u) << 23); }
+// eight block floats of a face row as bf16, exactly
+__device__ __forceinline__ u32x4 expand8(uint32_t w0, uint32_t w1, float scale) {
+    const uint32_t m0 = w0 & 0x7f7f7f7fu, m1 = w1 & 0x7f7f7f7fu;
+    return u32x4{activations_pair<0>(w0, m0, scale), activations_pair<2>(w0, m0, scale), activations_pair<0>(w1, m1, scale), activations_pair<2>(w1, m1, scale)};
 }
 
 __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_dim) {
@@ -277,7 +286,7 @@ __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_
 //   keys     go from memory into the registers of the MFMA operand (16 bytes per lane, whole tiles); block floats are expanded there
 //   values   go through 32 tokens of LDS that belong to the wavefront (no barriers) for their transposition: ds_read_b64_tr_b16 for
 //            bf16; block floats as words of four columns, of which each of four products takes one byte
-// The next block is on its way, in registers, while one is worked on.
+// The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int D, bool PACKED> struct StreamShape {
     static constexpr int SLABS = D / 32, TILE_BYTES = PACKED ? 1088 : 2048;
@@ -333,19 +342,11 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
 
     typedef __attribute__((address_space(3))) uint8_t lds_byte;
     lds_byte *const stage = (lds_byte *)lds + wave * S::STAGE;
-    // where this lane's pieces of a block's values go, and the token that a piece belongs to (exponents: 32 + face row * 16)
-    uint32_t to[S::LOADS], token_of[S::LOADS];
+    uint32_t to[S::LOADS];                                      // where this lane's pieces of a block's values go
 #pragma unroll
-    for (int i = 0; i < S::LOADS; ++i) {
-        const uint32_t c = i * 64 + lane;
-        if (PACKED) {
-            const uint32_t tile = c / 68, cc = c % 68, f = (cc - 4) >> 4, r = (cc - 4) & 15;
-            to[i] = tile * 1152 + (cc < 4 ? 1088 + cc * 16 : (tile & 1) * 32 + (f & 1) * 528 + (f >> 1) * 256 + r * 16);
-            token_of[i] = cc < 4 ? 32 + (cc >> 1) * 16 : (f >> 1) * 16 + r;
-        } else {
-            to[i] = c * 16;
-            token_of[i] = (c >> 6 & 1) * 16 + (c >> 1 & 15);
-        }
+    for (int n = 0; n < S::LOADS; ++n) {
+        const uint32_t c = n * 64 + lane, tile = c / 68, cc = c % 68, f = (cc - 4) >> 4, r = (cc - 4) & 15;
+        to[n] = !PACKED ? c * 16 : tile * 1152 + (cc < 4 ? 1088 + cc * 16 : (tile & 1) * 32 + (f & 1) * 528 + (f >> 1) * 256 + r * 16);
     }
     const uint32_t out_width = p.heads * D;
 
@@ -376,42 +377,34 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
         const uint32_t pos_min = pc.q.cached + pc.token0, pos_max = pc.q.cached + pc.token1;
         const uint32_t first_min = first_seen(p, pos_min), first_max = first_seen(p, pos_max);
 
-        // values of a block into LDS, zeros for the tokens outside [low, high]; true (wavefront) where one that stays is not finite
-        auto put_values = [&](const u32x4 (&v)[S::LOADS], uint32_t token0, uint32_t low, uint32_t high, bool look) __attribute__((always_inline)) {
-            const bool whole = token0 >= low && token0 + 31 <= high;
-            bool bad = false;
+        // values of a block into LDS
+        auto put_values = [&](const u32x4 (&v)[S::LOADS]) __attribute__((always_inline)) {
             lanes_in_order();
 #pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) {
-                u32x4 w = v[i];
-                if (!whole || look) {
-                    if (PACKED && token_of[i] >= 32) {
-#pragma unroll
-                        for (int b = 0; b < 16; ++b) {
-                            const uint32_t t = token0 + token_of[i] - 32 + b;
-                            if (t < low || t > high) w[b >> 2] &= ~(0xffu << (8 * (b & 3)));
-                        }
-                        if (look) bad |= exponents_not_finite(w);
-                    } else {
-                        const uint32_t t = token0 + token_of[i];
-                        if (t < low || t > high) w = u32x4{0, 0, 0, 0};
-                        if (look && !PACKED) bad |= not_finite(w);
-                    }
-                }
-                if (i + 1 < S::LOADS || S::CHUNKS % 64 == 0 || i * 64 + lane < S::CHUNKS) *(__attribute__((address_space(3))) u32x4 *)(stage + to[i]) = w;
-            }
+            for (int n = 0; n < S::LOADS; ++n)
+                if (n + 1 < S::LOADS || S::CHUNKS % 64 == 0 || n * 64 + lane < S::CHUNKS) *(__attribute__((address_space(3))) u32x4 *)(stage + to[n]) = v[n];
             lanes_in_order();
-            return look && __ballot(bad) != 0;
         };
-        // acc += values . weights for the rows with `only`'s token, or all
-        auto add_values = [&](const bf16x8 (&w)[MT], uint32_t only, auto all) __attribute__((always_inline)) {
-            constexpr bool ALL = decltype(all)::value;
+        // bf16 values: zeros for the tokens outside [low, high]
+        auto clear_values = [&](u32x4 (&v)[S::LOADS], uint32_t token0, uint32_t low, uint32_t high) __attribute__((always_inline)) {
+#pragma unroll
+            for (int n = 0; n < S::LOADS; ++n) {
+                const uint32_t c = n * 64 + lane, t = token0 + (c >> 6 & 1) * 16 + (c >> 1 & 15);
+                if (t < low || t > high) v[n] = u32x4{0, 0, 0, 0};
+            }
+        };
+        auto value_operand = [&](int c) __attribute__((always_inline)) {
+            union { s16x4 half[2]; bf16x8 v; } u;
+#pragma unroll
+            for (int th = 0; th < 2; ++th)
+                u.half[th] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(stage + (c >> 1) * 2048 + th * 1024 + (c & 1) * 512 + lane * 8));
+            return u.v;
+        };
+        // acc += values . weights
+        auto add_values = [&](const bf16x8 (&w)[MT]) __attribute__((always_inline)) {
             auto product = [&](const bf16x8 v, int c) __attribute__((always_inline)) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[mt], acc[mt][c], 0, 0, 0);
-                    if (ALL || row_token[mt] == only) acc[mt][c] = sum;
-                }
+                for (int mt = 0; mt < MT; ++mt) acc[mt][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w[mt], acc[mt][c], 0, 0, 0);
             };
             if constexpr (PACKED) {
 #pragma unroll
@@ -427,7 +420,7 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
                         for (int i = 0; i < 4; ++i) {
                             words[th * 4 + i] = *(__attribute__((address_space(3))) uint32_t *)(face + th * 256 + i * 16);
                             mags[th * 4 + i] = words[th * 4 + i] & 0x7f7f7f7fu;
-                            scale[th * 4 + i] = row_scale(e >> (8 * i) & 0xffu);
+                            scale[th * 4 + i] = block_scale(e >> (8 * i) & 0xffu);
                         }
                     }
                     product(weights_operand8<0>(words, mags, scale), grp * 4 + 0);
@@ -437,19 +430,28 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < S::COLS; ++c) {
-                    union { s16x4 half[2]; bf16x8 v; } u;
-#pragma unroll
-                    for (int th = 0; th < 2; ++th)
-                        u.half[th] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(stage + (c >> 1) * 2048 + th * 1024 + (c & 1) * 512 + lane * 8));
-                    product(u.v, c);
-                }
+                for (int c = 0; c < S::COLS; ++c) product(value_operand(c), c);
             }
         };
-        auto work_on = [&](StreamBlock<D, PACKED> &b, uint32_t block, uint64_t tile_row) __attribute__((always_inline)) {
+        // `next` is called once the block's registers are free
+        auto work_on = [&](StreamBlock<D, PACKED> &b, uint32_t block, uint64_t tile_row, auto &&next) __attribute__((always_inline)) {
             const uint32_t token0 = block * 32;
             const bool all_seen = token0 >= first_max && token0 + 31 <= pos_min;
-            const bool bad = put_values(b.v, token0, first_min, pos_max, !all_seen && pc.token0 != pc.token1);
+            bool odd = false;                                   // values that are not finite, and that some rows see and others do not
+            if constexpr (!PACKED) {
+                if (__builtin_expect(!(token0 >= first_min && token0 + 31 <= pos_max), 0)) clear_values(b.v, token0, first_min, pos_max);
+                if (__builtin_expect(!all_seen && pc.token0 != pc.token1, 0)) {
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int n = 0; n < S::LOADS; ++n) {
+                        const u32x4 taken = b.v[n] ^ pick(b.v[n], KEEP_FINITE);
+                        b.v[n] ^= taken;
+                        any |= taken[0] | taken[1] | taken[2] | taken[3];
+                    }
+                    odd = __ballot(any != 0) != 0;
+                }
+            }
+            put_values(b.v);
             f32x4 s[2][MT];
 #pragma unroll
             for (int th = 0; th < 2; ++th) {
@@ -458,12 +460,13 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
 #pragma unroll
                 for (int sl = 0; sl < S::SLABS; ++sl) {
                     bf16x8 k;
-                    if constexpr (PACKED) k = __builtin_bit_cast(bf16x8, activations_operand8(b.codes[th][sl][0], b.codes[th][sl][1], b.exps[th][sl]));
+                    if constexpr (PACKED) k = __builtin_bit_cast(bf16x8, expand8(b.codes[th][sl][0], b.codes[th][sl][1], block_scale(b.exps[th][sl])));
                     else k = __builtin_bit_cast(bf16x8, b.k[th][sl]);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) s[th][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[mt][sl], s[th][mt], 0, 0, 0);
                 }
             }
+            if (!odd) next();
             // weights of a row tile rounded to bf16, or what the rounding took off; their sum goes to l
             auto weights = [&](int mt, bool rest) __attribute__((always_inline)) {
                 const float base = floor_of(m[mt]);
@@ -503,43 +506,60 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
 #pragma unroll
                     for (int c = 0; c < S::COLS; ++c) acc[mt][c] *= shrink;
                 }
-                w[mt] = weights(mt, false);
             }
-            if (bad) {
-                for (uint32_t t = pc.token0; t <= pc.token1; ++t) {
-                    b.load_values(p.values + tile_row * (S::SLABS * S::TILE_BYTES), lane);
-                    put_values(b.v, token0, first_seen(p, pc.q.cached + t), pc.q.cached + t, false);
-                    add_values(w, t, std::false_type{});
-                }
-            } else {
-                add_values(w, 0, std::true_type{});
-                if (token0 + 31 >= pos_min) {
+            const int passes = token0 + 31 >= pos_min ? 2 : 1;
+            for (int pass = 0; pass < passes; ++pass) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) w[mt] = weights(mt, true);
-                    add_values(w, 0, std::true_type{});
+                for (int mt = 0; mt < MT; ++mt) w[mt] = weights(mt, pass != 0);
+                add_values(w);
+            }
+            if (__builtin_expect(odd, 0)) {
+                if constexpr (!PACKED) {
+                    for (int down = 0; down < 2; ++down) {
+                        b.load_values(p.values + tile_row * (S::SLABS * S::TILE_BYTES), lane);
+                        clear_values(b.v, token0, first_min, pos_max);
+#pragma unroll
+                        for (int n = 0; n < S::LOADS; ++n) b.v[n] = pick(b.v[n], down ? ONES_DOWN : ONES_UP);
+                        put_values(b.v);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            const uint32_t pos = pc.q.cached + row_token[mt], first = first_seen(p, pos);
+                            union { uint32_t words[4]; bf16x8 v; } seen;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t t = token0 + (i >> 1) * 16 + g * 4 + (i & 1) * 2;
+                                seen.words[i] = (t >= first && t <= pos ? 0x3f80u : 0u) | (t + 1 >= first && t + 1 <= pos ? 0x3f800000u : 0u);
+                            }
+#pragma unroll
+                            for (int c = 0; c < S::COLS; ++c) {
+                                const f32x4 count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_operand(c), seen.v, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (count[i] > 0.f) acc[mt][c][i] += down ? -INFINITY : INFINITY;
+                            }
+                        }
+                    }
                 }
+                next();
             }
         };
 
         // ---- this wavefront's blocks: pc.begin + wave, + 4, ... ------------------------------------------------------------------
         const uint32_t mine = pc.end > pc.begin + wave ? (pc.end - pc.begin - wave + 3) / 4 : 0;
         Pages<4> entries;
-        StreamBlock<D, PACKED> b[2];
-        uint64_t tile_row[2];
-        bool there[2];
-        auto request = [&](int which, uint32_t i) __attribute__((always_inline)) {
+        StreamBlock<D, PACKED> b;
+        uint64_t tile_row = 0;
+        bool there = false;
+        auto request = [&](uint32_t i) __attribute__((always_inline)) {
+            if (i >= mine) return;
             if ((i & 63) == 0) entries.load(p, pc, pc.begin + wave + i * 4);
-            there[which] = entries.at(p, pc.kv, i & 63, tile_row[which]);
-            b[which].load(p.keys, p.values, tile_row[which], lane);
+            there = entries.at(p, pc.kv, i & 63, tile_row);
+            b.load(p.keys, p.values, tile_row, lane);
         };
-        if (mine) request(0, 0);
-        for (uint32_t i = 0; i < mine; i += 2) {
-            if (i + 1 < mine) request(1, i + 1);
-            if (there[0]) work_on(b[0], pc.begin + wave + i * 4, tile_row[0]);
-            if (i + 1 < mine) {
-                if (i + 2 < mine) request(0, i + 2);
-                if (there[1]) work_on(b[1], pc.begin + wave + (i + 1) * 4, tile_row[1]);
-            }
+        request(0);
+        for (uint32_t i = 0; i < mine; ++i) {
+            if (there) work_on(b, pc.begin + wave + i * 4, tile_row, [&]() __attribute__((always_inline)) { request(i + 1); });
+            else request(i + 1);
         }
 
         // ---- join: wavefronts 2, 3 into 0, 1, then 1 into 0; afterwards wavefront 0 has it all -----------------------------------
@@ -624,7 +644,7 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 if ((uint32_t)(mt * 16 + x) >= pc.rows) continue;
-                const float by = l[mt] == 0.f ? 0.f : (PACKED ? Wfmt<7>::unscale : 1.f) / l[mt];
+                const float by = l[mt] == 0.f ? 0.f : 1.f / l[mt];
                 const uint32_t t = pc.q.start + row_token[mt], column = head[mt] * D;
                 if constexpr (PACKED) {
 #pragma unroll
@@ -748,55 +768,61 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
             load(p.keys, kreg, kexp);
             load(p.values, vreg, vexp);
         };
-        // Keys and values, or the values alone, of the loaded step into LDS; values outside [low, high], or without a page, as zeros.  True where one
-        // that stays is not finite.
-        auto put = [&](uint32_t buffer, uint32_t token0, uint32_t low, uint32_t high, const bool (&pages)[NB], bool keys, bool look) __attribute__((always_inline)) {
+        // Keys and values of the loaded step into LDS
+        auto put = [&](uint32_t buffer, bool keys) __attribute__((always_inline)) {
             lds_byte *const to = (lds_byte *)lds + buffer * 2 * S::HALF;
-            const bool whole = token0 >= low && token0 + NB * 32 - 1 <= high && pages[0] && pages[NB - 1];
-            bool bad = false;
 #pragma unroll
             for (int i = 0; i < S::EACH; ++i) {
                 if (S::PIECES % 512 && threadIdx.x + i * 512u >= (uint32_t)S::PIECES) break;
+                const uint32_t n = threadIdx.x + i * 512u, block = n / (S::PIECES / NB), within = n % (S::PIECES / NB);
+                if constexpr (PACKED) {
+                    const uint32_t face = within >> 4 & 3, r = within & 15, base = block * S::BLOCK + (within >> 4) * 512;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + ((h ^ (r >> 3)) * 16)) = expand8(kreg[i][2 * h], kreg[i][2 * h + 1], block_scale(kexp[i]));
+                        *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + (((r * 2 + h) ^ ((face & 1) * 8)) * 16)) = expand8(vreg[i][2 * h], vreg[i][2 * h + 1], block_scale(vexp[i]));
+                    }
+                } else {
+                    const uint32_t face = within >> 5 & 3, in_face = within & 31, r = in_face >> 1, base = block * S::BLOCK + (within >> 5) * 512;
+                    if (keys) *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + (((in_face & 1) ^ (r >> 3)) * 16)) = kreg[i];
+                    *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + ((in_face ^ ((face & 1) * 8)) * 16)) = vreg[i];
+                }
+            }
+        };
+        // bf16 values: zeros for tokens that no row of the unit sees
+        auto clear_values = [&](uint32_t token0, const bool (&pages)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < S::EACH; ++i) {
                 uint32_t block, from, token, exponent;
                 place(i, block, from, token, exponent);
                 const uint32_t t = token0 + block * 32 + token;
-                const bool gone = !whole && (t < low || t > high || !(NB == 2 && block ? pages[NB - 1] : pages[0]));
-                const uint32_t within = (threadIdx.x + i * 512u) % (S::PIECES / NB);
-                if constexpr (PACKED) {
-                    const uint32_t tile = within >> 6, face = within >> 4 & 3, r = within & 15;
-                    const uint32_t base = block * S::BLOCK + tile * 2048 + face * 512;
-                    if (look && !gone) bad |= vexp[i] >= 249u;
-                    const uint32_t ve = gone ? 0u : vexp[i];
-                    const u32x4 vc = gone ? u32x4{0, 0, 0, 0} : vreg[i];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (keys) *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + ((h ^ (r >> 3)) * 16)) = activations_operand8(kreg[i][2 * h], kreg[i][2 * h + 1], kexp[i]);
-                        *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + (((r * 2 + h) ^ ((face & 1) * 8)) * 16)) = activations_operand8(vc[2 * h], vc[2 * h + 1], ve);
-                    }
-                } else {
-                    const uint32_t face = within >> 5 & 3, in_face = within & 31, r = in_face >> 1;
-                    const uint32_t base = block * S::BLOCK + (within >> 5) * 512;
-                    const u32x4 v = gone ? u32x4{0, 0, 0, 0} : vreg[i];
-                    if (look) bad |= not_finite(v);
-                    if (keys) *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + (((in_face & 1) ^ (r >> 3)) * 16)) = kreg[i];
-                    *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + ((in_face ^ ((face & 1) * 8)) * 16)) = v;
-                }
+                if (t < first_min || t > pos_max || !(NB == 2 && block ? pages[NB - 1] : pages[0])) vreg[i] = u32x4{0, 0, 0, 0};
             }
-            return bad;
         };
 
         const uint32_t steps = (pc.end - pc.begin + NB - 1) / NB;
-        bool bad = false;
-        // rows of the unit see different parts of the step: values that are not finite have to be looked for
-        auto uneven = [&](uint32_t token0) { return pc.token0 != pc.token1 && !(token0 >= unit_first_max && token0 + NB * 32 - 1 <= unit_pos_min); };
+        bool odd = false;                                       // values of the step that are not finite, and that some rows see and others do not
         auto fill = [&](uint32_t step) __attribute__((always_inline)) {
-            const uint32_t token0 = (pc.begin + step * NB) * 32;
-            const bool look = uneven(token0);
-            const bool mine = put(step & 1, token0, first_min, pos_max, there, true, look);
+            const uint32_t token0 = (pc.begin + step * NB) * 32, last = token0 + NB * 32 - 1;
+            bool look = false;
+            uint32_t any = 0;
+            if constexpr (!PACKED) {
+                if (__builtin_expect(!(token0 >= first_min && last <= pos_max && there[0] && there[NB - 1]), 0)) clear_values(token0, there);
+                look = pc.token0 != pc.token1 && !(token0 >= unit_first_max && last <= unit_pos_min);
+                if (__builtin_expect(look, 0)) {
+#pragma unroll
+                    for (int i = 0; i < S::EACH; ++i) {
+                        const u32x4 taken = vreg[i] ^ pick(vreg[i], KEEP_FINITE);
+                        vreg[i] ^= taken;
+                        any |= taken[0] | taken[1] | taken[2] | taken[3];
+                    }
+                }
+            }
+            put(step & 1, true);
 #pragma unroll
             for (int b = 0; b < NB; ++b) ready[b] = there[b];
-            if (look) bad = __syncthreads_or(mine);
-            else { bad = false; __syncthreads(); }
+            if (look) odd = __syncthreads_or(any != 0);
+            else { odd = false; __syncthreads(); }
         };
         if (steps) {
             request(0);
@@ -865,58 +891,71 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
 #pragma unroll
                     for (int d = 0; d < DB; ++d) acc[d] *= shrink;
                 }
-                weights(false);
             }
-            // acc += values . weights for the rows with `only`'s token, or all
-            auto add_values = [&](uint32_t only, auto all) __attribute__((always_inline)) {
-                constexpr bool ALL = decltype(all)::value;
+            auto value_operand = [&](int d, int b, int h) __attribute__((always_inline)) {
+                union { s16x4 half[2]; bf16x8 v; } u;
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    f32x16 sum = acc[d];
+                for (int r = 0; r < 2; ++r)
+                    u.half[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(from + value_at + b * S::BLOCK + d * 2048 + h * 1024 + r * 256));
+                return u.v;
+            };
+            const int passes = skip ? 0 : last >= wave_pos_min ? 2 : 1;
+            for (int pass = 0; pass < passes; ++pass) {
+                weights(pass != 0);
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            union { s16x4 half[2]; bf16x8 v; } u;
+                        for (int h = 0; h < 2; ++h) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_operand(d, b, h), w[b][h], acc[d], 0, 0, 0);
+            }
+            if (__builtin_expect(odd, 0)) {
+                if constexpr (!PACKED) {
+                    // the step behind this one waits in registers, and is loaded again afterwards
+                    uint64_t rows_next[NB];
 #pragma unroll
-                            for (int r = 0; r < 2; ++r)
-                                u.half[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(from + value_at + b * S::BLOCK + d * 2048 + h * 1024 + r * 256));
-                            sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.v, w[b][h], sum, 0, 0, 0);
-                        }
-                    if (ALL || row_token == only) acc[d] = sum;
-                }
-            };
-            if (!bad) {
-                if (!skip) {
-                    add_values(0, std::true_type{});
-                    if (last >= wave_pos_min) {
-                        weights(true);
-                        add_values(0, std::true_type{});
+                    for (int b = 0; b < NB; ++b) {
+                        rows_next[b] = rows_of[b];
+                        const uint32_t block = pc.begin + step * NB + b;
+                        int32_t page = block < pc.end ? p.table[(uint64_t)pc.r * p.max_pages + block / p.page_blocks] : -1;
+                        if ((uint32_t)page >= p.pages) page = 0;
+                        rows_of[b] = ((uint64_t)page * p.kv_heads + pc.kv) * p.page_blocks + block % p.page_blocks;
                     }
-                }
-            } else {
-                // the step behind this one waits in registers, and is loaded again afterwards
-                bool mine[NB];
-                uint64_t rows_next[NB];
-                bool there_next[NB];
+                    for (int down = 0; down < 2; ++down) {
+                        load(p.values, vreg, vexp);
+                        clear_values(token0, ready);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    mine[b] = ready[b]; rows_next[b] = rows_of[b]; there_next[b] = there[b];
-                    const uint32_t block = pc.begin + step * NB + b;
-                    int32_t page = block < pc.end ? p.table[(uint64_t)pc.r * p.max_pages + block / p.page_blocks] : -1;
-                    if ((uint32_t)page >= p.pages) page = 0;
-                    rows_of[b] = ((uint64_t)page * p.kv_heads + pc.kv) * p.page_blocks + block % p.page_blocks;
-                }
-                for (uint32_t t = pc.token0; t <= pc.token1; ++t) {
-                    load(p.values, vreg, vexp);
-                    __syncthreads();
-                    put(step & 1, token0, first_seen(p, pc.q.cached + t), pc.q.cached + t, mine, false, false);
-                    __syncthreads();
-                    if (!skip) add_values(t, std::false_type{});
-                }
+                        for (int i = 0; i < S::EACH; ++i) vreg[i] = pick(vreg[i], down ? ONES_DOWN : ONES_UP);
+                        __syncthreads();
+                        put(step & 1, false);
+                        __syncthreads();
+                        if (skip) continue;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) { rows_of[b] = rows_next[b]; there[b] = there_next[b]; }
-                if (step + 1 < steps) load(p.values, vreg, vexp);
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                union { uint32_t words[4]; bf16x8 v; } seen;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t t = token0 + b * 32 + h * 16 + (i >> 1) * 8 + kh * 4 + (i & 1) * 2;
+                                    seen.words[i] = (t >= first && t <= pos ? 0x3f80u : 0u) | (t + 1 >= first && t + 1 <= pos ? 0x3f800000u : 0u);
+                                }
+#pragma unroll
+                                for (int d = 0; d < DB; ++d) {
+                                    f32x16 count;
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) count[i] = 0.f;
+                                    count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_operand(d, b, h), seen.v, count, 0, 0, 0);
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i)
+                                        if (count[i] > 0.f) acc[d][i] += down ? -INFINITY : INFINITY;
+                                }
+                            }
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) rows_of[b] = rows_next[b];
+                    if (step + 1 < steps) load(p.values, vreg, vexp);
+                }
             }
             if (step + 1 < steps) fill(step + 1);
         }
@@ -958,7 +997,7 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
             }
         }
         // columns 8 (i / 4) + 4 kh + i % 4 of 32: the swap leaves columns 8 kh .. 8 kh + 7 of a face row in each lane
-        const float by = l == 0.f ? 0.f : (PACKED ? Wfmt<7>::unscale : 1.f) / l;
+        const float by = l == 0.f ? 0.f : 1.f / l;
         const bool stored = (uint32_t)(wave * 32 + c) < pc.rows;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -979,7 +1018,7 @@ namespace {
 struct Route {
     uint32_t mt = 0;                       // row tiles of the kernel for few rows; 0: not launched
     bool tile = false;
-    uint32_t stream_target = 1024, tile_target = 512;
+    uint32_t stream_target = 256, tile_target = 256;       // resident workgroups: one per CU, or two
     size_t slot_bytes = 0, slots = 0;
 };
 Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCache &c) {
@@ -997,6 +1036,7 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
         if (r.tile) r.mt = 0;
     }
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
+    if (r.mt <= 2 && c.head_dim <= 128) r.stream_target = 512;
     if (r.mt) {
         const size_t cols = packed ? (c.head_dim + 63) / 64 * 4 : c.head_dim / 16;
         r.slot_bytes = (r.mt * cols * 16 + r.mt * 8) * 64;
@@ -1012,18 +1052,18 @@ int clear_counters(void *at, hipStream_t st) {
     return check_launch("clear_counters_kernel");
 }
 
-template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, uint32_t blocks, size_t lds, hipStream_t st) {
-    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(blocks), dim3(256), lds, st, p);
-    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(blocks), dim3(256), lds, st, p);
+template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, size_t lds, hipStream_t st) {
+    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(p.target), dim3(256), lds, st, p);
+    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(p.target), dim3(256), lds, st, p);
 }
 template <int D, int MOST> void launch_stream(const AttentionDev &p, uint32_t mt, bool packed, size_t lds, hipStream_t st) {
-    if (mt == 1) launch_stream<D, 1>(p, packed, 512, lds, st);
-    else if (mt == 2) launch_stream<D, 2>(p, packed, 512, lds, st);
-    else launch_stream<D, MOST>(p, packed, 512, lds, st);
+    if (mt == 1) launch_stream<D, 1>(p, packed, lds, st);
+    else if (mt == 2) launch_stream<D, 2>(p, packed, lds, st);
+    else launch_stream<D, MOST>(p, packed, lds, st);
 }
 template <int D> void launch_tile(const AttentionDev &p, bool packed, size_t lds, hipStream_t st) {
-    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(256), dim3(512), lds, st, p);
-    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(256), dim3(512), lds, st, p);
+    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(p.target), dim3(512), lds, st, p);
+    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(p.target), dim3(512), lds, st, p);
 }
 }  // namespace
 
@@ -1044,7 +1084,7 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     p.heads = x.heads; p.group = x.heads / c.kv_heads; p.window = x.window;
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
     // a scale of zero stands for one that no score survives: -inf, what is masked, has to stay -inf
-    p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 1e-30f) * (packed ? Wfmt<7>::unscale : 1.f);
+    p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 1e-30f);
     p.flip = x.scale < 0.f ? 0x80008000u : 0u;
 
     const Route route = route_of(p.tokens, p.requests, p.heads, c);
