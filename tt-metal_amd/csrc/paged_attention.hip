@@ -10,7 +10,7 @@
 //              rho % group of the group, so a decode step of 4 heads per key head is 4 rows, a chunk of 512 tokens 2048
 //   units      (request, key head, tile of ROWS rows).  A unit's tokens are cut into pieces of a common length, which is chosen from the
 //              lengths on the device so that the whole step comes to about `target` pieces: requests of any lengths, one long one among
-//              them, fill the chip evenly.  Every workgroup makes the same prefix sums over the requests and takes pieces
+//              them, fill the chip evenly.  Every wavefront makes the same prefix sums over the requests and takes pieces
 //              blockIdx, blockIdx + gridDim, ...  A unit of one piece is stored at once; the others leave (maximum, sum, fp32
 //              accumulators) in memory, and whoever comes last joins them, in the order of the pieces
 //   softmax    one pass: running maximum m and sum l per row in fp32, weights exp2(s - m).  m only moves when a score passes it
@@ -62,6 +62,11 @@ struct AttentionDev {
 constexpr uint32_t COUNTERS = 4096;        // at most 2 `target` slots, each could be a unit's first
 constexpr float LAZY = 8.f;                // how far (log2) a score may pass the running maximum
 
+// Operands go from LDS through a ring of this many, so that a product finds its own in registers: a read takes about as long as four products.
+constexpr int AHEAD = 4;
+// Reads of LDS and products stay in the order in which they are written; everything else may pass.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x476); }
+
 // ---- the work of a step ---------------------------------------------------------------------------------------------------------
 struct Request { uint32_t start, added, cached; };
 __device__ __forceinline__ Request request_at(const AttentionDev &p, uint32_t r) {
@@ -86,62 +91,58 @@ template <int ROWS> struct Extent {
     }
 };
 
-// Exclusive prefix sum over the workgroup, and the sum of all.
-template <int THREADS> __device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t *wave_sums, uint64_t &all) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t to = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(to, d);
-        if (lane >= (uint32_t)d) to += o;
-    }
-    __syncthreads();
-    if (lane == 63) wave_sums[wave] = to;
-    __syncthreads();
-    to -= v;
-    all = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < THREADS / 64; ++w) {
-        if (w < wave) to += wave_sums[w];
-        all += wave_sums[w];
-    }
-    return to;
+// Sums over the lanes up to and including this one, by DPP: no LDS and no barriers, the same in every wavefront.
+template <typename T> __device__ __forceinline__ T running_sum(T v) {
+    auto from = [](T x, auto ctrl, auto rows) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    using std::integral_constant;
+    typedef integral_constant<int, 0xf> all;
+    v += from(v, integral_constant<int, 0x111>{}, all{});                              // 1, 2, 4, 8 lanes down within 16
+    v += from(v, integral_constant<int, 0x112>{}, all{});
+    v += from(v, integral_constant<int, 0x114>{}, all{});
+    v += from(v, integral_constant<int, 0x118>{}, all{});
+    v += from(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});      // lane 15 of each 16 to the next
+    v += from(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});      // lane 31 to the upper half
+    return v;
 }
+template <typename T> __device__ __forceinline__ T last_lane(T v) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
 
-struct Plan { uint32_t piece, pieces; };   // blocks of a piece, pieces of the step
-// first_piece[requests + 1], first_slot[requests]: LDS
-template <int THREADS, int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const AttentionDev &p, uint32_t *first_piece, uint32_t *first_slot, uint64_t *wave_sums) {
-    const uint32_t each = (p.requests + THREADS - 1) / THREADS, r0 = min(threadIdx.x * each, p.requests), r1 = min(r0 + each, p.requests);
-    uint64_t work = 0, units = 0, all, all_units;
+// The pieces of the step.  Every wavefront makes the plan for itself: a lane has `each` requests, one where there are at most 64.
+struct Plan {
+    uint32_t each, piece, pieces;          // blocks of a piece, pieces of the step
+    uint32_t first_piece, first_slot;      // of this lane's requests
+    Request q;                             // this lane's first request
+};
+template <int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const AttentionDev &p) {
+    const uint32_t lane = threadIdx.x & 63;
+    Plan plan;
+    plan.each = (p.requests + 63) / 64;
+    const uint32_t r0 = min(lane * plan.each, p.requests), r1 = min(r0 + plan.each, p.requests);
+    plan.q = r0 < r1 ? request_at(p, r0) : Request{0, 0, 0};
+    float work = 0.f, units = 0.f;
     for (uint32_t r = r0; r < r1; ++r) {
-        const Extent<ROWS> e(p, request_at(p, r));
-        work += (uint64_t)e.units * e.blocks;
-        units += e.units;
+        const Extent<ROWS> e(p, r == r0 ? plan.q : request_at(p, r));
+        work += (float)e.units * (float)e.blocks;
+        units += (float)e.units;
     }
-    scan<THREADS>(work, wave_sums, all);
-    scan<THREADS>(units, wave_sums, all_units);
+    work = last_lane(running_sum(work));
+    units = last_lane(running_sum(units));
     // the last piece of a unit is on average half a piece: that many more come to about one for each resident workgroup
-    const uint64_t aim = max((uint64_t)p.target - min(all_units / 2, (uint64_t)p.target), (uint64_t)p.target / 4), share = (all + aim - 1) / aim;
-    const uint32_t piece = (uint32_t)(max(share, (uint64_t)1) + STEP - 1) / STEP * STEP;
-    uint64_t pieces = 0, slots = 0;        // of this lane's requests: pieces, and those of units with more than one, together in one scan
+    const float aim = fmaxf((float)p.target - 0.5f * units, 0.25f * (float)p.target);
+    plan.piece = ((uint32_t)fminf(fmaxf(ceilf(work / aim), 1.f), 1e9f) + STEP - 1) / STEP * STEP;
+    uint32_t pieces = 0, slots = 0;        // of this lane's requests: pieces, and those of units with more than one
     for (uint32_t r = r0; r < r1; ++r) {
-        const Extent<ROWS> e(p, request_at(p, r));
-        const uint32_t parts = (e.blocks + piece - 1) / piece;
-        pieces += (uint64_t)e.units * parts;
-        if (parts > 1) slots += (uint64_t)e.units * parts;
+        const Extent<ROWS> e(p, r == r0 ? plan.q : request_at(p, r));
+        const uint32_t parts = (e.blocks + plan.piece - 1) / plan.piece;
+        pieces += e.units * parts;
+        if (parts > 1) slots += e.units * parts;
     }
-    uint64_t at = scan<THREADS>(pieces | slots << 32, wave_sums, all);
-    for (uint32_t r = r0; r < r1; ++r) {
-        const Extent<ROWS> e(p, request_at(p, r));
-        const uint32_t parts = (e.blocks + piece - 1) / piece;
-        first_piece[r] = (uint32_t)at;
-        first_slot[r] = (uint32_t)(at >> 32);
-        at += (uint64_t)e.units * parts;
-        if (parts > 1) at += (uint64_t)e.units * parts << 32;
-    }
-    if (threadIdx.x == 0) first_piece[p.requests] = (uint32_t)all;
-    __syncthreads();
-    return {piece, (uint32_t)all};
+    const uint32_t pieces_to = running_sum(pieces), slots_to = running_sum(slots);
+    plan.first_piece = pieces_to - pieces;
+    plan.first_slot = slots_to - slots;
+    plan.pieces = last_lane(pieces_to);
+    return plan;
 }
 
 // One piece: rows [row0, row0 + rows) of a request and key head, blocks [begin, end) of those that the unit sees.
@@ -150,21 +151,27 @@ struct Piece {
     uint32_t r, kv, row0, rows, begin, end, parts, part, slot;
     uint32_t token0, token1;               // first and last token of the unit, counted from the request's first new one
 };
-template <int ROWS> __device__ __forceinline__ Piece piece_at(const AttentionDev &p, const Plan &plan, const uint32_t *first_piece, const uint32_t *first_slot, uint32_t index) {
-    uint32_t low = 0, high = p.requests;
-    while (high - low > 1) {
-        const uint32_t mid = (low + high) / 2;
-        if (first_piece[mid] <= index) low = mid; else high = mid;
+// False where the unit has fewer pieces than others of its request, and this is none of them.
+template <int ROWS> __device__ __forceinline__ bool piece_at(const AttentionDev &p, const Plan &plan, uint32_t index, Piece &x) {
+    const uint32_t owner = __popcll(__ballot(plan.first_piece <= index)) - 1;
+    uint32_t at = __builtin_amdgcn_readlane(plan.first_piece, owner), most, units;
+    x.slot = __builtin_amdgcn_readlane(plan.first_slot, owner);
+    x.r = owner * plan.each;
+    x.q = {(uint32_t)__builtin_amdgcn_readlane(plan.q.start, owner), (uint32_t)__builtin_amdgcn_readlane(plan.q.added, owner), (uint32_t)__builtin_amdgcn_readlane(plan.q.cached, owner)};
+    for (uint32_t i = 0;; ++i) {
+        const Extent<ROWS> e(p, x.q);
+        units = e.units;
+        most = (e.blocks + plan.piece - 1) / plan.piece;
+        if (index < at + units * most || i + 1 >= plan.each || x.r + 1 >= p.requests) break;
+        at += units * most;
+        if (most > 1) x.slot += units * most;
+        x.q = request_at(p, ++x.r);
     }
-    Piece x;
-    x.r = __builtin_amdgcn_readfirstlane(low);
-    x.q = request_at(p, x.r);
-    const Extent<ROWS> e(p, x.q);
-    const uint32_t most = (e.blocks + plan.piece - 1) / plan.piece, tiles = e.units / p.kv_heads;
-    uint32_t local = index - first_piece[x.r];
+    if (index - at >= units * most) return false;              // row_starts out of order
+    uint32_t local = index - at;
     x.kv = local % p.kv_heads; local /= p.kv_heads;
     x.part = local % most;
-    const uint32_t tile = tiles - 1 - local / most;            // the last tile of a chunk sees most: first
+    const uint32_t tile = units / p.kv_heads - 1 - local / most;                       // the last tile of a chunk sees most: first
     const uint32_t all_rows = x.q.added * p.group;
     x.row0 = tile * ROWS;
     x.rows = min((uint32_t)ROWS, all_rows - x.row0);
@@ -174,29 +181,26 @@ template <int ROWS> __device__ __forceinline__ Piece piece_at(const AttentionDev
     x.parts = max((end - begin + plan.piece - 1) / plan.piece, 1u);
     x.begin = min(begin + x.part * plan.piece, end);
     x.end = min(x.begin + plan.piece, end);
-    x.slot = first_slot[x.r] + (tile * p.kv_heads + x.kv) * most;
-    return x;
+    x.slot += (tile * p.kv_heads + x.kv) * most;
+    return x.part < x.parts;
 }
 
-// Pages of the blocks first, first + STRIDE, ... of a piece, 64 at a time: lane i has entry i, -1 for what is no page or lies past the end.
-template <int STRIDE> struct Pages {
-    int32_t page;
-    uint32_t within;
+// Where the blocks first, first + STRIDE, ... of a piece lie, 64 at a time: lane i has the byte at which the keys, and the values, of entry i
+// start, 0 (page 0) for what has no page or lies past the end.
+template <int STRIDE, int BLOCK_BYTES> struct Blocks {
+    uint32_t low, high;
+    uint64_t pages;                        // bit i: entry i has a page
     __device__ __forceinline__ void load(const AttentionDev &p, const Piece &x, uint32_t first) {
-        const uint32_t b = first + (threadIdx.x & 63) * STRIDE;
-        page = -1;
-        within = b % p.page_blocks;
-        if (b < x.end) {
-            page = p.table[(uint64_t)x.r * p.max_pages + b / p.page_blocks];
-            if ((uint32_t)page >= p.pages) page = -1;
-        }
+        const uint32_t b = first + (threadIdx.x & 63) * STRIDE, column = b / p.page_blocks;
+        const int32_t page = b < x.end ? p.table[(uint64_t)x.r * p.max_pages + column] : -1;
+        const bool there = (uint32_t)page < p.pages;
+        const uint64_t at = there ? (((uint64_t)page * p.kv_heads + x.kv) * p.page_blocks + (b - column * p.page_blocks)) * BLOCK_BYTES : 0;
+        low = (uint32_t)at;
+        high = (uint32_t)(at >> 32);
+        pages = __ballot(there);
     }
-    // number of the tile row of `head`, of page 0 where there is none; false there
-    __device__ __forceinline__ bool at(const AttentionDev &p, uint32_t head, uint32_t i, uint64_t &tile_row) const {
-        const int32_t g = __builtin_amdgcn_readlane(page, i);
-        tile_row = ((uint64_t)(uint32_t)max(g, 0) * p.kv_heads + head) * p.page_blocks + (uint32_t)__builtin_amdgcn_readlane(within, i);
-        return g >= 0;
-    }
+    __device__ __forceinline__ uint64_t at(uint32_t i) const { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(high, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(low, i); }
+    __device__ __forceinline__ bool has(uint32_t i) const { return pages >> i & 1; }
 };
 
 // ---- softmax ----------------------------------------------------------------------------------------------------------------------
@@ -225,15 +229,13 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), sum, false);
 }
 
-// ---- partial results: device-coherent accesses, past the L2 of the XCD; a fence over all of it would cost more ----------------------
-__device__ __forceinline__ void put_pair(uint8_t *to, float a, float b) {
-    __hip_atomic_store(reinterpret_cast<uint64_t *>(to), (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// ---- partial results -------------------------------------------------------------------------------------------------------------------
+// Stored past the L2 of the XCD (sc1): a release of all that the L2 holds would cost more than the kernel.  Loaded as any other memory, behind
+// an acquire: nobody has read these lines before in the launch.
+__device__ __forceinline__ void put_quad(uint8_t *to, const f32x4 &v) {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(to), "v"(v) : "memory");
 }
-__device__ __forceinline__ void get_pair(const uint8_t *from, float &a, float &b) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    a = __uint_as_float((uint32_t)v);
-    b = __uint_as_float((uint32_t)(v >> 32));
-}
+__device__ __forceinline__ f32x4 get_quad(const uint8_t *from) { return *reinterpret_cast<const f32x4 *>(from); }
 // Called by the whole workgroup once its partial result is on its way; true for the one that finds all the others' there.
 __device__ __forceinline__ bool last_of(const AttentionDev &p, const Piece &x, uint32_t *flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // this wavefront's stores have arrived
@@ -245,7 +247,9 @@ __device__ __forceinline__ bool last_of(const AttentionDev &p, const Piece &x, u
         *flag = last;
     }
     __syncthreads();
-    return *flag;
+    if (!*flag) return false;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    return true;
 }
 
 // LDS that lanes of one wavefront hand each other: the hardware keeps a wavefront's accesses in order, this keeps the compiler to it.
@@ -306,8 +310,7 @@ template <int D, bool PACKED> struct StreamBlock {
 #pragma unroll
         for (int i = 0; i < S::LOADS; ++i) v[i] = *reinterpret_cast<const u32x4 *>(base + min(i * 64 + lane, S::CHUNKS - 1) * 16);
     }
-    __device__ __forceinline__ void load(const uint8_t *keys, const uint8_t *values, uint64_t tile_row, int lane) {
-        const uint64_t at = tile_row * (S::SLABS * S::TILE_BYTES);
+    __device__ __forceinline__ void load(const uint8_t *keys, const uint8_t *values, uint64_t at, int lane) {
         const uint8_t *base = keys + at;
         const int x = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -326,19 +329,18 @@ template <int D, bool PACKED> struct StreamBlock {
 };
 
 template <int D, int MT, bool PACKED>
-__global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attention_stream_kernel(const AttentionDev p) {
+__global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void paged_attention_stream_kernel(const AttentionDev p) {
     using S = StreamShape<D, PACKED>;
     constexpr int ROWS = MT * 16, NACC = MT * S::COLS;          // NACC quads of accumulators
     constexpr int JOIN = 2 * (NACC * 16 + MT * 8) * 64;         // bytes: two wavefronts' state
     constexpr int LDS = 4 * S::STAGE > JOIN ? 4 * S::STAGE : JOIN;
+    constexpr bool Q_IN_LDS = MT > 2;                           // registers for more than two row tiles' queries are dearer than reading them again
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
-    __shared__ uint64_t wave_sums[4];
+    __shared__ u32x4 queries[Q_IN_LDS ? MT * S::SLABS * 64 : 1];
     __shared__ uint32_t flag;
-    extern __shared__ uint32_t tables[];
     const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (p.zero_rows) clear_rows(p, D);
-    const Plan plan = make_plan<256, ROWS, 4>(p, tables, tables + p.requests + 1, wave_sums);
+    const Plan plan = make_plan<ROWS, 4>(p);
 
     typedef __attribute__((address_space(3))) uint8_t lds_byte;
     lds_byte *const stage = (lds_byte *)lds + wave * S::STAGE;
@@ -351,21 +353,27 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
     const uint32_t out_width = p.heads * D;
 
     for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
-        const Piece pc = piece_at<ROWS>(p, plan, tables, tables + p.requests + 1, index);
-        if (pc.part >= pc.parts) continue;
-        bf16x8 q[MT][S::SLABS];
-        uint32_t row_token[MT], head[MT];
+        Piece pc;
+        if (!piece_at<ROWS>(p, plan, index, pc)) continue;
+        bf16x8 q[Q_IN_LDS ? 1 : MT][S::SLABS];
+        uint32_t row_token[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const uint32_t rho = pc.row0 + min((uint32_t)(mt * 16 + x), pc.rows - 1);       // rows past the last repeat it
             row_token[mt] = rho / p.group;
-            head[mt] = pc.kv * p.group + rho % p.group;
+            const uint32_t head = pc.kv * p.group + rho % p.group;
 #pragma unroll
             for (int s = 0; s < S::SLABS; ++s) {
-                u32x4 w = *reinterpret_cast<const u32x4 *>(p.rows + row_bytes_at(pc.q.start + row_token[mt], p.width, p.query_column + head[mt] * D + s * 32 + g * 8, p.tiled));
-                q[mt][s] = __builtin_bit_cast(bf16x8, w ^ u32x4{p.flip, p.flip, p.flip, p.flip});
+                if (Q_IN_LDS && (mt * S::SLABS + s) % 4 != wave) continue;
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(p.rows + row_bytes_at(pc.q.start + row_token[mt], p.width, p.query_column + head * D + s * 32 + g * 8, p.tiled)) ^ u32x4{p.flip, p.flip, p.flip, p.flip};
+                if constexpr (Q_IN_LDS) queries[(mt * S::SLABS + s) * 64 + lane] = w;
+                else q[mt][s] = __builtin_bit_cast(bf16x8, w);
             }
         }
+        auto query = [&](int mt, int s) __attribute__((always_inline)) {
+            if constexpr (Q_IN_LDS) return __builtin_bit_cast(bf16x8, queries[(mt * S::SLABS + s) * 64 + lane]);
+            else return q[mt][s];
+        };
         f32x4 acc[MT][S::COLS];
         float m[MT], l[MT];
 #pragma unroll
@@ -389,7 +397,7 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
         auto clear_values = [&](u32x4 (&v)[S::LOADS], uint32_t token0, uint32_t low, uint32_t high) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < S::LOADS; ++n) {
-                const uint32_t c = n * 64 + lane, t = token0 + (c >> 6 & 1) * 16 + (c >> 1 & 15);
+                const uint32_t t = token0 + (n & 1) * 16 + (lane >> 1 & 15);               // 64 pieces are a face row of a tile
                 if (t < low || t > high) v[n] = u32x4{0, 0, 0, 0};
             }
         };
@@ -429,12 +437,19 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
                     product(weights_operand8<3>(words, mags, scale), grp * 4 + 3);
                 }
             } else {
+                bf16x8 ring[AHEAD];
 #pragma unroll
-                for (int c = 0; c < S::COLS; ++c) product(value_operand(c), c);
+                for (int c = 0; c < AHEAD; ++c) ring[c] = value_operand(c);
+#pragma unroll
+                for (int c = 0; c < S::COLS; ++c) {
+                    product(ring[c % AHEAD], c);
+                    if (c + AHEAD < S::COLS) ring[c % AHEAD] = value_operand(c + AHEAD);
+                    keep_order();
+                }
             }
         };
         // `next` is called once the block's registers are free
-        auto work_on = [&](StreamBlock<D, PACKED> &b, uint32_t block, uint64_t tile_row, auto &&next) __attribute__((always_inline)) {
+        auto work_on = [&](StreamBlock<D, PACKED> &b, uint32_t block, uint64_t at, auto &&next) __attribute__((always_inline)) {
             const uint32_t token0 = block * 32;
             const bool all_seen = token0 >= first_max && token0 + 31 <= pos_min;
             bool odd = false;                                   // values that are not finite, and that some rows see and others do not
@@ -463,7 +478,7 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
                     if constexpr (PACKED) k = __builtin_bit_cast(bf16x8, expand8(b.codes[th][sl][0], b.codes[th][sl][1], block_scale(b.exps[th][sl])));
                     else k = __builtin_bit_cast(bf16x8, b.k[th][sl]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) s[th][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[mt][sl], s[th][mt], 0, 0, 0);
+                    for (int mt = 0; mt < MT; ++mt) s[th][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, query(mt, sl), s[th][mt], 0, 0, 0);
                 }
             }
             if (!odd) next();
@@ -488,13 +503,12 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
             for (int mt = 0; mt < MT; ++mt) {
                 if (!all_seen) {
                     const uint32_t pos = pc.q.cached + row_token[mt], first = first_seen(p, pos);
+                    const int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
 #pragma unroll
                     for (int th = 0; th < 2; ++th)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t t = token0 + th * 16 + g * 4 + i;
-                            if (t < first || t > pos) s[th][mt][i] = -INFINITY;
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            if (th * 16 + i < from || th * 16 + i > to) s[th][mt][i] = -INFINITY;
                 }
                 float top = fmaxf(fmaxf(s[0][mt][0], s[0][mt][1]), fmaxf(s[0][mt][2], s[0][mt][3]));
                 top = fmaxf(top, fmaxf(fmaxf(s[1][mt][0], s[1][mt][1]), fmaxf(s[1][mt][2], s[1][mt][3])));
@@ -507,16 +521,18 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
                     for (int c = 0; c < S::COLS; ++c) acc[mt][c] *= shrink;
                 }
             }
-            const int passes = token0 + 31 >= pos_min ? 2 : 1;
-            for (int pass = 0; pass < passes; ++pass) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) w[mt] = weights(mt, pass != 0);
+            for (int mt = 0; mt < MT; ++mt) w[mt] = weights(mt, false);
+            add_values(w);
+            if (__builtin_expect(token0 + 31 >= pos_min, 0)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) w[mt] = weights(mt, true);
                 add_values(w);
             }
             if (__builtin_expect(odd, 0)) {
                 if constexpr (!PACKED) {
                     for (int down = 0; down < 2; ++down) {
-                        b.load_values(p.values + tile_row * (S::SLABS * S::TILE_BYTES), lane);
+                        b.load_values(p.values + at, lane);
                         clear_values(b.v, token0, first_min, pos_max);
 #pragma unroll
                         for (int n = 0; n < S::LOADS; ++n) b.v[n] = pick(b.v[n], down ? ONES_DOWN : ONES_UP);
@@ -524,11 +540,12 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             const uint32_t pos = pc.q.cached + row_token[mt], first = first_seen(p, pos);
+                            const int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
                             union { uint32_t words[4]; bf16x8 v; } seen;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const uint32_t t = token0 + (i >> 1) * 16 + g * 4 + (i & 1) * 2;
-                                seen.words[i] = (t >= first && t <= pos ? 0x3f80u : 0u) | (t + 1 >= first && t + 1 <= pos ? 0x3f800000u : 0u);
+                                const int t = (i >> 1) * 16 + (i & 1) * 2;
+                                seen.words[i] = (t >= from && t <= to ? 0x3f80u : 0u) | (t + 1 >= from && t + 1 <= to ? 0x3f800000u : 0u);
                             }
 #pragma unroll
                             for (int c = 0; c < S::COLS; ++c) {
@@ -546,22 +563,45 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
 
         // ---- this wavefront's blocks: pc.begin + wave, + 4, ... ------------------------------------------------------------------
         const uint32_t mine = pc.end > pc.begin + wave ? (pc.end - pc.begin - wave + 3) / 4 : 0;
-        Pages<4> entries;
+        Blocks<4, S::SLABS * S::TILE_BYTES> blocks;
         StreamBlock<D, PACKED> b;
-        uint64_t tile_row = 0;
+        uint64_t at = 0;
         bool there = false;
         auto request = [&](uint32_t i) __attribute__((always_inline)) {
             if (i >= mine) return;
-            if ((i & 63) == 0) entries.load(p, pc, pc.begin + wave + i * 4);
-            there = entries.at(p, pc.kv, i & 63, tile_row);
-            b.load(p.keys, p.values, tile_row, lane);
+            if ((i & 63) == 0) blocks.load(p, pc, pc.begin + wave + i * 4);
+            at = blocks.at(i & 63);
+            there = blocks.has(i & 63);
+            b.load(p.keys, p.values, at, lane);
         };
         request(0);
+        if (Q_IN_LDS) __syncthreads();
         for (uint32_t i = 0; i < mine; ++i) {
-            if (there) work_on(b, pc.begin + wave + i * 4, tile_row, [&]() __attribute__((always_inline)) { request(i + 1); });
+            if (there) work_on(b, pc.begin + wave + i * 4, at, [&]() __attribute__((always_inline)) { request(i + 1); });
             else request(i + 1);
         }
 
+        // columns c of row tile mt that this lane has, divided by the sum of the weights: four of bf16, sixteen of block floats
+        auto store = [&](int mt, int c, const f32x4 *v, float sum) __attribute__((always_inline)) {
+            if ((uint32_t)(mt * 16 + x) >= pc.rows) return;
+            const uint32_t rho = pc.row0 + mt * 16 + x, token = rho / p.group, column = (pc.kv * p.group + rho % p.group) * D;
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            if constexpr (PACKED) {
+                const uint32_t d = c * 64 + g * 16;            // 4 i + byte
+                if (d >= (uint32_t)D) return;
+                uint32_t words[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) words[2 * i + h] = f32x2_to_bf16x2_rne(v[2 * h][i] * by, v[2 * h + 1][i] * by);
+                u32x4 *const o = reinterpret_cast<u32x4 *>(p.out + row_bytes_at(pc.q.start + token, out_width, column + d, p.tiled));
+                o[0] = u32x4{words[0], words[1], words[2], words[3]};
+                o[1] = u32x4{words[4], words[5], words[6], words[7]};
+            } else {
+                *reinterpret_cast<u32x2v *>(p.out + row_bytes_at(pc.q.start + token, out_width, column + c * 16 + g * 4, p.tiled)) =
+                    u32x2v{f32x2_to_bf16x2_rne(v[0][0] * by, v[0][1] * by), f32x2_to_bf16x2_rne(v[0][2] * by, v[0][3] * by)};
+            }
+        };
         // ---- join: wavefronts 2, 3 into 0, 1, then 1 into 0; afterwards wavefront 0 has it all -----------------------------------
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) l[mt] = sum_over_quarters(l[mt]);
@@ -599,114 +639,122 @@ __global__ __launch_bounds__(256, MT <= 2 && D <= 128 ? 2 : 1) void paged_attent
         };
         join_waves();
         if (pc.parts > 1) {
-            constexpr uint32_t SLOT = (NACC * 16 + MT * 8) * 64;
+            constexpr uint32_t SLOT = (NACC + MT) * 1024;
             const bool fits = pc.slot + pc.parts <= p.slots;       // always, unless row_starts is out of order
             if (wave == 0 && fits) {
-                uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + lane * 8;
+                uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + lane * 16;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    put_pair(at + mt * 512, m[mt], l[mt]);
+                    put_quad(at + mt * 1024, f32x4{m[mt], l[mt], 0.f, 0.f});
 #pragma unroll
-                    for (int c = 0; c < S::COLS; ++c)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) put_pair(at + (MT + (mt * S::COLS + c) * 2 + h) * 512, acc[mt][c][2 * h], acc[mt][c][2 * h + 1]);
+                    for (int c = 0; c < S::COLS; ++c) put_quad(at + (MT + mt * S::COLS + c) * 1024, acc[mt][c]);
                 }
             }
             if (!fits || !last_of(p, pc, &flag)) { __syncthreads(); continue; }
-#pragma unroll
+            // A wavefront takes every fourth of the columns that a lane stores at once.  A load from another XCD's stores takes 1.7 us, so as many
+            // parts as there are registers for are on their way together; the last part stands in for those behind it
+            constexpr int TOGETHER = PACKED ? 4 : 1, ITEMS = S::COLS / TOGETHER, MINE = (ITEMS + 3) / 4, GROUP = MINE * TOGETHER <= 2 ? 8 : 4;
+            const uint8_t *const at = p.partial + (uint64_t)pc.slot * SLOT + lane * 16;
             for (int mt = 0; mt < MT; ++mt) {
-                m[mt] = -INFINITY; l[mt] = 0.f;
+                float top = -INFINITY, sum = 0.f;
+                f32x4 out[MINE][TOGETHER];
 #pragma unroll
-                for (int c = 0; c < S::COLS; ++c) acc[mt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-            for (uint32_t part = wave; part < pc.parts; part += 4) {
-                const uint8_t *const at = p.partial + (uint64_t)(pc.slot + part) * SLOT + lane * 8;
+                for (int n = 0; n < MINE; ++n)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    float m2, l2;
-                    get_pair(at + mt * 512, m2, l2);
-                    f32x4 other[S::COLS];
+                    for (int t = 0; t < TOGETHER; ++t) out[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (uint32_t part = 0; part < pc.parts; part += GROUP) {
+                    f32x4 ml[GROUP], o[GROUP][MINE][TOGETHER];
 #pragma unroll
-                    for (int c = 0; c < S::COLS; ++c)
+                    for (int k = 0; k < GROUP; ++k) {
+                        const uint8_t *const from = at + (uint64_t)min(part + k, pc.parts - 1) * SLOT;
+                        ml[k] = get_quad(from + mt * 1024);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float a, b2;
-                            get_pair(at + (MT + (mt * S::COLS + c) * 2 + h) * 512, a, b2);
-                            other[c][2 * h] = a;
-                            other[c][2 * h + 1] = b2;
-                        }
-                    take(mt, m2, l2, [&](int c) { return other[c]; });
-                }
-            }
-            join_waves();
-        }
-        if (wave == 0) {
+                        for (int n = 0; n < MINE; ++n)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                if ((uint32_t)(mt * 16 + x) >= pc.rows) continue;
-                const float by = l[mt] == 0.f ? 0.f : 1.f / l[mt];
-                const uint32_t t = pc.q.start + row_token[mt], column = head[mt] * D;
-                if constexpr (PACKED) {
-#pragma unroll
-                    for (int grp = 0; grp < S::COLS / 4; ++grp) {
-                        const uint32_t d = grp * 64 + g * 16;      // 16 neighbouring columns: 4 i + byte
-                        if (d >= (uint32_t)D) continue;
-                        uint32_t words[8];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) words[2 * i + h] = f32x2_to_bf16x2_rne(acc[mt][grp * 4 + 2 * h][i] * by, acc[mt][grp * 4 + 2 * h + 1][i] * by);
-                        u32x4 *const o = reinterpret_cast<u32x4 *>(p.out + row_bytes_at(t, out_width, column + d, p.tiled));
-                        o[0] = u32x4{words[0], words[1], words[2], words[3]};
-                        o[1] = u32x4{words[4], words[5], words[6], words[7]};
+                            for (int t = 0; t < TOGETHER; ++t) o[k][n][t] = get_quad(from + (MT + mt * S::COLS + min(n * 4 + wave, ITEMS - 1) * TOGETHER + t) * 1024);
                     }
-                } else {
+                    __builtin_amdgcn_sched_barrier(0);          // all of them, before the first is waited for
+                    float next = top;
 #pragma unroll
-                    for (int c = 0; c < S::COLS; ++c)
-                        *reinterpret_cast<u32x2v *>(p.out + row_bytes_at(t, out_width, column + c * 16 + g * 4, p.tiled)) =
-                            u32x2v{f32x2_to_bf16x2_rne(acc[mt][c][0] * by, acc[mt][c][1] * by), f32x2_to_bf16x2_rne(acc[mt][c][2] * by, acc[mt][c][3] * by)};
+                    for (int k = 0; k < GROUP; ++k) next = fmaxf(next, ml[k][0]);
+                    const float base = floor_of(next), shrink = __builtin_amdgcn_exp2f(top - base);
+                    top = next;
+                    sum *= shrink;
+#pragma unroll
+                    for (int n = 0; n < MINE; ++n)
+#pragma unroll
+                        for (int t = 0; t < TOGETHER; ++t) out[n][t] *= shrink;
+#pragma unroll
+                    for (int k = 0; k < GROUP; ++k) {
+                        if (part + k >= pc.parts) break;
+                        const float by = __builtin_amdgcn_exp2f(ml[k][0] - base);
+                        sum += ml[k][1] * by;
+#pragma unroll
+                        for (int n = 0; n < MINE; ++n)
+#pragma unroll
+                            for (int t = 0; t < TOGETHER; ++t) out[n][t] += o[k][n][t] * by;
+                    }
                 }
+#pragma unroll
+                for (int n = 0; n < MINE; ++n)
+                    if (n * 4 + wave < ITEMS) store(mt, n * 4 + wave, out[n], sum);
             }
+        } else if (wave == 0) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int c = 0; c < S::COLS / (PACKED ? 4 : 1); ++c) store(mt, c, &acc[mt][c * (PACKED ? 4 : 1)], l[mt]);
         }
         __syncthreads();                                        // LDS is the next piece's
     }
+    if (p.zero_rows) clear_rows(p, D);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Many rows (chunks, prompts): bound by the matrix cores.  Eight wavefronts of 32 rows each share a unit of 256 rows and its keys and values,
-// which go through two LDS buffers of 64 tokens (32 where heads have 256 elements) as bf16; block floats are expanded on the way,
-// once for all 256 rows.  v_mfma_f32_32x32x16_bf16.
+// Many rows (chunks, prompts): bound by the matrix cores.  Eight wavefronts (four where heads have 256 elements) of 32 rows each share a
+// unit and its keys and values, 64 tokens (32) a step, which go through LDS as bf16; block floats are expanded on the way,
+// once for all rows of the unit.  v_mfma_f32_32x32x16_bf16.
+//   phases   a step is a phase of vector work (masks, softmax, the next tokens into LDS) and one of matrix work (values of this step, then
+//            keys of the next).  The two wavefronts of a SIMD are a phase apart, kept there by a barrier after every phase: one has the
+//            matrix cores while the other has the vector ALU.  In step, both wait for the same unit: [512 new tokens
+//            behind 7680], 32 heads, 105 us against the time below
+//   LDS      three buffers each for keys and values.  In vector phase i the keys of step i + 2 and the values of step i + 1 are written, read by
+//            either half of the workgroup until the end of the matrix phases i + 1, which are one phase apart
 //   keys     16-byte chunk (row r, half h) of a face lies at r * 32 + (h ^ (r / 8)) * 16: what a pass of a ds_read_b128 touches lies
 //            in different banks
 //   values   read transposed (ds_read_b64_tr_b16); the 128-byte halves of the row groups are exchanged in the right-hand faces, for the
 //            same reason
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int D, bool PACKED> struct TileShape {
+    static constexpr int WAVES = D == 256 ? 4 : 8;              // heads of 256 elements need all the registers of their SIMD
     static constexpr int NB = D == 256 ? 1 : 2;                 // blocks of 32 tokens per step
     static constexpr int BLOCK = D * 64, HALF = NB * BLOCK;     // bytes of a block, and of the keys or the values of a step
     static constexpr int TILE_BYTES = PACKED ? 1088 : 2048, ROW_BYTES = D / 32 * TILE_BYTES;
     // pieces of a step's keys, and of its values: 16 bytes of bf16, or a face row of block floats
-    static constexpr int PIECES = PACKED ? NB * 2 * D : NB * D * 4, EACH = (PIECES + 511) / 512;
+    static constexpr int PIECES = PACKED ? NB * 2 * D : NB * D * 4, EACH = (PIECES + WAVES * 64 - 1) / (WAVES * 64);
 };
 
+// End of a phase: what this wavefront has written to LDS is there.  Loads from memory stay in flight.
+__device__ __forceinline__ void end_phase() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 template <int D, bool PACKED>
-__global__ __launch_bounds__(512) void paged_attention_tile_kernel(const AttentionDev p) {
+__global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_attention_tile_kernel(const AttentionDev p) {
     using S = TileShape<D, PACKED>;
-    constexpr int ROWS = 256, NB = S::NB, SLABS = D / 16, DB = D / 32;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * S::HALF];                // [buffer][keys | values]
-    __shared__ uint64_t wave_sums[8];
+    constexpr int WAVES = S::WAVES, THREADS = WAVES * 64, ROWS = WAVES * 32, NB = S::NB, SLABS = D / 16, DB = D / 32;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[6 * S::HALF];                // keys, then values, three buffers each
     __shared__ uint32_t flag;
-    extern __shared__ uint32_t tables[];
     const int lane = threadIdx.x & 63, c = lane & 31, kh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool second = WAVES == 8 && wave >= 4;                // the half that runs a phase behind
     typedef __attribute__((address_space(3))) uint8_t lds_byte;
-    if (p.zero_rows) clear_rows(p, D);
-    const Plan plan = make_plan<512, ROWS, NB>(p, tables, tables + p.requests + 1, wave_sums);
+    const Plan plan = make_plan<ROWS, NB>(p);
     const uint32_t out_width = p.heads * D;
 
     for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
-        const Piece pc = piece_at<ROWS>(p, plan, tables, tables + p.requests + 1, index);
-        if (pc.part >= pc.parts) continue;
+        Piece pc;
+        if (!piece_at<ROWS>(p, plan, index, pc)) continue;
         const bool idle = (uint32_t)wave * 32 >= pc.rows;       // a wavefront without rows only moves keys and values
         const uint32_t rho = pc.row0 + min((uint32_t)(wave * 32 + c), pc.rows - 1);
         const uint32_t row_token = rho / p.group, head = pc.kv * p.group + rho % p.group;
@@ -716,7 +764,7 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
             u32x4 w = *reinterpret_cast<const u32x4 *>(p.rows + row_bytes_at(pc.q.start + row_token, p.width, p.query_column + head * D + s * 16 + kh * 8, p.tiled));
             q[s] = __builtin_bit_cast(bf16x8, w ^ u32x4{p.flip, p.flip, p.flip, p.flip});
         }
-        f32x16 acc[DB];
+        f32x16 acc[DB], s[NB];
         float m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -728,13 +776,24 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
         const uint32_t unit_pos_min = pc.q.cached + pc.token0, unit_first_max = first_seen(p, pos_max);
         const uint32_t wave_pos_min = pc.q.cached + (pc.row0 + min((uint32_t)wave * 32, pc.rows - 1)) / p.group, wave_pos_max = pc.q.cached + (pc.row0 + min((uint32_t)wave * 32 + 31, pc.rows - 1)) / p.group;
         const uint32_t wave_first_min = first_seen(p, wave_pos_min), wave_first_max = first_seen(p, wave_pos_max);
+        const uint32_t steps = (pc.end - pc.begin + NB - 1) / NB;
+        auto token_of = [&](uint32_t step) { return (pc.begin + step * NB) * 32; };
+        // steps [step_from, step_to) have something for this wavefront
+        const uint32_t step_to = idle || wave_pos_max < token_of(0) ? 0 : min((wave_pos_max / 32 - pc.begin) / NB + 1, steps);
+        const uint32_t step_from = wave_first_min / 32 > pc.begin ? min((wave_first_min / 32 - pc.begin) / NB, step_to) : 0;
+        // rows of the unit see different parts of the step
+        auto uneven = [&](uint32_t step) { return pc.token0 != pc.token1 && !(token_of(step) >= unit_first_max && token_of(step) + NB * 32 - 1 <= unit_pos_min); };
 
-        Pages<1> entries;
+        // ---- keys and values: memory -> registers -> LDS ------------------------------------------------------------------------------
+        Blocks<1, S::ROW_BYTES> blocks;
+        uint64_t keys_at[NB], values_at[NB];                    // of the step whose keys, and whose values, are asked for next
+        uint32_t have = 0;                                      // which blocks of four steps, from the current one on, have pages: bit NB * step + block
         u32x4 kreg[S::EACH], vreg[S::EACH];
         uint32_t kexp[S::EACH], vexp[S::EACH];
+        const uint32_t thread = threadIdx.x & (THREADS - 1);    // with its range for the compiler to see
         // piece i of this thread: block of the step, byte in the block's tiles (keys and values alike), token of the block
         auto place = [&](int i, uint32_t &block, uint32_t &from, uint32_t &token, uint32_t &exponent) __attribute__((always_inline)) {
-            const uint32_t n = min(threadIdx.x + i * 512u, (uint32_t)S::PIECES - 1), per_block = S::PIECES / NB;
+            const uint32_t n = min(thread + i * (uint32_t)THREADS, (uint32_t)S::PIECES - 1), per_block = S::PIECES / NB;
             block = n / per_block;
             const uint32_t within = n % per_block;
             if (PACKED) {
@@ -748,188 +807,272 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
                 token = (within >> 6 & 1) * 16 + (within >> 1 & 15);
             }
         };
-        uint64_t rows_of[NB];
-        bool there[NB], ready[NB];                              // of the step that is loaded, and of the one that lies in LDS
-        auto load = [&](const uint8_t *tensor, u32x4 (&v)[S::EACH], uint32_t (&e)[S::EACH]) __attribute__((always_inline)) {
+        auto load = [&](const uint8_t *tensor, const uint64_t (&at)[NB], u32x4 (&v)[S::EACH], uint32_t (&e)[S::EACH]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < S::EACH; ++i) {
                 uint32_t block, from, token, exponent;
                 place(i, block, from, token, exponent);
-                const uint8_t *base = tensor + (NB == 2 && block ? rows_of[NB - 1] : rows_of[0]) * S::ROW_BYTES;
+                const uint8_t *base = tensor + (NB == 2 && block ? at[NB - 1] : at[0]);
                 v[i] = *reinterpret_cast<const u32x4 *>(base + from);
                 e[i] = PACKED ? base[exponent] : 0u;
             }
         };
-        auto request = [&](uint32_t step) __attribute__((always_inline)) {
-            const uint32_t i = step * NB;
-            if ((i & 63) == 0) entries.load(p, pc, pc.begin + i);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) there[b] = entries.at(p, pc.kv, (i + b) & 63, rows_of[b]);
-            load(p.keys, kreg, kexp);
-            load(p.values, vreg, vexp);
+        // where the keys of `step` lie, which is `ahead` of the current one; behind the last step, page 0
+        auto refill = [&](uint32_t step) __attribute__((always_inline)) {
+            if ((step * NB & 63) == 0) blocks.load(p, pc, pc.begin + step * NB);
         };
-        // Keys and values of the loaded step into LDS
-        auto put = [&](uint32_t buffer, bool keys) __attribute__((always_inline)) {
-            lds_byte *const to = (lds_byte *)lds + buffer * 2 * S::HALF;
+        auto look_up = [&](uint32_t step, int ahead) __attribute__((always_inline)) {
+            const uint32_t i = step * NB & 63;
+            have |= (uint32_t)(blocks.pages >> i & ((1u << NB) - 1)) << (ahead * NB);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) keys_at[b] = blocks.at(i + b);
+        };
+        auto put = [&](uint32_t to, const u32x4 (&v)[S::EACH], const uint32_t (&e)[S::EACH], bool values) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < S::EACH; ++i) {
-                if (S::PIECES % 512 && threadIdx.x + i * 512u >= (uint32_t)S::PIECES) break;
-                const uint32_t n = threadIdx.x + i * 512u, block = n / (S::PIECES / NB), within = n % (S::PIECES / NB);
+                const uint32_t n = thread + i * (uint32_t)THREADS, block = n / (S::PIECES / NB), within = n % (S::PIECES / NB);
+                if (S::PIECES % THREADS && n >= (uint32_t)S::PIECES) break;
+                lds_byte *const face_at = (lds_byte *)lds + to + block * S::BLOCK + (PACKED ? within >> 4 : within >> 5) * 512;
+                // 16-byte chunk of a face, and where it goes: see above
+                auto chunk = [&](uint32_t at, uint32_t face, const u32x4 &w) __attribute__((always_inline)) {
+                    const uint32_t where = values ? at ^ ((face & 1) * 8) : (at & ~1u) | ((at & 1) ^ (at >> 4));
+                    *(__attribute__((address_space(3))) u32x4 *)(face_at + where * 16) = w;
+                };
                 if constexpr (PACKED) {
-                    const uint32_t face = within >> 4 & 3, r = within & 15, base = block * S::BLOCK + (within >> 4) * 512;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + ((h ^ (r >> 3)) * 16)) = expand8(kreg[i][2 * h], kreg[i][2 * h + 1], block_scale(kexp[i]));
-                        *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + (((r * 2 + h) ^ ((face & 1) * 8)) * 16)) = expand8(vreg[i][2 * h], vreg[i][2 * h + 1], block_scale(vexp[i]));
-                    }
+                    const float scale = block_scale(e[i]);
+                    chunk((within & 15) * 2, within >> 4, expand8(v[i][0], v[i][1], scale));
+                    chunk((within & 15) * 2 + 1, within >> 4, expand8(v[i][2], v[i][3], scale));
                 } else {
-                    const uint32_t face = within >> 5 & 3, in_face = within & 31, r = in_face >> 1, base = block * S::BLOCK + (within >> 5) * 512;
-                    if (keys) *(__attribute__((address_space(3))) u32x4 *)(to + base + r * 32 + (((in_face & 1) ^ (r >> 3)) * 16)) = kreg[i];
-                    *(__attribute__((address_space(3))) u32x4 *)(to + S::HALF + base + ((in_face ^ ((face & 1) * 8)) * 16)) = vreg[i];
+                    chunk(within & 31, within >> 5, v[i]);
                 }
             }
         };
         // bf16 values: zeros for tokens that no row of the unit sees
-        auto clear_values = [&](uint32_t token0, const bool (&pages)[NB]) __attribute__((always_inline)) {
+        auto clear_values = [&](uint32_t token0, uint32_t pages) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < S::EACH; ++i) {
                 uint32_t block, from, token, exponent;
                 place(i, block, from, token, exponent);
                 const uint32_t t = token0 + block * 32 + token;
-                if (t < first_min || t > pos_max || !(NB == 2 && block ? pages[NB - 1] : pages[0])) vreg[i] = u32x4{0, 0, 0, 0};
+                if (t < first_min || t > pos_max || !(pages >> block & 1)) vreg[i] = u32x4{0, 0, 0, 0};
             }
         };
-
-        const uint32_t steps = (pc.end - pc.begin + NB - 1) / NB;
-        bool odd = false;                                       // values of the step that are not finite, and that some rows see and others do not
-        auto fill = [&](uint32_t step) __attribute__((always_inline)) {
-            const uint32_t token0 = (pc.begin + step * NB) * 32, last = token0 + NB * 32 - 1;
-            bool look = false;
-            uint32_t any = 0;
+        uint32_t odd = 0;                                       // values that are not finite, in steps that rows see differently
+        auto put_values = [&](uint32_t to, uint32_t step, int ahead) __attribute__((always_inline)) {
             if constexpr (!PACKED) {
-                if (__builtin_expect(!(token0 >= first_min && last <= pos_max && there[0] && there[NB - 1]), 0)) clear_values(token0, there);
-                look = pc.token0 != pc.token1 && !(token0 >= unit_first_max && last <= unit_pos_min);
-                if (__builtin_expect(look, 0)) {
+                const uint32_t token0 = token_of(step), pages = have >> (ahead * NB) & ((1u << NB) - 1);
+                if (__builtin_expect(!(token0 >= first_min && token0 + NB * 32 - 1 <= pos_max && pages == (1u << NB) - 1), 0)) clear_values(token0, pages);
+                if (__builtin_expect(uneven(step), 0)) {
 #pragma unroll
                     for (int i = 0; i < S::EACH; ++i) {
                         const u32x4 taken = vreg[i] ^ pick(vreg[i], KEEP_FINITE);
                         vreg[i] ^= taken;
-                        any |= taken[0] | taken[1] | taken[2] | taken[3];
+                        odd |= taken[0] | taken[1] | taken[2] | taken[3];
                     }
                 }
             }
-            put(step & 1, true);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) ready[b] = there[b];
-            if (look) odd = __syncthreads_or(any != 0);
-            else { odd = false; __syncthreads(); }
+            put(to, vreg, vexp, true);
         };
+
+        // ---- products -----------------------------------------------------------------------------------------------------------------
+        const uint32_t key_at = (c >> 4) * 1024 + (c & 15) * 32 + ((kh ^ (c >> 3 & 1)) * 16);
+        const uint32_t fc = lane >> 4 & 1, value_at = 3 * S::HALF + fc * 512 + ((kh * 128 + (lane & 15) * 8) ^ (fc * 128));
+        constexpr int N_KEYS = NB * SLABS, N_VALUES = DB * 2 * NB;
+        auto key_operand = [&](uint32_t buffer, int i) __attribute__((always_inline)) {
+            const int b = i / SLABS, sl = i % SLABS;
+            return __builtin_bit_cast(bf16x8, *(__attribute__((address_space(3))) u32x4 *)((lds_byte *)lds + buffer + key_at + b * S::BLOCK + (sl >> 1) * 2048 + (sl & 1) * 512));
+        };
+        // elements 32 (i / 2 NB) .. + 31, tokens 16 (i % 2 NB) .. + 15 of the step
+        auto value_operand = [&](uint32_t buffer, int i) __attribute__((always_inline)) {
+            const int d = i / (2 * NB), b = i / 2 % NB, h = i % 2;
+            union { s16x4 half[2]; bf16x8 v; } u;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                u.half[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)((lds_byte *)lds + buffer + value_at + b * S::BLOCK + d * 2048 + h * 1024 + r * 256));
+            return u.v;
+        };
+        bf16x8 ring[AHEAD], w[NB][2];
+        auto clear_scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+        };
+        auto multiply_keys = [&](uint32_t buffer) __attribute__((always_inline)) {         // the ring holds the first operands
+            clear_scores();
+#pragma unroll
+            for (int i = 0; i < N_KEYS; ++i) {
+                s[i / SLABS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % AHEAD], q[i % SLABS], s[i / SLABS], 0, 0, 0);
+                if (i + AHEAD < N_KEYS) ring[i % AHEAD] = key_operand(buffer, i + AHEAD);
+                keep_order();
+            }
+        };
+        // ... and is left with the first operands of the keys in `next`
+        auto multiply_values = [&](uint32_t buffer, uint32_t next) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < N_VALUES; ++i) {
+                acc[i / (2 * NB)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % AHEAD], w[i / 2 % NB][i % 2], acc[i / (2 * NB)], 0, 0, 0);
+                ring[i % AHEAD] = i + AHEAD < N_VALUES ? value_operand(buffer, i + AHEAD) : key_operand(next, i + AHEAD - N_VALUES);
+                keep_order();
+            }
+        };
+        static_assert(N_VALUES % AHEAD == 0, "the ring starts over with the keys");
+        // weights rounded to bf16, or what the rounding took off; their sum goes to l
+        auto weights = [&](bool rest) __attribute__((always_inline)) {
+            const float base = floor_of(m);
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    union { uint32_t words[4]; bf16x8 v; } u;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float e[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[b][h * 8 + 2 * i + j], p.scale, -base));
+                        uint32_t rounded = f32x2_to_bf16x2_rne(e[0], e[1]);
+                        if (rest) rounded = f32x2_to_bf16x2_rne(e[0] - __uint_as_float(rounded << 16), e[1] - __uint_as_float(rounded & 0xffff0000u));
+                        u.words[i] = rounded;
+                        l = add_pair(rounded, l);
+                    }
+                    w[b][h] = u.v;
+                }
+        };
+
+        uint32_t buffer[3] = {0, S::HALF, 2 * S::HALF};         // of the current step, the next one, the one after
         if (steps) {
-            request(0);
-            fill(0);
+            u32x4 k1[S::EACH];
+            uint32_t e1[S::EACH];
+            refill(0);
+            look_up(0, 0);
+            load(p.keys, keys_at, kreg, kexp);
+            load(p.values, keys_at, vreg, vexp);
+            look_up(1, 1);
+            load(p.keys, keys_at, k1, e1);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) values_at[b] = keys_at[b];
+            put(buffer[0], kreg, kexp, false);
+            put_values(buffer[0] + 3 * S::HALF, 0, 0);
+            put(buffer[1], k1, e1, false);
+            load(p.values, values_at, vreg, vexp);
+            look_up(2, 2);
+            load(p.keys, keys_at, kreg, kexp);
+            __syncthreads();
+            if (second) end_phase();
         }
-        const uint32_t key_at = (c >> 4) * 1024 + (c & 15) * 32 + ((kh ^ (c >> 3 & 1)) * 16);                     // + slab
-        const uint32_t fc = lane >> 4 & 1, value_at = S::HALF + fc * 512 + ((kh * 128 + (lane & 15) * 8) ^ (fc * 128));
-        for (uint32_t step = 0; step < steps; ++step) {
-            if (step + 1 < steps) request(step + 1);
-            const uint32_t token0 = (pc.begin + step * NB) * 32, last = token0 + NB * 32 - 1;
-            lds_byte *const from = (lds_byte *)lds + (step & 1) * 2 * S::HALF;
-            const bool skip = idle || token0 > wave_pos_max || last < wave_first_min;
-            bf16x8 w[NB][2];
-            f32x16 s[NB];
-            // weights rounded to bf16, or what the rounding took off; their sum goes to l
-            auto weights = [&](bool rest) __attribute__((always_inline)) {
-                const float base = floor_of(m);
+        // what a step does for the steps behind it: in its vector phase, and, once the registers are free, in its matrix phase
+        // (unless there are none: then it moves what is not looked at, which is less work than asking)
+        auto bring = [&](uint32_t step) __attribute__((always_inline)) {
+            refill(step + 3);
+            put_values(buffer[1] + 3 * S::HALF, step + 1, 1);
+            put(buffer[2], kreg, kexp, false);
+        };
+        auto ask = [&](uint32_t step) __attribute__((always_inline)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) values_at[b] = keys_at[b];
+            load(p.values, values_at, vreg, vexp);
+            look_up(step + 3, 3);
+            load(p.keys, keys_at, kreg, kexp);
+        };
+        auto turn = [&]() __attribute__((always_inline)) {
+            have >>= NB;
+            const uint32_t done = buffer[0];
+            buffer[0] = buffer[1]; buffer[1] = buffer[2]; buffer[2] = done;
+        };
+        uint32_t step = 0;
+        auto pass_by = [&](uint32_t to) __attribute__((always_inline)) {                    // steps with nothing for this wavefront
+            for (; step < to; ++step) {
+                bring(step);
+                end_phase();
+                ask(step);
+                end_phase();
+                turn();
+            }
+        };
+        pass_by(step_from);
+        if (step_from < step_to) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) ring[i] = key_operand(buffer[0], i);
+            multiply_keys(buffer[0]);
+        }
+        for (; step < step_to; ++step) {
+            // ---- vector work ------------------------------------------------------------------------------------------------------------
+            const uint32_t token0 = token_of(step), last = token0 + NB * 32 - 1;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) ring[i] = value_operand(buffer[0], i);
+            keep_order();
+            if (__builtin_expect(!(token0 >= wave_first_max && last <= wave_pos_min && (have & ((1u << NB) - 1)) == (1u << NB) - 1), 0)) {
+                // against constants: the tokens' numbers would be held in registers over all steps
+                const int from = (int)(first - token0) - kh * 4, to = (int)(pos - token0) - kh * 4;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        union { uint32_t words[4]; bf16x8 v; } u;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float e[2];
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[b][h * 8 + 2 * i + j], p.scale, -base));
-                            uint32_t rounded = f32x2_to_bf16x2_rne(e[0], e[1]);
-                            if (rest) rounded = f32x2_to_bf16x2_rne(e[0] - __uint_as_float(rounded << 16), e[1] - __uint_as_float(rounded & 0xffff0000u));
-                            u.words[i] = rounded;
-                            l = add_pair(rounded, l);
-                        }
-                        w[b][h] = u.v;
+                    for (int i = 0; i < 16; ++i) {
+                        const int t = b * 32 + (i >> 2) * 8 + (i & 3);
+                        if (t < from || t > to || !(have >> b & 1)) s[b][i] = -INFINITY;
                     }
-            };
-            if (!skip) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-                    for (int sl = 0; sl < SLABS; ++sl) {
-                        const u32x4 k = *(__attribute__((address_space(3))) u32x4 *)(from + key_at + b * S::BLOCK + (sl >> 1) * 2048 + (sl & 1) * 512);
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k), q[sl], s[b], 0, 0, 0);
-                    }
-                }
-                if (!(token0 >= wave_first_max && last <= wave_pos_min && ready[0] && ready[NB - 1])) {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint32_t t = token0 + b * 32 + (i >> 2) * 8 + kh * 4 + (i & 3);
-                            if (t < first || t > pos || !ready[b]) s[b][i] = -INFINITY;
-                        }
-                }
-                float top = s[0][0];
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-                top = max_over_halves(top) * p.scale;
-                if (__ballot(top > m + LAZY || (m == -INFINITY && top > m))) {
-                    const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - floor_of(next));
-                    m = next;
-                    l *= shrink;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] *= shrink;
-                }
             }
-            auto value_operand = [&](int d, int b, int h) __attribute__((always_inline)) {
-                union { s16x4 half[2]; bf16x8 v; } u;
+            float top = s[0][0];
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    u.half[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(from + value_at + b * S::BLOCK + d * 2048 + h * 1024 + r * 256));
-                return u.v;
-            };
-            const int passes = skip ? 0 : last >= wave_pos_min ? 2 : 1;
-            for (int pass = 0; pass < passes; ++pass) {
-                weights(pass != 0);
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+            top = max_over_halves(top) * p.scale;
+            if (__ballot(top > m + LAZY || (m == -INFINITY && top > m))) {
+                const float next = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - floor_of(next));
+                m = next;
+                l *= shrink;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_operand(d, b, h), w[b][h], acc[d], 0, 0, 0);
+                for (int d = 0; d < DB; ++d) acc[d] *= shrink;
             }
-            if (__builtin_expect(odd, 0)) {
-                if constexpr (!PACKED) {
-                    // the step behind this one waits in registers, and is loaded again afterwards
-                    uint64_t rows_next[NB];
+            weights(false);
+            // here, and not where they are used, in the other phase
+#pragma unroll
+            for (int b = 0; b < NB; ++b) asm volatile("" : "+v"(w[b][0]), "+v"(w[b][1]));
+            bring(step);
+            end_phase();
+            // ---- matrix work ------------------------------------------------------------------------------------------------------------
+            ask(step);
+            __builtin_amdgcn_s_setprio(1);
+            multiply_values(buffer[0], buffer[1]);
+            if (__builtin_expect(last >= wave_pos_min, 0)) {
+                weights(true);
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) ring[i] = value_operand(buffer[0], i);
+                multiply_values(buffer[0], buffer[1]);
+            }
+            multiply_keys(buffer[1]);                           // behind the last step: of whatever is there, and nobody looks
+            __builtin_amdgcn_s_setprio(0);
+            end_phase();
+            turn();
+        }
+        pass_by(steps);
+        if (steps && WAVES == 8 && !second) end_phase();        // both halves have passed as many barriers
+
+        if constexpr (!PACKED) {
+            if (__builtin_expect(pc.token0 != pc.token1 && __syncthreads_or(odd != 0), 0)) {
+                // once more over the steps that rows see differently: ones in place of the values that were taken out, counted by those who see them
+                for (step = 0; step < steps; ++step) {
+                    if (!uneven(step)) continue;
+                    uint32_t pages = 0;
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        rows_next[b] = rows_of[b];
                         const uint32_t block = pc.begin + step * NB + b;
                         int32_t page = block < pc.end ? p.table[(uint64_t)pc.r * p.max_pages + block / p.page_blocks] : -1;
+                        pages |= (uint32_t)((uint32_t)page < p.pages) << b;
                         if ((uint32_t)page >= p.pages) page = 0;
-                        rows_of[b] = ((uint64_t)page * p.kv_heads + pc.kv) * p.page_blocks + block % p.page_blocks;
+                        values_at[b] = (((uint64_t)page * p.kv_heads + pc.kv) * p.page_blocks + block % p.page_blocks) * S::ROW_BYTES;
                     }
                     for (int down = 0; down < 2; ++down) {
-                        load(p.values, vreg, vexp);
-                        clear_values(token0, ready);
+                        load(p.values, values_at, vreg, vexp);
+                        clear_values(token_of(step), pages);
 #pragma unroll
                         for (int i = 0; i < S::EACH; ++i) vreg[i] = pick(vreg[i], down ? ONES_DOWN : ONES_UP);
                         __syncthreads();
-                        put(step & 1, false);
+                        put(3 * S::HALF, vreg, vexp, true);
                         __syncthreads();
-                        if (skip) continue;
+                        if (step < step_from || step >= step_to) continue;
+                        const int from = (int)(first - token_of(step)) - kh * 4, to = (int)(pos - token_of(step)) - kh * 4;
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -937,40 +1080,36 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
                                 union { uint32_t words[4]; bf16x8 v; } seen;
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
-                                    const uint32_t t = token0 + b * 32 + h * 16 + (i >> 1) * 8 + kh * 4 + (i & 1) * 2;
-                                    seen.words[i] = (t >= first && t <= pos ? 0x3f80u : 0u) | (t + 1 >= first && t + 1 <= pos ? 0x3f800000u : 0u);
+                                    const int t = b * 32 + h * 16 + (i >> 1) * 8 + (i & 1) * 2;
+                                    seen.words[i] = (t >= from && t <= to ? 0x3f80u : 0u) | (t + 1 >= from && t + 1 <= to ? 0x3f800000u : 0u);
                                 }
 #pragma unroll
                                 for (int d = 0; d < DB; ++d) {
                                     f32x16 count;
 #pragma unroll
                                     for (int i = 0; i < 16; ++i) count[i] = 0.f;
-                                    count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_operand(d, b, h), seen.v, count, 0, 0, 0);
+                                    count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_operand(0, (d * NB + b) * 2 + h), seen.v, count, 0, 0, 0);
 #pragma unroll
                                     for (int i = 0; i < 16; ++i)
                                         if (count[i] > 0.f) acc[d][i] += down ? -INFINITY : INFINITY;
                                 }
                             }
                     }
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) rows_of[b] = rows_next[b];
-                    if (step + 1 < steps) load(p.values, vreg, vexp);
                 }
             }
-            if (step + 1 < steps) fill(step + 1);
         }
 
         l = sum_over_halves(l);
         if (pc.parts > 1) {
-            constexpr uint32_t PART = (DB * 8 + 1) * 512, SLOT = 8 * PART;             // of a wavefront, of a workgroup
+            constexpr uint32_t PART = (DB * 4 + 1) * 1024, SLOT = WAVES * PART;        // of a wavefront, of a workgroup
             const bool fits = pc.slot + pc.parts <= p.slots;   // always, unless row_starts is out of order
             if (fits && !idle) {
-                uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + wave * PART + lane * 8;
-                put_pair(at, m, l);
+                uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + wave * PART + lane * 16;
+                put_quad(at, f32x4{m, l, 0.f, 0.f});
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) put_pair(at + (1 + d * 8 + i) * 512, acc[d][2 * i], acc[d][2 * i + 1]);
+                    for (int i = 0; i < 4; ++i) put_quad(at + (1 + d * 4 + i) * 1024, f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]});
             }
             if (!fits || !last_of(p, pc, &flag)) { __syncthreads(); continue; }
             m = -INFINITY; l = 0.f;
@@ -978,22 +1117,28 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-            for (uint32_t part = 0; part < (idle ? 0 : pc.parts); ++part) {
-                const uint8_t *const at = p.partial + (uint64_t)(pc.slot + part) * SLOT + wave * PART + lane * 8;
-                float m2, l2;
-                get_pair(at, m2, l2);
-                const float next = fmaxf(m, m2), by = __builtin_amdgcn_exp2f(m - floor_of(next)), by2 = __builtin_amdgcn_exp2f(m2 - floor_of(next));
-                m = next;
-                l = l * by + l2 * by2;
+            if (!idle) {
+                // Two parts on their way together: a load from another XCD's stores takes 1.7 us.  The last part stands in for one behind it
+                const uint8_t *const at = p.partial + (uint64_t)pc.slot * SLOT + wave * PART + lane * 16;
+                for (uint32_t part = 0; part < pc.parts; part += 2) {
+                    f32x4 ml[2], o[2][DB * 4];
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
+                    for (int k = 0; k < 2; ++k) {
+                        const uint8_t *const from = at + (uint64_t)min(part + k, pc.parts - 1) * SLOT;
+                        ml[k] = get_quad(from);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float a, b;
-                        get_pair(at + (1 + d * 8 + i) * 512, a, b);
-                        acc[d][2 * i] = acc[d][2 * i] * by + a * by2;
-                        acc[d][2 * i + 1] = acc[d][2 * i + 1] * by + b * by2;
+                        for (int i = 0; i < DB * 4; ++i) o[k][i] = get_quad(from + (1 + i) * 1024);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                    const float next = fmaxf(m, fmaxf(ml[0][0], ml[1][0])), base = floor_of(next), by = __builtin_amdgcn_exp2f(m - base);
+                    const float by0 = __builtin_amdgcn_exp2f(ml[0][0] - base), by1 = part + 1 < pc.parts ? __builtin_amdgcn_exp2f(ml[1][0] - base) : 0.f;
+                    m = next;
+                    l = l * by + ml[0][1] * by0 + ml[1][1] * by1;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] * by + o[0][d * 4 + i / 4][i & 3] * by0 + (part + 1 < pc.parts ? o[1][d * 4 + i / 4][i & 3] * by1 : 0.f);
+                }
             }
         }
         // columns 8 (i / 4) + 4 kh + i % 4 of 32: the swap leaves columns 8 kh .. 8 kh + 7 of a face row in each lane
@@ -1010,6 +1155,7 @@ __global__ __launch_bounds__(512) void paged_attention_tile_kernel(const Attenti
             }
         __syncthreads();                                        // LDS is the next piece's
     }
+    if (p.zero_rows) clear_rows(p, D);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
@@ -1026,23 +1172,21 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     const uint32_t group = heads / c.kv_heads;
     const uint64_t rows = (uint64_t)((tokens + requests - 1) / std::max(requests, 1u)) * group;       // of an average request
     const uint32_t most = c.head_dim == 64 ? 5 : c.head_dim == 256 ? 2 : 4;
-    const uint64_t wanted = (std::max<uint64_t>(rows, 1) + 15) / 16;
-    r.mt = wanted <= 1 ? 1 : wanted <= 2 ? 2 : most;
-    const bool few = (uint64_t)tokens <= 8ull * requests || (uint64_t)tokens * group <= r.mt * 16, many = rows >= 256;
-    r.tile = !few;
-    if (many) r.mt = 0;
-    if (requests == 1) {                   // its length is known
-        r.tile = rows > most * 16;
-        if (r.tile) r.mt = 0;
-    }
+    auto tiles_for = [&](uint64_t n) { return n <= 16 ? 1u : n <= 32 ? 2u : most; };
+    // Few tokens per request: the kernel for few rows takes them all, in tiles for an average request.  Many: the other takes them all.  In
+    // between the step is a mixture: single tokens go to the one, and every request that is more than its tile to the other.
+    r.mt = tiles_for(rows);
+    if (requests == 1) r.tile = rows > most * 16;              // its length is known
+    else r.tile = tokens > 8ull * requests && (uint64_t)tokens * group > r.mt * 16;
+    if (r.tile) r.mt = requests == 1 || rows >= 256 ? 0 : tiles_for(group);
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
     if (r.mt <= 2 && c.head_dim <= 128) r.stream_target = 512;
     if (r.mt) {
         const size_t cols = packed ? (c.head_dim + 63) / 64 * 4 : c.head_dim / 16;
-        r.slot_bytes = (r.mt * cols * 16 + r.mt * 8) * 64;
+        r.slot_bytes = (r.mt * cols + r.mt) * 1024;
         r.slots = 2 * (size_t)r.stream_target * r.slot_bytes;
     }
-    if (r.tile) r.slots = std::max(r.slots, 2 * (size_t)r.tile_target * 8 * ((size_t)c.head_dim / 32 * 8 + 1) * 512);
+    if (r.tile) r.slots = std::max(r.slots, 2 * (size_t)r.tile_target * (c.head_dim == 256 ? 4 : 8) * ((size_t)c.head_dim / 32 * 4 + 1) * 1024);
     return r;
 }
 
@@ -1052,18 +1196,19 @@ int clear_counters(void *at, hipStream_t st) {
     return check_launch("clear_counters_kernel");
 }
 
-template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, size_t lds, hipStream_t st) {
-    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(p.target), dim3(256), lds, st, p);
-    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(p.target), dim3(256), lds, st, p);
+template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, hipStream_t st) {
+    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(p.target), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(p.target), dim3(256), 0, st, p);
 }
-template <int D, int MOST> void launch_stream(const AttentionDev &p, uint32_t mt, bool packed, size_t lds, hipStream_t st) {
-    if (mt == 1) launch_stream<D, 1>(p, packed, lds, st);
-    else if (mt == 2) launch_stream<D, 2>(p, packed, lds, st);
-    else launch_stream<D, MOST>(p, packed, lds, st);
+template <int D, int MOST> void launch_stream(const AttentionDev &p, uint32_t mt, bool packed, hipStream_t st) {
+    if (mt == 1) launch_stream<D, 1>(p, packed, st);
+    else if (mt == 2) launch_stream<D, 2>(p, packed, st);
+    else launch_stream<D, MOST>(p, packed, st);
 }
-template <int D> void launch_tile(const AttentionDev &p, bool packed, size_t lds, hipStream_t st) {
-    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(p.target), dim3(512), lds, st, p);
-    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(p.target), dim3(512), lds, st, p);
+template <int D> void launch_tile(const AttentionDev &p, bool packed, hipStream_t st) {
+    constexpr uint32_t threads = TileShape<D, false>::WAVES * 64;
+    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(p.target), dim3(threads), 0, st, p);
+    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(p.target), dim3(threads), 0, st, p);
 }
 }  // namespace
 
@@ -1105,16 +1250,15 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     p.counters = (uint32_t *)memory;
     p.partial = memory + COUNTERS * 4;
     p.zero_rows = 1;
-    const size_t lds = (2 * (size_t)p.requests + 1) * 4;
     if (route.mt) {
         p.least_rows = 1;
         p.most_rows = route.tile ? route.mt * 16 : 0xffffffffu;
         p.target = route.stream_target; p.slots = 2 * p.target;
         switch (c.head_dim) {
-            case 64: launch_stream<64, 5>(p, route.mt, packed, lds, st); break;
-            case 96: launch_stream<96, 4>(p, route.mt, packed, lds, st); break;
-            case 128: launch_stream<128, 4>(p, route.mt, packed, lds, st); break;
-            default: launch_stream<256, 2>(p, route.mt, packed, lds, st); break;
+            case 64: launch_stream<64, 5>(p, route.mt, packed, st); break;
+            case 96: launch_stream<96, 4>(p, route.mt, packed, st); break;
+            case 128: launch_stream<128, 4>(p, route.mt, packed, st); break;
+            default: launch_stream<256, 2>(p, route.mt, packed, st); break;
         }
         if (int rc = check_launch("paged_attention_stream_kernel")) return rc;
         p.zero_rows = 0;
@@ -1124,10 +1268,10 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
         p.most_rows = 0xffffffffu;
         p.target = route.tile_target; p.slots = 2 * p.target;
         switch (c.head_dim) {
-            case 64: launch_tile<64>(p, packed, lds, st); break;
-            case 96: launch_tile<96>(p, packed, lds, st); break;
-            case 128: launch_tile<128>(p, packed, lds, st); break;
-            default: launch_tile<256>(p, packed, lds, st); break;
+            case 64: launch_tile<64>(p, packed, st); break;
+            case 96: launch_tile<96>(p, packed, st); break;
+            case 128: launch_tile<128>(p, packed, st); break;
+            default: launch_tile<256>(p, packed, st); break;
         }
         if (int rc = check_launch("paged_attention_tile_kernel")) return rc;
     }
