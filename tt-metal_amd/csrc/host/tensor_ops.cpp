@@ -809,13 +809,27 @@ CacheShape cache_shape(const Tensor &keys, const Tensor &values, int device, con
     if (keys.dtype != DataType::BFLOAT16 && keys.dtype != DataType::BFLOAT8_B) raise("TT_FATAL: " + op + ": a cache must be BFLOAT16 or BFLOAT8_B, got " + name_of(keys.dtype));
     return {keys.padded[0], keys.padded[1], keys.padded[2], keys.padded[3]};
 }
-Tensor integers(const Dims &shape, int device) {
-    Tensor t;
-    t.shape = t.padded = shape;
-    t.dtype = DataType::UINT32;
-    t.layout = Layout::ROW_MAJOR;
-    t.buffer = allocate(product(shape) * 4, device);
-    return t;
+// UINT32 tensors of these shapes in one allocation: what an allocation costs is more than what a step's tables do
+std::vector<Tensor> integers(const std::vector<Dims> &shapes, int device) {
+    auto room = [](const Dims &shape) { return (size_t)(product(shape) * 4 + 255) / 256 * 256; };
+    size_t all = 0;
+    for (const Dims &shape : shapes) all += room(shape);
+    const Buffer whole = allocate(all, device);
+    std::vector<Tensor> out;
+    size_t at = 0;
+    for (const Dims &shape : shapes) {
+        Tensor t;
+        t.shape = t.padded = shape;
+        t.dtype = DataType::UINT32;
+        t.layout = Layout::ROW_MAJOR;
+        t.buffer = whole;
+        t.buffer.data = (uint8_t *)whole.data + at;
+        t.buffer.offset = at;
+        t.buffer.nbytes = (size_t)product(shape) * 4;
+        at += room(shape);
+        out.push_back(std::move(t));
+    }
+    return out;
 }
 const int32_t *ints(const Tensor &t) { return (const int32_t *)t.buffer.data; }
 int32_t *ints(Tensor &t) { return (int32_t *)t.buffer.data; }
@@ -847,7 +861,7 @@ std::vector<Tensor> paged_tables(const Tensor &cached, const Tensor &added, cons
         raise("TT_FATAL: " + op + ": page_table must be [requests, pages], got " + list_of(page_table.shape) + " for " + std::to_string(requests) + " requests");
     if (free_pages.volume() > 0x7fffffffu) raise("TT_FATAL: " + op + ": too many free pages");
     DeviceGuard guard(device);
-    std::vector<Tensor> out{integers(page_table.padded, device), integers({tokens}, device), integers({requests + 1}, device), integers({2}, device)};
+    std::vector<Tensor> out = integers({page_table.padded, {tokens}, {requests + 1}, {2}}, device);
     check(ttmi_paged_tables(ints(cached), ints(added), requests, page_size, ints(page_table), page_table.padded.back(), ints(free_pages), (uint32_t)free_pages.volume(), tokens,
                             ints(out[0]), ints(out[1]), ints(out[2]), ints(out[3]), stream_of(device)));
     return out;

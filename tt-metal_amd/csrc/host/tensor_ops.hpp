@@ -27,6 +27,7 @@ struct Buffer {
     size_t nbytes = 0;
     int device = -1;
     std::shared_ptr<void> owner;
+    size_t offset = 0;             // of data in the owner's memory, where several tensors share an allocation
 };
 
 // What the embedding provides.

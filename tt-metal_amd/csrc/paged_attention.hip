@@ -78,6 +78,23 @@ __device__ __forceinline__ uint32_t first_seen(const AttentionDev &p, uint32_t p
     return p.window && position >= p.window ? position - p.window + 1 : 0u;
 }
 
+// Token and head of rows: rho = token * group + head.  A piece's rows are counted from its first token on, where the quotient is small: a product
+// with the reciprocal is off by one at most.
+struct Rows {
+    uint32_t token0, base, group;
+    float inverse;
+    __device__ __forceinline__ Rows(uint32_t token0, uint32_t group) : token0(token0), base(token0 * group), group(group), inverse(__builtin_amdgcn_rcpf((float)group)) {}
+    __device__ __forceinline__ void at(uint32_t rho, uint32_t &token, uint32_t &head) const {
+        const uint32_t n = rho - base;
+        uint32_t q = (uint32_t)((float)n * inverse);
+        int32_t rest = (int32_t)(n - q * group);
+        if (rest < 0) { --q; rest += group; }
+        if (rest >= (int32_t)group) { ++q; rest -= group; }
+        token = token0 + q;
+        head = (uint32_t)rest;
+    }
+};
+
 template <int ROWS> struct Extent {
     uint32_t units, blocks;                // units of the request; 32-token blocks that one of them has at most
     __device__ __forceinline__ Extent(const AttentionDev &p, const Request &q) {
@@ -355,13 +372,28 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
     for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
         Piece pc;
         if (!piece_at<ROWS>(p, plan, index, pc)) continue;
+        // this wavefront's blocks: pc.begin + wave, + 4, ...; the first one is asked for before the queries
+        const uint32_t mine = pc.end > pc.begin + wave ? (pc.end - pc.begin - wave + 3) / 4 : 0;
+        Blocks<4, S::SLABS * S::TILE_BYTES> blocks;
+        StreamBlock<D, PACKED> b;
+        uint64_t at = 0;
+        bool there = false;
+        auto request = [&](uint32_t i) __attribute__((always_inline)) {
+            if (i >= mine) return;
+            if ((i & 63) == 0) blocks.load(p, pc, pc.begin + wave + i * 4);
+            at = blocks.at(i & 63);
+            there = blocks.has(i & 63);
+            b.load(p.keys, p.values, at, lane);
+        };
+        request(0);
         bf16x8 q[Q_IN_LDS ? 1 : MT][S::SLABS];
         uint32_t row_token[MT];
+        const Rows rows(pc.token0, p.group);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            const uint32_t rho = pc.row0 + min((uint32_t)(mt * 16 + x), pc.rows - 1);       // rows past the last repeat it
-            row_token[mt] = rho / p.group;
-            const uint32_t head = pc.kv * p.group + rho % p.group;
+            uint32_t head;
+            rows.at(pc.row0 + min((uint32_t)(mt * 16 + x), pc.rows - 1), row_token[mt], head);               // rows past the last repeat it
+            head += pc.kv * p.group;
 #pragma unroll
             for (int s = 0; s < S::SLABS; ++s) {
                 if (Q_IN_LDS && (mt * S::SLABS + s) % 4 != wave) continue;
@@ -499,6 +531,8 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
                 return u.v;
             };
             bf16x8 w[MT];
+            float top[MT];
+            bool move = false;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 if (!all_seen) {
@@ -510,11 +544,15 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
                         for (int i = 0; i < 4; ++i)
                             if (th * 16 + i < from || th * 16 + i > to) s[th][mt][i] = -INFINITY;
                 }
-                float top = fmaxf(fmaxf(s[0][mt][0], s[0][mt][1]), fmaxf(s[0][mt][2], s[0][mt][3]));
-                top = fmaxf(top, fmaxf(fmaxf(s[1][mt][0], s[1][mt][1]), fmaxf(s[1][mt][2], s[1][mt][3])));
-                top = max_over_quarters(top) * p.scale;
-                if (__ballot(top > m[mt] + LAZY || (m[mt] == -INFINITY && top > m[mt]))) {
-                    const float next = fmaxf(m[mt], top), shrink = __builtin_amdgcn_exp2f(m[mt] - floor_of(next));
+                top[mt] = fmaxf(fmaxf(s[0][mt][0], s[0][mt][1]), fmaxf(s[0][mt][2], s[0][mt][3]));
+                top[mt] = fmaxf(top[mt], fmaxf(fmaxf(s[1][mt][0], s[1][mt][1]), fmaxf(s[1][mt][2], s[1][mt][3])));
+                top[mt] = max_over_quarters(top[mt]) * p.scale;
+                move |= top[mt] > m[mt] + LAZY || (m[mt] == -INFINITY && top[mt] > m[mt]);
+            }
+            if (__ballot(move)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const float next = fmaxf(m[mt], top[mt]), shrink = __builtin_amdgcn_exp2f(m[mt] - floor_of(next));
                     m[mt] = next;
                     l[mt] *= shrink;
 #pragma unroll
@@ -561,20 +599,6 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
             }
         };
 
-        // ---- this wavefront's blocks: pc.begin + wave, + 4, ... ------------------------------------------------------------------
-        const uint32_t mine = pc.end > pc.begin + wave ? (pc.end - pc.begin - wave + 3) / 4 : 0;
-        Blocks<4, S::SLABS * S::TILE_BYTES> blocks;
-        StreamBlock<D, PACKED> b;
-        uint64_t at = 0;
-        bool there = false;
-        auto request = [&](uint32_t i) __attribute__((always_inline)) {
-            if (i >= mine) return;
-            if ((i & 63) == 0) blocks.load(p, pc, pc.begin + wave + i * 4);
-            at = blocks.at(i & 63);
-            there = blocks.has(i & 63);
-            b.load(p.keys, p.values, at, lane);
-        };
-        request(0);
         if (Q_IN_LDS) __syncthreads();
         for (uint32_t i = 0; i < mine; ++i) {
             if (there) work_on(b, pc.begin + wave + i * 4, at, [&]() __attribute__((always_inline)) { request(i + 1); });
@@ -584,7 +608,9 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
         // columns c of row tile mt that this lane has, divided by the sum of the weights: four of bf16, sixteen of block floats
         auto store = [&](int mt, int c, const f32x4 *v, float sum) __attribute__((always_inline)) {
             if ((uint32_t)(mt * 16 + x) >= pc.rows) return;
-            const uint32_t rho = pc.row0 + mt * 16 + x, token = rho / p.group, column = (pc.kv * p.group + rho % p.group) * D;
+            uint32_t token, column;
+            rows.at(pc.row0 + mt * 16 + x, token, column);
+            column = (pc.kv * p.group + column) * D;
             const float by = sum == 0.f ? 0.f : 1.f / sum;
             if constexpr (PACKED) {
                 const uint32_t d = c * 64 + g * 16;            // 4 i + byte
@@ -653,51 +679,62 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
             if (!fits || !last_of(p, pc, &flag)) { __syncthreads(); continue; }
             // A wavefront takes every fourth of the columns that a lane stores at once.  A load from another XCD's stores takes 1.7 us, so as many
             // parts as there are registers for are on their way together; the last part stands in for those behind it
-            constexpr int TOGETHER = PACKED ? 4 : 1, ITEMS = S::COLS / TOGETHER, MINE = (ITEMS + 3) / 4, GROUP = MINE * TOGETHER <= 2 ? 8 : 4;
+            constexpr int TOGETHER = PACKED ? 4 : 1, PER_TILE = S::COLS / TOGETHER, ITEMS = MT * PER_TILE;
+            constexpr int MINE = PACKED || ITEMS <= 4 ? 1 : 2, GROUP = PACKED ? 6 : 8;                   // items, parts at a time
             const uint8_t *const at = p.partial + (uint64_t)pc.slot * SLOT + lane * 16;
-            for (int mt = 0; mt < MT; ++mt) {
-                float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+            for (int first = wave; first < ITEMS; first += 4 * MINE) {
+                int mt[MINE], column[MINE];
+                float top[MINE], sum[MINE];
                 f32x4 out[MINE][TOGETHER];
 #pragma unroll
-                for (int n = 0; n < MINE; ++n)
+                for (int n = 0; n < MINE; ++n) {
+                    const int item = min(first + n * 4, ITEMS - 1);
+                    mt[n] = item / PER_TILE;
+                    column[n] = item % PER_TILE;
+                    top[n] = -INFINITY;
+                    sum[n] = 0.f;
 #pragma unroll
                     for (int t = 0; t < TOGETHER; ++t) out[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll 1
                 for (uint32_t part = 0; part < pc.parts; part += GROUP) {
-                    f32x4 ml[GROUP], o[GROUP][MINE][TOGETHER];
+                    float2 ml[GROUP][MINE];
+                    f32x4 o[GROUP][MINE][TOGETHER];
 #pragma unroll
                     for (int k = 0; k < GROUP; ++k) {
                         const uint8_t *const from = at + (uint64_t)min(part + k, pc.parts - 1) * SLOT;
-                        ml[k] = get_quad(from + mt * 1024);
 #pragma unroll
-                        for (int n = 0; n < MINE; ++n)
+                        for (int n = 0; n < MINE; ++n) {
+                            ml[k][n] = *reinterpret_cast<const float2 *>(from + mt[n] * 1024);
 #pragma unroll
-                            for (int t = 0; t < TOGETHER; ++t) o[k][n][t] = get_quad(from + (MT + mt * S::COLS + min(n * 4 + wave, ITEMS - 1) * TOGETHER + t) * 1024);
+                            for (int t = 0; t < TOGETHER; ++t) o[k][n][t] = get_quad(from + (MT + (mt[n] * PER_TILE + column[n]) * TOGETHER + t) * 1024);
+                        }
                     }
                     __builtin_amdgcn_sched_barrier(0);          // all of them, before the first is waited for
-                    float next = top;
 #pragma unroll
-                    for (int k = 0; k < GROUP; ++k) next = fmaxf(next, ml[k][0]);
-                    const float base = floor_of(next), shrink = __builtin_amdgcn_exp2f(top - base);
-                    top = next;
-                    sum *= shrink;
+                    for (int n = 0; n < MINE; ++n) {
+                        float next = top[n];
 #pragma unroll
-                    for (int n = 0; n < MINE; ++n)
+                        for (int k = 0; k < GROUP; ++k) next = fmaxf(next, ml[k][n].x);
+                        const float base = floor_of(next), shrink = __builtin_amdgcn_exp2f(top[n] - base);
+                        top[n] = next;
+                        sum[n] *= shrink;
 #pragma unroll
                         for (int t = 0; t < TOGETHER; ++t) out[n][t] *= shrink;
 #pragma unroll
-                    for (int k = 0; k < GROUP; ++k) {
-                        if (part + k >= pc.parts) break;
-                        const float by = __builtin_amdgcn_exp2f(ml[k][0] - base);
-                        sum += ml[k][1] * by;
-#pragma unroll
-                        for (int n = 0; n < MINE; ++n)
+                        for (int k = 0; k < GROUP; ++k) {
+                            if (part + k >= pc.parts) break;
+                            const float by = __builtin_amdgcn_exp2f(ml[k][n].x - base);
+                            sum[n] += ml[k][n].y * by;
 #pragma unroll
                             for (int t = 0; t < TOGETHER; ++t) out[n][t] += o[k][n][t] * by;
+                        }
                     }
                 }
 #pragma unroll
                 for (int n = 0; n < MINE; ++n)
-                    if (n * 4 + wave < ITEMS) store(mt, n * 4 + wave, out[n], sum);
+                    if (first + n * 4 < ITEMS) store(mt[n], column[n], out[n], sum[n]);
             }
         } else if (wave == 0) {
 #pragma unroll
@@ -756,8 +793,9 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         Piece pc;
         if (!piece_at<ROWS>(p, plan, index, pc)) continue;
         const bool idle = (uint32_t)wave * 32 >= pc.rows;       // a wavefront without rows only moves keys and values
-        const uint32_t rho = pc.row0 + min((uint32_t)(wave * 32 + c), pc.rows - 1);
-        const uint32_t row_token = rho / p.group, head = pc.kv * p.group + rho % p.group;
+        uint32_t row_token, head;
+        Rows(pc.token0, p.group).at(pc.row0 + min((uint32_t)(wave * 32 + c), pc.rows - 1), row_token, head);
+        head += pc.kv * p.group;
         bf16x8 q[SLABS];
 #pragma unroll
         for (int s = 0; s < SLABS; ++s) {
@@ -1180,7 +1218,7 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     else r.tile = tokens > 8ull * requests && (uint64_t)tokens * group > r.mt * 16;
     if (r.tile) r.mt = requests == 1 || rows >= 256 ? 0 : tiles_for(group);
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
-    if (r.mt <= 2 && c.head_dim <= 128) r.stream_target = 512;
+    if ((r.mt <= 2 && c.head_dim <= 128) || c.head_dim == 64) r.stream_target = 512;
     if (r.mt) {
         const size_t cols = packed ? (c.head_dim + 63) / 64 * 4 : c.head_dim / 16;
         r.slot_bytes = (r.mt * cols + r.mt) * 1024;

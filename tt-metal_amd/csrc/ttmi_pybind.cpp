@@ -76,6 +76,7 @@ void bind_tensor_layer(py::module_ &m) {
         .def_property_readonly("device", [](const host::Tensor &t) { return t.buffer.device; })
         .def_property_readonly("nbytes", [](const host::Tensor &t) { return t.buffer.nbytes; })
         .def_property_readonly("data_ptr", [](const host::Tensor &t) { return (uintptr_t)t.buffer.data; })
+        .def_property_readonly("offset", [](const host::Tensor &t) { return t.buffer.offset; }, "bytes between the start of `storage` and the tensor")
         .def_property_readonly("storage", &owner_of, "the object that owns the memory (a flat torch.uint8 tensor)")
         .def("volume", &host::Tensor::volume);
 

@@ -202,9 +202,11 @@ class Tensor:
     @property
     def _buf(self):
         """The buffer as a torch tensor of the storage element type (dense ROW_MAJOR data in the padded shape, else flat)."""
-        elements = self._t.storage[:self._t.nbytes].view(_TORCH[self._dtype])
-        if self._layout == Layout.ROW_MAJOR and self._dtype not in _BFP:
-            return elements.view(self._padded)
+        t = self._t
+        dtype = t.dtype
+        elements = _bytes_of(t).view(_TORCH[dtype])
+        if t.layout == Layout.ROW_MAJOR and dtype not in _BFP:
+            return elements.view(t.padded_shape)
         return elements
 
     @property
@@ -290,6 +292,14 @@ class Tensor:
         return _as_torch(_m().to_torch(self._t))
 
 
+def _bytes_of(handle) -> "torch.Tensor":
+    """The bytes of a tensor of the C++ layer, a view of the torch tensor that owns them."""
+    storage, nbytes = handle.storage, handle.nbytes
+    if storage.numel() == nbytes:
+        return storage
+    return storage.narrow(0, handle.offset, nbytes)
+
+
 def _wrap(handle) -> Tensor:
     return Tensor(None, _handle=handle)
 
@@ -297,7 +307,7 @@ def _wrap(handle) -> Tensor:
 def _as_torch(host_handle) -> "torch.Tensor":
     """A host tensor of the C++ layer as a torch tensor of its padded shape (the memory is torch's own already)."""
     dtype = _TORCH[DataType(host_handle.dtype)]
-    return host_handle.storage[:host_handle.nbytes].view(dtype).view(tuple(host_handle.padded_shape))
+    return _bytes_of(host_handle).view(dtype).view(tuple(host_handle.padded_shape))
 
 
 def _handle_or_none(t):
