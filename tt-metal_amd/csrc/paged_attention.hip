@@ -23,9 +23,9 @@
 //              few tokens have no others for the roundings to cancel against: in the block where a row ends what the rounding
 //              took off is a second product
 //   masks      a score that does not count becomes -inf, its weight 0.  bf16 values that no row of the unit sees (behind the last token,
-//              before the window) are zeroed on their way into LDS: 0 x NaN is NaN.  Where rows of a unit see different tokens,
-//              values that are not finite are taken out as well, and two products with ones in their places say which rows
-//              see them.  Block floats are always finite here: see block_scale
+//              before the window) are zeroed on their way into LDS: 0 x NaN is NaN.  Where rows of a unit see different tokens, or one
+//              ends (what a rounding took off may have either sign), values that are not finite are taken out as well, and two
+//              products with ones in their places say which rows see them.  Block floats are always finite here: see block_scale
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -484,10 +484,10 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
         auto work_on = [&](StreamBlock<D, PACKED> &b, uint32_t block, uint64_t at, auto &&next) __attribute__((always_inline)) {
             const uint32_t token0 = block * 32;
             const bool all_seen = token0 >= first_max && token0 + 31 <= pos_min;
-            bool odd = false;                                   // values that are not finite, and that some rows see and others do not
+            bool odd = false;                                   // values that are not finite, where rows see different tokens or one ends
             if constexpr (!PACKED) {
                 if (__builtin_expect(!(token0 >= first_min && token0 + 31 <= pos_max), 0)) clear_values(b.v, token0, first_min, pos_max);
-                if (__builtin_expect(!all_seen && pc.token0 != pc.token1, 0)) {
+                if (__builtin_expect(token0 + 31 >= pos_min || (!all_seen && pc.token0 != pc.token1), 0)) {
                     uint32_t any = 0;
 #pragma unroll
                     for (int n = 0; n < S::LOADS; ++n) {
@@ -819,8 +819,8 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         // steps [step_from, step_to) have something for this wavefront
         const uint32_t step_to = idle || wave_pos_max < token_of(0) ? 0 : min((wave_pos_max / 32 - pc.begin) / NB + 1, steps);
         const uint32_t step_from = wave_first_min / 32 > pc.begin ? min((wave_first_min / 32 - pc.begin) / NB, step_to) : 0;
-        // rows of the unit see different parts of the step
-        auto uneven = [&](uint32_t step) { return pc.token0 != pc.token1 && !(token_of(step) >= unit_first_max && token_of(step) + NB * 32 - 1 <= unit_pos_min); };
+        // rows of the unit see different parts of the step, or one ends in it
+        auto uneven = [&](uint32_t step) { return !(token_of(step) >= unit_first_max && token_of(step) + NB * 32 - 1 < unit_pos_min); };
 
         // ---- keys and values: memory -> registers -> LDS ------------------------------------------------------------------------------
         Blocks<1, S::ROW_BYTES> blocks;
@@ -895,7 +895,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                 if (t < first_min || t > pos_max || !(pages >> block & 1)) vreg[i] = u32x4{0, 0, 0, 0};
             }
         };
-        uint32_t odd = 0;                                       // values that are not finite, in steps that rows see differently
+        uint32_t odd = 0;                                       // values that are not finite, in uneven steps
         auto put_values = [&](uint32_t to, uint32_t step, int ahead) __attribute__((always_inline)) {
             if constexpr (!PACKED) {
                 const uint32_t token0 = token_of(step), pages = have >> (ahead * NB) & ((1u << NB) - 1);
@@ -1088,8 +1088,8 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         if (steps && WAVES == 8 && !second) end_phase();        // both halves have passed as many barriers
 
         if constexpr (!PACKED) {
-            if (__builtin_expect(pc.token0 != pc.token1 && __syncthreads_or(odd != 0), 0)) {
-                // once more over the steps that rows see differently: ones in place of the values that were taken out, counted by those who see them
+            if (__builtin_expect(__syncthreads_or(odd != 0), 0)) {
+                // once more over the uneven steps: ones in place of the values that were taken out, counted by those who see them
                 for (step = 0; step < steps; ++step) {
                     if (!uneven(step)) continue;
                     uint32_t pages = 0;
@@ -1266,8 +1266,8 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     p.pages = c.pages; p.kv_heads = c.kv_heads; p.page_blocks = c.page_size / 32;
     p.heads = x.heads; p.group = x.heads / c.kv_heads; p.window = x.window;
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
-    // a scale of zero stands for one that no score survives: -inf, what is masked, has to stay -inf
-    p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 1e-30f);
+    // a scale of zero stands for the smallest one: -inf, what is masked, has to stay -inf
+    p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 0x1p-126f);
     p.flip = x.scale < 0.f ? 0x80008000u : 0u;
 
     const Route route = route_of(p.tokens, p.requests, p.heads, c);
