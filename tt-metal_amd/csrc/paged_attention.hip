@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
     constexpr int ROWS = MT * 16, NACC = MT * S::COLS;          // NACC quads of accumulators
     constexpr int JOIN = 2 * (NACC * 16 + MT * 8) * 64;         // bytes: two wavefronts' state
     constexpr int LDS = 4 * S::STAGE > JOIN ? 4 * S::STAGE : JOIN;
-    constexpr bool Q_IN_LDS = MT > 2;                           // registers for more than two row tiles' queries are dearer than reading them again
+    constexpr bool Q_IN_LDS = MT > 2 || (MT == 2 && D > 64);
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
     __shared__ u32x4 queries[Q_IN_LDS ? MT * S::SLABS * 64 : 1];
     __shared__ uint32_t flag;
@@ -467,6 +467,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
                     product(weights_operand8<1>(words, mags, scale), grp * 4 + 1);
                     product(weights_operand8<2>(words, mags, scale), grp * 4 + 2);
                     product(weights_operand8<3>(words, mags, scale), grp * 4 + 3);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
                 bf16x8 ring[AHEAD];
@@ -512,6 +513,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) s[th][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, query(mt, sl), s[th][mt], 0, 0, 0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (!odd) next();
             // weights of a row tile rounded to bf16, or what the rounding took off; their sum goes to l
@@ -578,7 +580,8 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             const uint32_t pos = pc.q.cached + row_token[mt], first = first_seen(p, pos);
-                            const int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
+                            int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
+                            asm volatile("" : "+v"(from), "+v"(to));            // compared here, not held in registers from before the loop
                             union { uint32_t words[4]; bf16x8 v; } seen;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
@@ -591,6 +594,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
                                     if (count[i] > 0.f) acc[mt][c][i] += down ? -INFINITY : INFINITY;
+                                __builtin_amdgcn_sched_barrier(0);
                             }
                         }
                     }
@@ -1110,7 +1114,8 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                         put(3 * S::HALF, vreg, vexp, true);
                         __syncthreads();
                         if (step < step_from || step >= step_to) continue;
-                        const int from = (int)(first - token_of(step)) - kh * 4, to = (int)(pos - token_of(step)) - kh * 4;
+                        int from = (int)(first - token_of(step)) - kh * 4, to = (int)(pos - token_of(step)) - kh * 4;
+                        asm volatile("" : "+v"(from), "+v"(to));                // compared here, not held in registers from before the loop
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -1130,6 +1135,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
 #pragma unroll
                                     for (int i = 0; i < 16; ++i)
                                         if (count[i] > 0.f) acc[d][i] += down ? -INFINITY : INFINITY;
+                                    __builtin_amdgcn_sched_barrier(0);
                                 }
                             }
                     }
@@ -1209,8 +1215,8 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     Route r;
     const uint32_t group = heads / c.kv_heads;
     const uint64_t rows = (uint64_t)((tokens + requests - 1) / std::max(requests, 1u)) * group;       // of an average request
-    const uint32_t most = c.head_dim == 64 ? 5 : c.head_dim == 256 ? 2 : 4;
-    auto tiles_for = [&](uint64_t n) { return n <= 16 ? 1u : n <= 32 ? 2u : most; };
+    const uint32_t most = c.head_dim == 64 ? 5 : c.head_dim == 256 ? 1 : 4;
+    auto tiles_for = [&](uint64_t n) { return std::min(n <= 16 ? 1u : n <= 32 ? 2u : most, most); };
     // Few tokens per request: the kernel for few rows takes them all, in tiles for an average request.  Many: the other takes them all.  In
     // between the step is a mixture: single tokens go to the one, and every request that is more than its tile to the other.
     r.mt = tiles_for(rows);
@@ -1240,8 +1246,10 @@ template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, 
 }
 template <int D, int MOST> void launch_stream(const AttentionDev &p, uint32_t mt, bool packed, hipStream_t st) {
     if (mt == 1) launch_stream<D, 1>(p, packed, st);
-    else if (mt == 2) launch_stream<D, 2>(p, packed, st);
-    else launch_stream<D, MOST>(p, packed, st);
+    else if constexpr (MOST > 1) {
+        if (mt == 2) launch_stream<D, 2>(p, packed, st);
+        else launch_stream<D, MOST>(p, packed, st);
+    }
 }
 template <int D> void launch_tile(const AttentionDev &p, bool packed, hipStream_t st) {
     constexpr uint32_t threads = TileShape<D, false>::WAVES * 64;
@@ -1296,7 +1304,7 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
             case 64: launch_stream<64, 5>(p, route.mt, packed, st); break;
             case 96: launch_stream<96, 4>(p, route.mt, packed, st); break;
             case 128: launch_stream<128, 4>(p, route.mt, packed, st); break;
-            default: launch_stream<256, 2>(p, route.mt, packed, st); break;
+            default: launch_stream<256, 1>(p, route.mt, packed, st); break;
         }
         if (int rc = check_launch("paged_attention_stream_kernel")) return rc;
         p.zero_rows = 0;
