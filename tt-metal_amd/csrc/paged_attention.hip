@@ -1208,6 +1208,7 @@ namespace {
 struct Route {
     uint32_t mt = 0;                       // row tiles of the kernel for few rows; 0: not launched
     bool tile = false;
+    uint32_t few = 0;                      // most rows of a request that go to the kernel for few rows where both are launched
     uint32_t stream_target = 256, tile_target = 256;       // resident workgroups: one per CU, or two
     size_t slot_bytes = 0, slots = 0;
 };
@@ -1215,14 +1216,16 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     Route r;
     const uint32_t group = heads / c.kv_heads;
     const uint64_t rows = (uint64_t)((tokens + requests - 1) / std::max(requests, 1u)) * group;       // of an average request
-    const uint32_t most = c.head_dim == 64 ? 5 : c.head_dim == 256 ? 1 : 4;
-    auto tiles_for = [&](uint64_t n) { return std::min(n <= 16 ? 1u : n <= 32 ? 2u : most, most); };
-    // Few tokens per request: the kernel for few rows takes them all, in tiles for an average request.  Many: the other takes them all.  In
+    // Row tiles that a wavefront has registers for, and rows up to which this kernel is the faster one, in units of that many tiles
+    const uint32_t most = c.head_dim == 64 ? 5 : c.head_dim == 256 ? 1 : 2;
+    const uint32_t limit = c.head_dim == 64 ? 80 : c.head_dim == 256 ? 64 : 32;
+    auto tiles_for = [&](uint64_t n) { return std::min(n <= 16 ? 1u : n <= 32 ? 2u : 5u, most); };
+    // Few rows per request: the kernel for few rows takes them all, in tiles for an average request.  Many: the other takes them all.  In
     // between the step is a mixture: single tokens go to the one, and every request that is more than its tile to the other.
-    r.mt = tiles_for(rows);
-    if (requests == 1) r.tile = rows > most * 16;              // its length is known
-    else r.tile = tokens > 8ull * requests && (uint64_t)tokens * group > r.mt * 16;
-    if (r.tile) r.mt = requests == 1 || rows >= 256 ? 0 : tiles_for(group);
+    r.tile = rows > limit || (requests > 1 && tokens > 8ull * requests && (uint64_t)tokens * group > limit);
+    if (!r.tile) r.mt = tiles_for(rows);
+    else if (requests > 1 && rows < 256 && group <= limit) r.mt = tiles_for(group);
+    r.few = c.head_dim == 256 ? limit : r.mt * 16;
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
     if ((r.mt <= 2 && c.head_dim <= 128) || c.head_dim == 64) r.stream_target = 512;
     if (r.mt) {
@@ -1247,7 +1250,7 @@ template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, 
 template <int D, int MOST> void launch_stream(const AttentionDev &p, uint32_t mt, bool packed, hipStream_t st) {
     if (mt == 1) launch_stream<D, 1>(p, packed, st);
     else if constexpr (MOST > 1) {
-        if (mt == 2) launch_stream<D, 2>(p, packed, st);
+        if (MOST == 2 || mt == 2) launch_stream<D, 2>(p, packed, st);
         else launch_stream<D, MOST>(p, packed, st);
     }
 }
@@ -1298,19 +1301,19 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     p.zero_rows = 1;
     if (route.mt) {
         p.least_rows = 1;
-        p.most_rows = route.tile ? route.mt * 16 : 0xffffffffu;
+        p.most_rows = route.tile ? route.few : 0xffffffffu;
         p.target = route.stream_target; p.slots = 2 * p.target;
         switch (c.head_dim) {
             case 64: launch_stream<64, 5>(p, route.mt, packed, st); break;
-            case 96: launch_stream<96, 4>(p, route.mt, packed, st); break;
-            case 128: launch_stream<128, 4>(p, route.mt, packed, st); break;
+            case 96: launch_stream<96, 2>(p, route.mt, packed, st); break;
+            case 128: launch_stream<128, 2>(p, route.mt, packed, st); break;
             default: launch_stream<256, 1>(p, route.mt, packed, st); break;
         }
         if (int rc = check_launch("paged_attention_stream_kernel")) return rc;
         p.zero_rows = 0;
     }
     if (route.tile) {
-        p.least_rows = route.mt ? route.mt * 16 + 1 : 1;
+        p.least_rows = route.mt ? route.few + 1 : 1;
         p.most_rows = 0xffffffffu;
         p.target = route.tile_target; p.slots = 2 * p.target;
         switch (c.head_dim) {
