@@ -51,7 +51,7 @@ struct AttentionDev {
     uint32_t tokens, out_rows, width, query_column, requests, max_pages;
     uint32_t pages, kv_heads, page_blocks, heads, group, window;
     uint32_t least_rows, most_rows;        // requests of that many rows per key head are this launch's
-    uint32_t target, slots;                // workgroups that are resident at once; partial results that fit
+    uint32_t target, slots;                // about how many pieces the step is cut into; partial results that fit
     uint32_t *counters;                    // pieces of a unit that are done, by the unit's first slot; all zero between launches
     uint8_t *partial;
     float scale;                           // |scale| log2(e)
@@ -63,7 +63,7 @@ constexpr uint32_t COUNTERS = 4096;        // at most 2 `target` slots, each cou
 constexpr float LAZY = 8.f;                // how far (log2) a score may pass the running maximum
 
 // Operands go from LDS through a ring of this many, so that a product finds its own in registers: a read takes about as long as four products.
-constexpr int AHEAD = 4;
+constexpr int AHEAD = 2;
 // Reads of LDS and products stay in the order in which they are written; everything else may pass.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x476); }
 
@@ -1205,11 +1205,12 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
 namespace {
 // Which kernels a step needs: the lengths are on the device, the host knows how many tokens there are for how many requests.
+constexpr uint32_t TILE_TARGET = 256;      // of the kernel for many rows: one workgroup per CU
 struct Route {
     uint32_t mt = 0;                       // row tiles of the kernel for few rows; 0: not launched
     bool tile = false;
     uint32_t few = 0;                      // most rows of a request that go to the kernel for few rows where both are launched
-    uint32_t stream_target = 256, tile_target = 256;       // resident workgroups: one per CU, or two
+    uint32_t target = 256, grid = 256;     // of the kernel for few rows: pieces to aim at, workgroups that are resident at once
     size_t slot_bytes = 0, slots = 0;
 };
 Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCache &c) {
@@ -1222,18 +1223,19 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     auto tiles_for = [&](uint64_t n) { return std::min(n <= 16 ? 1u : n <= 32 ? 2u : 5u, most); };
     // Few rows per request: the kernel for few rows takes them all, in tiles for an average request.  Many: the other takes them all.  In
     // between the step is a mixture: single tokens go to the one, and every request that is more than its tile to the other.
-    r.tile = rows > limit || (requests > 1 && tokens > 8ull * requests && (uint64_t)tokens * group > limit);
+    r.tile = rows > limit || (requests > 1 && tokens > 8ull * requests && (uint64_t)tokens * group > 512);
     if (!r.tile) r.mt = tiles_for(rows);
     else if (requests > 1 && rows < 256 && group <= limit) r.mt = tiles_for(group);
     r.few = c.head_dim == 256 ? limit : r.mt * 16;
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
-    if ((r.mt <= 2 && c.head_dim <= 128) || c.head_dim == 64) r.stream_target = 512;
+    if (c.head_dim <= 128) r.grid = 512;
+    if (c.head_dim <= 128 && packed) r.target = 512;
     if (r.mt) {
         const size_t cols = packed ? (c.head_dim + 63) / 64 * 4 : c.head_dim / 16;
         r.slot_bytes = (r.mt * cols + r.mt) * 1024;
-        r.slots = 2 * (size_t)r.stream_target * r.slot_bytes;
+        r.slots = 2 * (size_t)r.grid * r.slot_bytes;
     }
-    if (r.tile) r.slots = std::max(r.slots, 2 * (size_t)r.tile_target * (c.head_dim == 256 ? 4 : 8) * ((size_t)c.head_dim / 32 * 4 + 1) * 1024);
+    if (r.tile) r.slots = std::max(r.slots, 2 * (size_t)TILE_TARGET * (c.head_dim == 256 ? 4 : 8) * ((size_t)c.head_dim / 32 * 4 + 1) * 1024);
     return r;
 }
 
@@ -1243,21 +1245,21 @@ int clear_counters(void *at, hipStream_t st) {
     return check_launch("clear_counters_kernel");
 }
 
-template <int D, int MT> void launch_stream(const AttentionDev &p, bool packed, hipStream_t st) {
-    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(p.target), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(p.target), dim3(256), 0, st, p);
+template <int D, int MT> void launch_stream(const AttentionDev &p, uint32_t grid, bool packed, hipStream_t st) {
+    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(grid), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(grid), dim3(256), 0, st, p);
 }
-template <int D, int MOST> void launch_stream(const AttentionDev &p, uint32_t mt, bool packed, hipStream_t st) {
-    if (mt == 1) launch_stream<D, 1>(p, packed, st);
+template <int D, int MOST> void launch_stream(const AttentionDev &p, const Route &route, bool packed, hipStream_t st) {
+    if (route.mt == 1) launch_stream<D, 1>(p, route.grid, packed, st);
     else if constexpr (MOST > 1) {
-        if (MOST == 2 || mt == 2) launch_stream<D, 2>(p, packed, st);
-        else launch_stream<D, MOST>(p, packed, st);
+        if (MOST == 2 || route.mt == 2) launch_stream<D, 2>(p, route.grid, packed, st);
+        else launch_stream<D, MOST>(p, route.grid, packed, st);
     }
 }
 template <int D> void launch_tile(const AttentionDev &p, bool packed, hipStream_t st) {
     constexpr uint32_t threads = TileShape<D, false>::WAVES * 64;
-    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(p.target), dim3(threads), 0, st, p);
-    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(p.target), dim3(threads), 0, st, p);
+    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(TILE_TARGET), dim3(threads), 0, st, p);
+    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(TILE_TARGET), dim3(threads), 0, st, p);
 }
 }  // namespace
 
@@ -1302,12 +1304,12 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     if (route.mt) {
         p.least_rows = 1;
         p.most_rows = route.tile ? route.few : 0xffffffffu;
-        p.target = route.stream_target; p.slots = 2 * p.target;
+        p.target = route.target; p.slots = 2 * route.grid;
         switch (c.head_dim) {
-            case 64: launch_stream<64, 5>(p, route.mt, packed, st); break;
-            case 96: launch_stream<96, 2>(p, route.mt, packed, st); break;
-            case 128: launch_stream<128, 2>(p, route.mt, packed, st); break;
-            default: launch_stream<256, 1>(p, route.mt, packed, st); break;
+            case 64: launch_stream<64, 5>(p, route, packed, st); break;
+            case 96: launch_stream<96, 2>(p, route, packed, st); break;
+            case 128: launch_stream<128, 2>(p, route, packed, st); break;
+            default: launch_stream<256, 1>(p, route, packed, st); break;
         }
         if (int rc = check_launch("paged_attention_stream_kernel")) return rc;
         p.zero_rows = 0;
@@ -1315,7 +1317,7 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     if (route.tile) {
         p.least_rows = route.mt ? route.few + 1 : 1;
         p.most_rows = 0xffffffffu;
-        p.target = route.tile_target; p.slots = 2 * p.target;
+        p.target = TILE_TARGET; p.slots = 2 * p.target;
         switch (c.head_dim) {
             case 64: launch_tile<64>(p, packed, st); break;
             case 96: launch_tile<96>(p, packed, st); break;
