@@ -33,7 +33,8 @@ def attention(rows, keys, values, table, cached, starts, heads, head_dim, page_s
 
     bound: how far a kernel may be off that adds up in fp32, rounds the probabilities and the result to bf16.  With the weights w_j
     of a row, A = sum_j w_j |v_j| element by element and e the largest error of a score (head_dim + 2 roundings of its terms in
-    fp32, and the exponential's own 2^-21):  2^-9 |out| for the result's rounding, 2^-8 A for that of the probabilities and for their sum in
+    fp32, and the exponential's own 2^-21):  2^-9 |out| for the result's rounding (half of what that
+    can take: bf16 has 8 significant bits), 2^-8 A for that of the probabilities and for their sum in
     the denominator, 2 e A for the scores (numerator and denominator), and as much again as 2^-20 A for the sums."""
     kv_heads, pages = keys.shape[1], keys.shape[0]
     scale = head_dim ** -0.5 if scale is None else scale

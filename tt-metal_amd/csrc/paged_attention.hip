@@ -10,11 +10,13 @@
 //              rho % group of the group, so a decode step of 4 heads per key head is 4 rows, a chunk of 512 tokens 2048
 //   units      (request, key head, tile of ROWS rows).  A unit's tokens are cut into pieces of a common length, which is chosen from the
 //              lengths on the device so that the whole step comes to about `target` pieces: requests of any lengths, one long one among
-//              them, fill the chip evenly.  Every wavefront makes the same prefix sums over the requests and takes pieces
-//              blockIdx, blockIdx + gridDim, ...  A unit of one piece is stored at once; the others leave (maximum, sum, fp32
-//              accumulators) in memory, and whoever comes last joins them, in the order of the pieces
+//              them, fill the chip evenly.  Every wavefront makes the same prefix sums over the requests (1 us for 64 of them) and
+//              takes pieces blockIdx, blockIdx + gridDim, ...  A unit of one piece is stored at once; the others leave (maximum, sum, fp32
+//              accumulators) in memory, and whoever comes last joins them, in the order of the pieces: results do not depend on
+//              who that is.  The join costs 3 us for one row tile, 8 for five, 15 for 256 rows of 128 elements in four parts
 //   softmax    one pass: running maximum m and sum l per row in fp32, weights exp2(s - m).  m only moves when a score passes it
-//              by more than 2^8 in weight, so that the accumulators are hardly ever rescaled
+//              by more than 2^8 in weight, so that the accumulators are hardly ever rescaled (two prompts of 5000 tokens, 32 heads on 8
+//              key heads, window 4096: 527 us, 566 where m always moves)
 //   products   keys times queries and values times weights, both transposed: a lane's accumulators belong to one row, so m, l and the
 //              rescaling are the lane's own, and the weights leave the first product in the very lanes that the second one
 //              wants them in (the tokens of a k step are permuted alike on both sides).  Weights are rounded to bf16 for
@@ -62,7 +64,8 @@ struct AttentionDev {
 constexpr uint32_t COUNTERS = 4096;        // at most 2 `target` slots, each could be a unit's first
 constexpr float LAZY = 8.f;                // how far (log2) a score may pass the running maximum
 
-// Operands go from LDS through a ring of this many, so that a product finds its own in registers: a read takes about as long as four products.
+// Operands go from LDS through a ring of this many, so that a product finds its own in registers.  Four took 537 us where two take 527 (two prompts of
+// 5000 tokens with a window of 4096): they are eight registers more, which are spilled.
 constexpr int AHEAD = 2;
 // Reads of LDS and products stay in the order in which they are written; everything else may pass.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x476); }
@@ -248,7 +251,7 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
 
 // ---- partial results -------------------------------------------------------------------------------------------------------------------
 // Stored past the L2 of the XCD (sc1): a release of all that the L2 holds would cost more than the kernel.  Loaded as any other memory, behind
-// an acquire: nobody has read these lines before in the launch.
+// an acquire: nobody has read these lines before in the launch, and loads past the L2 were slower.
 __device__ __forceinline__ void put_quad(uint8_t *to, const f32x4 &v) {
     asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(to), "v"(v) : "memory");
 }
@@ -304,10 +307,15 @@ __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Few rows (decode, drafts): bound by reading the cache.  Four wavefronts share a unit of MT x 16 rows and take its 32-token blocks in
 // turn, each with softmax state of its own; they are joined at the end.  v_mfma_f32_16x16x32_bf16.
+//   32 users x 4000 tokens, 8 key heads of 128 elements, 4 query heads to each: bf16 105 us = 5.0 TB/s, the rate of a large copy; BFLOAT8_B
+//   72 us = 3.9 TB/s, its vector ALU two thirds busy with the expansion (4 instructions for a value).  17 query heads to a key head, two row
+//   tiles: 112 and 83 us.  One user, 1500 tokens: 11 us, of which launch 2.5, plan and piece 2, first loads 2, joins 4
 //   keys     go from memory into the registers of the MFMA operand (16 bytes per lane, whole tiles); block floats are expanded there
 //   values   go through 32 tokens of LDS that belong to the wavefront (no barriers) for their transposition: ds_read_b64_tr_b16 for
 //            bf16; block floats as words of four columns, of which each of four products takes one byte
-// The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.
+// The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.  Nothing may spill in that loop: a reload
+// from scratch memory waits for all loads before it, the next block's among them (two row tiles of 128 elements with 66 spilled registers:
+// 185 us instead of 83).  Hence the scheduling barriers between products of different operands.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int D, bool PACKED> struct StreamShape {
     static constexpr int SLABS = D / 32, TILE_BYTES = PACKED ? 1088 : 2048;
@@ -351,7 +359,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
     constexpr int ROWS = MT * 16, NACC = MT * S::COLS;          // NACC quads of accumulators
     constexpr int JOIN = 2 * (NACC * 16 + MT * 8) * 64;         // bytes: two wavefronts' state
     constexpr int LDS = 4 * S::STAGE > JOIN ? 4 * S::STAGE : JOIN;
-    constexpr bool Q_IN_LDS = MT > 2 || (MT == 2 && D > 64);
+    constexpr bool Q_IN_LDS = MT > 2 || (MT == 2 && D > 64);    // the registers are needed for the next block
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
     __shared__ u32x4 queries[Q_IN_LDS ? MT * S::SLABS * 64 : 1];
     __shared__ uint32_t flag;
@@ -752,13 +760,18 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Many rows (chunks, prompts): bound by the matrix cores.  Eight wavefronts (four where heads have 256 elements) of 32 rows each share a
+// Many rows (chunks, prompts): bound by the vector ALU beside the matrix cores.  Eight wavefronts (four where heads have 256 elements) of 32 rows each share a
 // unit and its keys and values, 64 tokens (32) a step, which go through LDS as bf16; block floats are expanded on the way,
 // once for all rows of the unit.  v_mfma_f32_32x32x16_bf16.
 //   phases   a step is a phase of vector work (masks, softmax, the next tokens into LDS) and one of matrix work (values of this step, then
 //            keys of the next).  The two wavefronts of a SIMD are a phase apart, kept there by a barrier after every phase: one has the
-//            matrix cores while the other has the vector ALU.  In step, both wait for the same unit: [512 new tokens
-//            behind 7680], 32 heads, 105 us against the time below
+//            matrix cores while the other has the vector ALU.  In step, both wait for the same unit: 615 us instead of 527 for two
+//            prompts of 5000 tokens (BFLOAT8_B cache, window 4096, 32 heads on 8 key heads), 106 instead of 94 for 512 tokens behind 7680
+//            (bf16).  With the wavefronts in their matrix phase not preferred (s_setprio): 560 and 97.  The additions of the
+//            weights belong into the matrix phase, although v_dot2_f32_bf16 takes 20 cycles beside products: 566 and 102 us in the other
+//   rate     those prompts: 527 us = 0.82 PFLOP/s of what the masks leave, a large product reaches 1.22; matrix cores busy 44 % of the time,
+//            vector ALU 66 %: an instruction takes it 8 cycles while the matrix cores work, and a step of 32 products (1024 cycles) has 300
+//            of them for each wavefront, 140 for expanding block floats, 32 exponentials among the rest
 //   LDS      three buffers each for keys and values.  In vector phase i the keys of step i + 2 and the values of step i + 1 are written, read by
 //            either half of the workgroup until the end of the matrix phases i + 1, which are one phase apart
 //   keys     16-byte chunk (row r, half h) of a face lies at r * 32 + (h ^ (r / 8)) * 16: what a pass of a ds_read_b128 touches lies
@@ -1217,17 +1230,26 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     Route r;
     const uint32_t group = heads / c.kv_heads;
     const uint64_t rows = (uint64_t)((tokens + requests - 1) / std::max(requests, 1u)) * group;       // of an average request
-    // Row tiles that a wavefront has registers for, and rows up to which this kernel is the faster one, in units of that many tiles
+    // Row tiles that a wavefront has registers for, and rows up to which the kernel for few rows is the faster one, in units of that many
+    // tiles.  16 users x 4000 tokens, 8 key heads, bf16: 64 elements, 64 rows 44 us (many rows: 58); 96 elements, 40 rows in four tiles 70
+    // (65); 128 elements, 32 rows 51 (74), 40 rows in four tiles 191 (74); 256 elements, 64 rows 154 (206), 80 rows 199 (218); two tiles of 256 elements, 17 rows 524 (one: 196).
     const uint32_t most = c.head_dim == 64 ? 5 : c.head_dim == 256 ? 1 : 2;
     const uint32_t limit = c.head_dim == 64 ? 80 : c.head_dim == 256 ? 64 : 32;
     auto tiles_for = [&](uint64_t n) { return std::min(n <= 16 ? 1u : n <= 32 ? 2u : 5u, most); };
     // Few rows per request: the kernel for few rows takes them all, in tiles for an average request.  Many: the other takes them all.  In
-    // between the step is a mixture: single tokens go to the one, and every request that is more than its tile to the other.
+    // between, and where more than 8 tokens per request come to more than 512 rows, the step is a mixture: single tokens go to the one, and every
+    // request that is more than its tile to the other.  31 single tokens behind 2000 and a prompt, 8 key heads, both kernels (few rows alone):
+    // 300 rows of 64 elements 45 us (33), of 128 elements 69 (49); 1000 rows of 64 elements 51 (74); 1200 rows 47 (66).  From 256 rows per request on the
+    // launch that has nothing to do costs more than single tokens among the prompts: 8 prompts of 500 tokens 54 us (56), 31 single tokens and
+    // a prompt of 4000 257 (259).
     r.tile = rows > limit || (requests > 1 && tokens > 8ull * requests && (uint64_t)tokens * group > 512);
     if (!r.tile) r.mt = tiles_for(rows);
     else if (requests > 1 && rows < 256 && group <= limit) r.mt = tiles_for(group);
     r.few = c.head_dim == 256 ? limit : r.mt * 16;
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
+    // Two workgroups fit a CU up to 128 elements.  One piece for each CU fills the memory pipes of bf16, and is less to join than two: 32 users x 2000
+    // tokens, 128 elements 44 us (two: 50), 64 elements 24 (30).  The expansion of block floats takes both: 8 users x 26000 tokens 102 us (one: 136).
+    // The second workgroup stays for steps of more units than CUs: 64 users x 500 tokens 25 us (28 without it).
     if (c.head_dim <= 128) r.grid = 512;
     if (c.head_dim <= 128 && packed) r.target = 512;
     if (r.mt) {
