@@ -59,7 +59,7 @@ TTMI_API const char *ttmi_version(void);
  * (tt_metal/impl/debug/watcher_server.cpp) or never; there is no call of this kind in it. */
 TTMI_API int ttmi_device_status(void);
 
-/* The library's own device memory.  A matmul called without a workspace takes its scratch — partial-sum slots, or the
+/* The library's own device memory.  A matmul, or paged attention, called without a workspace takes its scratch — partial-sum slots, or the
  * weights expanded to bf16 (2 bytes per weight) — from a buffer that the library allocates on first use and keeps, one per
  * purpose, device and stream (launches on different streams may overlap and never share one); a buffer that has become
  * too small is replaced by one at least twice its size and kept aside until now.  Nothing is freed while the process runs
