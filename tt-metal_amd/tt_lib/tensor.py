@@ -98,7 +98,9 @@ def _m():
                 return torch.empty(nbytes, dtype=torch.uint8)
             return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
 
-        mod.set_runtime(allocate, lambda device: torch.cuda.current_stream(device).cuda_stream, torch.cuda.is_available)
+        # the current stream's handle without an object around it, where torch has that: 0.2 us of every call instead of 2.7
+        stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        mod.set_runtime(allocate, stream, torch.cuda.is_available)
         _modules[_module_name] = mod
     return _modules[_module_name]
 
@@ -206,7 +208,8 @@ class Tensor:
         dtype = t.dtype
         elements = _bytes_of(t).view(_TORCH[dtype])
         if t.layout == Layout.ROW_MAJOR and dtype not in _BFP:
-            return elements.view(t.padded_shape)
+            shape = t.padded_shape
+            return elements if len(shape) == 1 else elements.view(shape)
         return elements
 
     @property
