@@ -307,15 +307,15 @@ __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Few rows (decode, drafts): bound by reading the cache.  Four wavefronts share a unit of MT x 16 rows and take its 32-token blocks in
 // turn, each with softmax state of its own; they are joined at the end.  v_mfma_f32_16x16x32_bf16.
-//   32 users x 4000 tokens, 8 key heads of 128 elements, 4 query heads to each: bf16 105 us = 5.0 TB/s, the rate of a large copy; BFLOAT8_B
+//   32 users x 4000 tokens, 8 key heads of 128 elements, 4 query heads to each: bf16 94 us = 5.6 TB/s (a large copy moves 4.9); BFLOAT8_B
 //   72 us = 3.9 TB/s, its vector ALU two thirds busy with the expansion (4 instructions for a value).  17 query heads to a key head, two row
-//   tiles: 112 and 83 us.  One user, 1500 tokens: 11 us, of which launch 2.5, plan and piece 2, first loads 2, joins 4
+//   tiles: 98 and 83 us.  One user, 1500 tokens: 11 us, of which launch 2.5, plan and piece 2, first loads 2, joins 4
 //   keys     go from memory into the registers of the MFMA operand (16 bytes per lane, whole tiles); block floats are expanded there
 //   values   go through 32 tokens of LDS that belong to the wavefront (no barriers) for their transposition: ds_read_b64_tr_b16 for
 //            bf16; block floats as words of four columns, of which each of four products takes one byte
 // The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.  Nothing may spill in that loop: a reload
-// from scratch memory waits for all loads before it, the next block's among them (two row tiles of 128 elements with 66 spilled registers:
-// 185 us instead of 83).  Hence the scheduling barriers between products of different operands.
+// from scratch memory waits for all loads before it, the next block's among them (two row tiles of 128 elements in BFLOAT8_B with 66 spilled
+// registers: 185 us instead of 83).  Hence the scheduling barriers between products of different operands.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int D, bool PACKED> struct StreamShape {
     static constexpr int SLABS = D / 32, TILE_BYTES = PACKED ? 1088 : 2048;
