@@ -1306,12 +1306,13 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     p.flip = x.scale < 0.f ? 0x80008000u : 0u;
 
     const Route route = route_of(p.tokens, p.requests, p.heads, c);
-    const size_t bytes = COUNTERS * 4 + route.slots;
-    uint8_t *memory = (uint8_t *)x.workspace;
+    // Without requests there are no pieces, hence no counters and no partial results: rows are cleared, and that needs no memory.
+    uint8_t *memory = p.requests ? (uint8_t *)x.workspace : nullptr;
     static std::mutex fresh_guard;         // another thread's launch on this stream stays behind the clearing of a new buffer
     if (memory) {
         if (int rc = clear_counters(memory, st)) return rc;
-    } else {
+    } else if (p.requests) {
+        const size_t bytes = COUNTERS * 4 + route.slots;
         std::lock_guard<std::mutex> lock(fresh_guard);
         if (stream_is_capturing(st) && !scratch_held(SCRATCH_PAGED, st, bytes))
             return fail(TTMI_ERR_UNSUPPORTED, "paged attention: a captured call cannot allocate its %zu bytes of scratch: make one on this stream before the capture, or bring a workspace", bytes);
@@ -1320,8 +1321,10 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
         if (fresh)
             if (int rc = clear_counters(memory, st)) return rc;
     }
-    p.counters = (uint32_t *)memory;
-    p.partial = memory + COUNTERS * 4;
+    if (memory) {
+        p.counters = (uint32_t *)memory;
+        p.partial = memory + COUNTERS * 4;
+    }
     p.zero_rows = 1;
     if (route.mt) {
         p.least_rows = 1;
