@@ -313,7 +313,9 @@ TTMI_API int ttmi_paged_write(const void *rows, int layout, uint32_t tokens, uin
  *   out        bf16 [tokens, heads * head_dim], layout as `rows` (TILE: padding rows are zeros)
  *   head_dim   64, 96, 128 or 256; heads a multiple of kv_heads
  *   workspace  NULL (a buffer of the library, see above) or ttmi_paged_attention_workspace_bytes() bytes, 256-byte aligned: fp32
- *              partial results of rows whose tokens are dealt out to several workgroups */
+ *              partial results of rows whose tokens are dealt out to several workgroups (0 bytes, and none is looked at, without tokens or
+ *              requests).  A call that is captured into a graph needs one, which is the graph's from then on: replays may run on any
+ *              stream beside any other call, and the library's buffers belong to streams (NULL: TTMI_ERR_UNSUPPORTED) */
 TTMI_API size_t ttmi_paged_attention_workspace_bytes(uint32_t tokens, uint32_t requests, uint32_t heads, int cache_dtype, uint32_t kv_heads, uint32_t head_dim);
 TTMI_API int ttmi_paged_attention(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t query_column, const void *key_cache,
                          const void *value_cache, int cache_dtype, uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim,

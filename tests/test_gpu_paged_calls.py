@@ -43,3 +43,69 @@ def test_no_requests_and_a_workspace(tokens):
     base = (neighbour.data_ptr() + 255) // 256 * 256
     capi.check(attend(rows, caches, ints([]).view(0, 2), ints([]), ints([0]), out, workspace=base, workspace_bytes=0))
     assert (neighbour == 0x5a).all() and not out.any()
+
+
+# ---- graphs -----------------------------------------------------------------------------------------------------------------------------
+def test_a_captured_call_takes_no_buffer_of_a_stream():
+    """Also where the stream has one: the graph may be replayed on another stream, while the next call of this one has the buffer."""
+    torch.manual_seed(2)
+    caches, _ = caches_of(60)
+    table, cached, starts = ints([list(range(60))]), ints([1900]), ints([0, 1])
+    rows, out = torch.randn(1, HEADS * DIM, device="cuda").bfloat16(), torch.empty(1, HEADS * DIM, dtype=torch.bfloat16, device="cuda")
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        capi.check(attend(rows, caches, table, cached, starts, out))
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        status = attend(rows, caches, table, cached, starts, out)
+        message = capi.lib().ttmi_last_error().decode()
+        empty = attend(rows, caches, table[:0], cached, starts, out)          # no requests: nothing that needs memory
+    assert status == 3 and "captured call" in message and empty == 0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "bfloat8_b"])
+def test_graphs_of_one_stream_side_by_side(dtype):
+    """A step of single tokens and a chunk, captured one after the other on one stream and replayed at once on two others, beside eager calls on
+    the stream of the capture: every replay has the bits of the eager call, also after the library has given its buffers back."""
+    import ttnn
+
+    torch.manual_seed(3)
+    device = ttnn.open_device(0)
+    heads, kv_heads, dim, page_size, pages = 8, 2, 128, 64, 64
+    E = ttnn.experimental
+    caches = [E.allocate_paged_cache(pages, kv_heads, page_size, dim, dtype=getattr(ttnn, dtype), device=device) for _ in range(2)]
+    for cache in caches:
+        x = torch.randn(pages, kv_heads, page_size, dim, device="cuda")
+        cache._buf.copy_(capi.tilize(x.bfloat16()) if dtype == "bfloat16" else capi.pack_tensor(capi.BFLOAT8_B, x))
+    put = lambda v: ttnn.from_torch(torch.tensor(v, dtype=torch.int32), device=device)
+    table = put([list(range(pages))])
+    rows = [ttnn.from_torch(torch.randn(1, 1, n, heads * dim).bfloat16(), layout=ttnn.TILE_LAYOUT, device=device) for n in (1, 200)]
+    cached, starts = [put([3000]), put([3500])], [put([0, 1]), put([0, 200])]
+    step = lambda i: E.attend_paged_cache(rows[i], *caches, table, cached[i], starts[i], num_heads=heads)
+    captured_on = torch.cuda.Stream()
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=captured_on):
+            outs.append(step(i))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for replay, lengths in enumerate([(3000, 3500), (700, 1800), (3999, 40), (2, 3333)]):
+        for c, n in zip(cached, lengths):
+            c._buf.fill_(n)
+        want = [step(i)._buf.clone() for i in range(2)]
+        for out in outs:
+            out._buf.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(captured_on):
+            beside = [step(i)._buf for i in (0, 1, 0)]
+        torch.cuda.synchronize()
+        for i, got in [(0, outs[0]._buf), (1, outs[1]._buf), (0, beside[0]), (1, beside[1]), (0, beside[2])]:
+            assert torch.equal(got, want[i]), (replay, i)
+        if replay == 1:
+            capi.release_scratch()
+    ttnn.close_device(device)

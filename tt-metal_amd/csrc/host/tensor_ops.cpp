@@ -65,6 +65,14 @@ Buffer allocate(size_t nbytes, int device) {
     return b;
 }
 
+// whether what is launched on the stream now is recorded into a graph
+bool is_captured(hipStream_t stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &status) == hipSuccess) return status != hipStreamCaptureStatusNone;
+    (void)hipGetLastError();                                    // the default stream while another one is captured
+    return true;
+}
+
 // copies between host and device memory on the runtime's stream and waits for it
 void copy(Buffer &dst, const Buffer &src, size_t nbytes) {
     if (!nbytes) return;
@@ -122,8 +130,7 @@ bool through_slots(void *host, bool to_device, uint32_t batch, uint32_t h, size_
     hipPointerAttribute_t kind{};
     if (hipPointerGetAttributes(&kind, host) != hipSuccess) (void)hipGetLastError();
     else if (kind.type == hipMemoryTypeHost) return false;      // the caller's memory is pinned itself: one copy at the link's rate
-    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &capturing) != hipSuccess || capturing != hipStreamCaptureStatusNone) return false;
+    if (is_captured(stream)) return false;
     std::unique_lock<std::mutex> taken(g_slots_guard, std::try_to_lock);
     if (!taken.owns_lock()) return false;
     if (!g_slots && hipHostMalloc((void **)&g_slots, SLOT_BYTES * SLOT_WORKERS * SLOTS_PER_WORKER, SLOT_FLAGS) != hipSuccess) {
@@ -896,9 +903,14 @@ Tensor paged_attention(const Tensor &rows, const Tensor &key_cache, const Tensor
     Tensor out = rows;
     out.shape.back() = out.padded.back() = heads * c.head_dim;
     out.buffer = allocate(storage_bytes(out.dtype, out.layout, out.padded), device);
+    void *const stream = stream_of(device);
+    // What is recorded may be replayed on any stream beside any other call, so it has memory of its own, from where the recorded tensors have theirs
+    Buffer workspace;
+    if (const size_t bytes = ttmi_paged_attention_workspace_bytes(tokens, requests, heads, (int)key_cache.dtype, c.kv_heads, c.head_dim); bytes && is_captured((hipStream_t)stream))
+        workspace = allocate(bytes, device);
     check(ttmi_paged_attention(rows.buffer.data, (int)rows.layout, tokens, width, query_column, key_cache.buffer.data, value_cache.buffer.data, (int)key_cache.dtype, c.pages, c.kv_heads,
                                c.page_size, c.head_dim, ints(page_table), requests, page_table.padded.back(), ints(cached), ints(row_starts), heads,
-                               scale ? *scale : 1.f / std::sqrt((float)c.head_dim), window, out.buffer.data, nullptr, 0, stream_of(device)));
+                               scale ? *scale : 1.f / std::sqrt((float)c.head_dim), window, out.buffer.data, workspace.data, workspace.nbytes, stream));
     return out;
 }
 

@@ -1314,8 +1314,8 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     } else if (p.requests) {
         const size_t bytes = COUNTERS * 4 + route.slots;
         std::lock_guard<std::mutex> lock(fresh_guard);
-        if (stream_is_capturing(st) && !scratch_held(SCRATCH_PAGED, st, bytes))
-            return fail(TTMI_ERR_UNSUPPORTED, "paged attention: a captured call cannot allocate its %zu bytes of scratch: make one on this stream before the capture, or bring a workspace", bytes);
+        // what is recorded may be replayed on any stream beside any other call: the buffer of the stream that is captured is not its own
+        if (stream_is_capturing(st)) return fail(TTMI_ERR_UNSUPPORTED, "paged attention: a captured call takes no scratch of the library's, bring a workspace of %zu bytes", bytes);
         bool fresh = false;
         if (int rc = scratch_get(SCRATCH_PAGED, st, bytes, (void **)&memory, &fresh)) return rc;
         if (fresh)
