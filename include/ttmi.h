@@ -307,8 +307,8 @@ TTMI_API int ttmi_paged_write(const void *rows, int layout, uint32_t tokens, uin
  * request r; its head h, columns [query_column + h * head_dim, + head_dim), attends with key head h / (heads / kv_heads) to the
  * tokens j of the request with p - window < j <= p (window 0: all j <= p):  out = sum_j softmax_j(scale q . k_j) v_j, in
  * fp32, probabilities rounded to bf16 for the product with the values, rounded once to bf16.  Tokens without a page are left
- * out, as is what lies in a page behind the last token, whatever its bits; a row with nothing to attend to, and the rows behind
- * row_starts[requests], are zeros.  Requests may have any number of new tokens each, none among them: decode steps, chunks of prompts
+ * out, as is what lies in a page behind the last token, whatever its bits; a row with nothing to attend to, and rows of no request
+ * (before row_starts[0], behind row_starts[requests]), are zeros.  Requests may have any number of new tokens each, none among them: decode steps, chunks of prompts
  * and mixtures are one call.
  *   out        bf16 [tokens, heads * head_dim], layout as `rows` (TILE: padding rows are zeros)
  *   head_dim   64, 96, 128 or 256; heads a multiple of kv_heads

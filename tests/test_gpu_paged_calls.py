@@ -6,6 +6,7 @@ rounding takes up to 2^-8, of which the bound there holds half)."""
 import pytest
 import torch
 
+import paged_model
 from ttmi import capi
 
 pytestmark = pytest.mark.gpu
@@ -109,3 +110,45 @@ def test_graphs_of_one_stream_side_by_side(dtype):
         if replay == 1:
             capi.release_scratch()
     ttnn.close_device(device)
+
+
+# ---- row starts -----------------------------------------------------------------------------------------------------------------------
+def check_rows(layout, tokens, starts, owners, cached, window=0, width=20, scale=None):
+    """One call with these row starts into memory full of ones: owners = (first row, rows) of every request as they should be taken; every other row,
+    those that fill up the last tiles among them, is zeros, and what lies behind the output stays."""
+    torch.manual_seed(4)
+    requests = len(cached)
+    caches, (keys, values) = caches_of(requests * width + 1)
+    table = torch.arange(requests * width).view(requests, width)
+    rows = torch.randn(tokens, HEADS * DIM).bfloat16()
+    wide, whole = HEADS * DIM, (tokens + 31) // 32 * 32 if layout == capi.TILE else tokens
+    padded = torch.cat([rows, torch.zeros(whole - tokens, wide).bfloat16()])
+    given = capi.tilize(padded.cuda()[None]) if layout == capi.TILE else rows.cuda()
+    out = torch.ones(whole * wide + 4096, dtype=torch.bfloat16, device="cuda")
+    capi.check(attend(given.view(-1, wide), caches, ints(table.tolist()).view(requests, width), ints(cached), ints(starts), out, layout=layout, window=window, scale=scale, tokens=tokens))
+    assert (out[whole * wide:] == 1).all()
+    got = out[:whole * wide].cpu()
+    if layout == capi.TILE:
+        got = got.view(-1, wide // 32, 2, 2, 16, 16).permute(0, 2, 4, 1, 3, 5)
+    got = got.reshape(whole, wide).double()
+    taken = torch.zeros(whole, dtype=torch.bool)
+    for r, (first, n) in enumerate(owners):
+        taken[first:first + n] = True
+        if n:
+            want, bound = paged_model.attention(rows[first:first + n], keys, values, [table[r].tolist()], [cached[r]], [0, n], HEADS, DIM, PAGE, window=window, scale=scale)
+            off = (got[first:first + n] - want).abs()
+            assert (off <= bound + 2.0 ** -9 * want.abs()).all(), f"request {r}: worst {(off / bound).max():.2f} of the bound"
+    assert not got[~taken].any()
+
+
+@pytest.mark.parametrize("layout", [capi.ROW_MAJOR, capi.TILE])
+@pytest.mark.parametrize("tokens,starts,owners,cached", [
+    (9, [3, 4, 6], [(3, 1), (4, 2)], [50, 33]),                    # a slice of a step's starts: rows before the first one
+    (33, [3, 5, 40], [(3, 2), (5, 28)], [0, 64]),                  # more rows said than there are
+    (333, [70, 71, 400], [(70, 1), (71, 262)], [100, 3]),          # the same in the kernel for many rows
+    (40, [35], [], []),                                            # no requests at all
+    (40, [-7, 2, 5], [(0, 2), (2, 3)], [9, 40]),                   # below zero is zero
+    (5, [9, 12, 40], [(5, 0), (5, 0)], [9, 40]),                   # all of it past the last row
+])
+def test_rows_of_no_request_are_zeros(layout, tokens, starts, owners, cached):
+    check_rows(layout, tokens, starts, owners, cached)

@@ -297,11 +297,15 @@ __device__ __forceinline__ u32x4 expand8(uint32_t w0, uint32_t w1, float scale) 
     return u32x4{activations_pair<0>(w0, m0, scale), activations_pair<2>(w0, m0, scale), activations_pair<0>(w1, m1, scale), activations_pair<2>(w1, m1, scale)};
 }
 
+// Zeros for the rows of no request: those before the first one's and behind the last one's, with the rows that fill up the last tiles.
 __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_dim) {
-    const uint32_t width = p.heads * head_dim, pieces = width / 8, from = min((uint32_t)max(p.starts[p.requests], 0), p.out_rows);
-    const uint64_t all = (uint64_t)(p.out_rows - from) * pieces;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (uint64_t)gridDim.x * blockDim.x)
-        *reinterpret_cast<u32x4 *>(p.out + row_bytes_at(from + (uint32_t)(i / pieces), width, (uint32_t)(i % pieces) * 8, p.tiled)) = u32x4{0, 0, 0, 0};
+    const uint32_t width = p.heads * head_dim, pieces = width / 8;
+    const uint32_t before = min((uint32_t)max(p.starts[0], 0), p.tokens), behind = max(min((uint32_t)max(p.starts[p.requests], 0), p.tokens), before);
+    const uint64_t all = (uint64_t)(before + p.out_rows - behind) * pieces;
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (uint64_t)gridDim.x * blockDim.x) {
+        const uint32_t row = (uint32_t)(i / pieces);
+        *reinterpret_cast<u32x4 *>(p.out + row_bytes_at(row < before ? row : row - before + behind, width, (uint32_t)(i % pieces) * 8, p.tiled)) = u32x4{0, 0, 0, 0};
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
