@@ -308,8 +308,9 @@ TTMI_API int ttmi_paged_write(const void *rows, int layout, uint32_t tokens, uin
  * tokens j of the request with p - window < j <= p (window 0: all j <= p):  out = sum_j softmax_j(scale q . k_j) v_j, in
  * fp32, probabilities rounded to bf16 for the product with the values, rounded once to bf16.  Tokens without a page are left
  * out, as is what lies in a page behind the last token, whatever its bits; a row with nothing to attend to, and rows of no request
- * (before row_starts[0], behind row_starts[requests]), are zeros.  Requests may have any number of new tokens each, none among them: decode steps, chunks of prompts
- * and mixtures are one call.
+ * (before row_starts[0], behind row_starts[requests]), are zeros.  Row starts ascend; one that lies below an earlier
+ * one is read as that one, so no row belongs to two requests.  Requests may have any number of new tokens each, none among them: decode
+ * steps, chunks of prompts and mixtures are one call.
  *   out        bf16 [tokens, heads * head_dim], layout as `rows` (TILE: padding rows are zeros)
  *   head_dim   64, 96, 128 or 256; heads a multiple of kv_heads
  *   workspace  NULL (a buffer of the library, see above) or ttmi_paged_attention_workspace_bytes() bytes, 256-byte aligned: fp32

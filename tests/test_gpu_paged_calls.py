@@ -152,3 +152,34 @@ def check_rows(layout, tokens, starts, owners, cached, window=0, width=20, scale
 ])
 def test_rows_of_no_request_are_zeros(layout, tokens, starts, owners, cached):
     check_rows(layout, tokens, starts, owners, cached)
+
+
+def owners_of(starts, tokens):
+    """Every request's rows where a start below an earlier one is read as that one."""
+    at, owners = min(max(starts[0], 0), tokens), []
+    for s in starts[1:]:
+        to = max(at, min(max(s, 0), tokens))
+        owners.append((at, to - at))
+        at = to
+    return owners
+
+
+@pytest.mark.parametrize("layout", [capi.ROW_MAJOR, capi.TILE])
+@pytest.mark.parametrize("tokens,starts,cached", [
+    (10, [0, 5, 3, 8], [40, 3, 70]),
+    (10, [0, 8, 4], [33, 5]),                                      # the last start lies inside the first request's rows
+    (10, [6, 2, 9], [64, 31]),
+    (260, [0, 200, 100, 1, 250], [10, 0, 7, 90]),                  # the kernel for many rows
+    (70, [0, 40, 1, 41, 0, 42], [5, 0, 9, 300, 20]),               # both kernels, or one for a mixture
+    (300, [(37 * i) % 290 for i in range(200)], [(11 * i) % 90 for i in range(199)]),         # several requests to a lane
+])
+def test_row_starts_that_do_not_ascend(layout, tokens, starts, cached):
+    """No row belongs to two requests; the rows that are some request's hold its answer, the same every time."""
+    check_rows(layout, tokens, starts, owners_of(starts, tokens), cached)
+
+
+def test_a_step_after_row_starts_that_do_not_ascend():
+    """Long contexts, cut into pieces: nothing is left of them in the counters that the next call on the stream finds."""
+    for _ in range(2):
+        check_rows(capi.ROW_MAJOR, 6, [0, 3, 1, 2, 5, 0], owners_of([0, 3, 1, 2, 5, 0], 6), [3000, 2500, 100, 3100, 900], width=100)
+        check_rows(capi.ROW_MAJOR, 5, [0, 1, 2, 3, 4, 5], [(i, 1) for i in range(5)], [3000, 2500, 100, 3100, 900], width=100)

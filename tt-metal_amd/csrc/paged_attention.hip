@@ -34,7 +34,6 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
-#include <type_traits>
 
 #include "bfp_dequant.h"
 #include "paged_cache.h"
@@ -72,10 +71,14 @@ __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x
 
 // ---- the work of a step ---------------------------------------------------------------------------------------------------------
 struct Request { uint32_t start, added, cached; };
-__device__ __forceinline__ Request request_at(const AttentionDev &p, uint32_t r) {
-    const uint32_t from = min((uint32_t)max(p.starts[r], 0), p.tokens), to = min((uint32_t)max(p.starts[r + 1], 0), p.tokens);
-    return {from, to > from ? to - from : 0u, (uint32_t)max(p.cached[r], 0)};
+__device__ __forceinline__ uint32_t start_at(const AttentionDev &p, uint32_t r) { return min((uint32_t)max(p.starts[r], 0), p.tokens); }
+// Request r from what memory says of it.  `taken`: rows up to here belong to the requests before.  Row starts ascend, and then it changes nothing; where they
+// do not, it keeps two requests from the same rows.
+__device__ __forceinline__ Request request_of(uint32_t start, uint32_t end, int32_t cached, uint32_t taken) {
+    const uint32_t from = max(start, taken), to = max(end, from);
+    return {from, to - from, (uint32_t)max(cached, 0)};
 }
+__device__ __forceinline__ Request request_at(const AttentionDev &p, uint32_t r, uint32_t taken) { return request_of(start_at(p, r), start_at(p, r + 1), p.cached[r], taken); }
 // first token that a row at `position` sees
 __device__ __forceinline__ uint32_t first_seen(const AttentionDev &p, uint32_t position) {
     return p.window && position >= p.window ? position - p.window + 1 : 0u;
@@ -111,27 +114,27 @@ template <int ROWS> struct Extent {
     }
 };
 
-// Sums over the lanes up to and including this one, by DPP: no LDS and no barriers, the same in every wavefront.
-template <typename T> __device__ __forceinline__ T running_sum(T v) {
-    auto from = [](T x, auto ctrl, auto rows) {
-        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
-    };
-    using std::integral_constant;
-    typedef integral_constant<int, 0xf> all;
-    v += from(v, integral_constant<int, 0x111>{}, all{});                              // 1, 2, 4, 8 lanes down within 16
-    v += from(v, integral_constant<int, 0x112>{}, all{});
-    v += from(v, integral_constant<int, 0x114>{}, all{});
-    v += from(v, integral_constant<int, 0x118>{}, all{});
-    v += from(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});      // lane 15 of each 16 to the next
-    v += from(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});      // lane 31 to the upper half
-    return v;
+// Sums (maxima of numbers that are not negative) over the lanes up to and including this one, by DPP: no LDS and no barriers, the same in every wavefront.
+template <int CTRL, int ROWS, typename T> __device__ __forceinline__ T lane_from(T x) {           // 0 where there is none
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
 }
+template <typename T, typename Join> __device__ __forceinline__ T running(T v, Join join) {
+    v = join(v, lane_from<0x111, 0xf>(v));                      // 1, 2, 4, 8 lanes down within 16
+    v = join(v, lane_from<0x112, 0xf>(v));
+    v = join(v, lane_from<0x114, 0xf>(v));
+    v = join(v, lane_from<0x118, 0xf>(v));
+    v = join(v, lane_from<0x142, 0xa>(v));                      // lane 15 of each 16 to the next
+    return join(v, lane_from<0x143, 0xc>(v));                   // lane 31 to the upper half
+}
+template <typename T> __device__ __forceinline__ T running_sum(T v) { return running(v, [](T a, T b) { return a + b; }); }
+__device__ __forceinline__ uint32_t running_max(uint32_t v) { return running(v, [](uint32_t a, uint32_t b) { return max(a, b); }); }
 template <typename T> __device__ __forceinline__ T last_lane(T v) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
 
 // The pieces of the step.  Every wavefront makes the plan for itself: a lane has `each` requests, one where there are at most 64.
 struct Plan {
     uint32_t each, piece, pieces;          // blocks of a piece, pieces of the step
     uint32_t first_piece, first_slot;      // of this lane's requests
+    uint32_t begin, end;                   // first row of the first request, end of the last one's rows
     Request q;                             // this lane's first request
 };
 template <int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const AttentionDev &p) {
@@ -139,10 +142,21 @@ template <int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const At
     Plan plan;
     plan.each = (p.requests + 63) / 64;
     const uint32_t r0 = min(lane * plan.each, p.requests), r1 = min(r0 + plan.each, p.requests);
-    plan.q = r0 < r1 ? request_at(p, r0) : Request{0, 0, 0};
+    uint32_t start = 0, end = 0;           // of the first one; these loads are on their way together
+    int32_t cached = 0;
+    if (r0 < r1) { start = start_at(p, r0); end = start_at(p, r0 + 1); cached = p.cached[r0]; }
+    uint32_t top = max(start, end);        // up to the end of this lane's requests
+    for (uint32_t r = r0 + 2; r <= r1; ++r) top = max(top, start_at(p, r));
+    top = running_max(top);
+    plan.end = last_lane(top);
+    const uint32_t taken = lane_from<0x138, 0xf>(top);         // by the lanes before
+    plan.q = r0 < r1 ? request_of(start, end, cached, taken) : Request{0, 0, 0};
+    plan.begin = __builtin_amdgcn_readfirstlane(plan.q.start);
     float work = 0.f, units = 0.f;
+    Request q = plan.q;
     for (uint32_t r = r0; r < r1; ++r) {
-        const Extent<ROWS> e(p, r == r0 ? plan.q : request_at(p, r));
+        if (r > r0) q = request_at(p, r, q.start + q.added);
+        const Extent<ROWS> e(p, q);
         work += (float)e.units * (float)e.blocks;
         units += (float)e.units;
     }
@@ -152,8 +166,10 @@ template <int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const At
     const float aim = fmaxf((float)p.target - 0.5f * units, 0.25f * (float)p.target);
     plan.piece = ((uint32_t)fminf(fmaxf(ceilf(work / aim), 1.f), 1e9f) + STEP - 1) / STEP * STEP;
     uint32_t pieces = 0, slots = 0;        // of this lane's requests: pieces, and those of units with more than one
+    q = plan.q;
     for (uint32_t r = r0; r < r1; ++r) {
-        const Extent<ROWS> e(p, r == r0 ? plan.q : request_at(p, r));
+        if (r > r0) q = request_at(p, r, q.start + q.added);
+        const Extent<ROWS> e(p, q);
         const uint32_t parts = (e.blocks + plan.piece - 1) / plan.piece;
         pieces += e.units * parts;
         if (parts > 1) slots += e.units * parts;
@@ -185,9 +201,9 @@ template <int ROWS> __device__ __forceinline__ bool piece_at(const AttentionDev 
         if (index < at + units * most || i + 1 >= plan.each || x.r + 1 >= p.requests) break;
         at += units * most;
         if (most > 1) x.slot += units * most;
-        x.q = request_at(p, ++x.r);
+        x.q = request_at(p, ++x.r, x.q.start + x.q.added);
     }
-    if (index - at >= units * most) return false;              // row_starts out of order
+    if (index - at >= units * most) return false;              // only if the lengths changed meanwhile
     uint32_t local = index - at;
     x.kv = local % p.kv_heads; local /= p.kv_heads;
     x.part = local % most;
@@ -298,9 +314,8 @@ __device__ __forceinline__ u32x4 expand8(uint32_t w0, uint32_t w1, float scale) 
 }
 
 // Zeros for the rows of no request: those before the first one's and behind the last one's, with the rows that fill up the last tiles.
-__device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_dim) {
+__device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_dim, uint32_t before, uint32_t behind) {
     const uint32_t width = p.heads * head_dim, pieces = width / 8;
-    const uint32_t before = min((uint32_t)max(p.starts[0], 0), p.tokens), behind = max(min((uint32_t)max(p.starts[p.requests], 0), p.tokens), before);
     const uint64_t all = (uint64_t)(before + p.out_rows - behind) * pieces;
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (uint64_t)gridDim.x * blockDim.x) {
         const uint32_t row = (uint32_t)(i / pieces);
@@ -682,7 +697,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
         join_waves();
         if (pc.parts > 1) {
             constexpr uint32_t SLOT = (NACC + MT) * 1024;
-            const bool fits = pc.slot + pc.parts <= p.slots;       // always, unless row_starts is out of order
+            const bool fits = pc.slot + pc.parts <= p.slots;       // always: the plan makes fewer than two slots to a piece that it aims at
             if (wave == 0 && fits) {
                 uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + lane * 16;
 #pragma unroll
@@ -760,7 +775,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
         }
         __syncthreads();                                        // LDS is the next piece's
     }
-    if (p.zero_rows) clear_rows(p, D);
+    if (p.zero_rows) clear_rows(p, D, plan.begin, plan.end);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -1163,7 +1178,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         l = sum_over_halves(l);
         if (pc.parts > 1) {
             constexpr uint32_t PART = (DB * 4 + 1) * 1024, SLOT = WAVES * PART;        // of a wavefront, of a workgroup
-            const bool fits = pc.slot + pc.parts <= p.slots;   // always, unless row_starts is out of order
+            const bool fits = pc.slot + pc.parts <= p.slots;   // always: the plan makes fewer than two slots to a piece that it aims at
             if (fits && !idle) {
                 uint8_t *const at = p.partial + (uint64_t)(pc.slot + pc.part) * SLOT + wave * PART + lane * 16;
                 put_quad(at, f32x4{m, l, 0.f, 0.f});
@@ -1216,7 +1231,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
             }
         __syncthreads();                                        // LDS is the next piece's
     }
-    if (p.zero_rows) clear_rows(p, D);
+    if (p.zero_rows) clear_rows(p, D, plan.begin, plan.end);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
