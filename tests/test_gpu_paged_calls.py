@@ -183,3 +183,18 @@ def test_a_step_after_row_starts_that_do_not_ascend():
     for _ in range(2):
         check_rows(capi.ROW_MAJOR, 6, [0, 3, 1, 2, 5, 0], owners_of([0, 3, 1, 2, 5, 0], 6), [3000, 2500, 100, 3100, 900], width=100)
         check_rows(capi.ROW_MAJOR, 5, [0, 1, 2, 3, 4, 5], [(i, 1) for i in range(5)], [3000, 2500, 100, 3100, 900], width=100)
+
+
+# ---- a scale of zero ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens", [1, 150])
+def test_a_scale_of_zero_weighs_all_alike(tokens):
+    """Scores of 2^120 and more times 0: the mean of the values that a row sees."""
+    torch.manual_seed(5)
+    pages, cached = 12, 200
+    keys, values = torch.randn(pages, KV_HEADS, PAGE, DIM).bfloat16() * 2.0 ** 60, torch.randn(pages, KV_HEADS, PAGE, DIM).bfloat16()
+    rows = (torch.randn(tokens, HEADS * DIM) * 2.0 ** 60).bfloat16()
+    out = torch.empty(tokens, HEADS * DIM, dtype=torch.bfloat16, device="cuda")
+    caches = (capi.tilize(keys.cuda()), capi.tilize(values.cuda()), pages, KV_HEADS)
+    capi.check(attend(rows.cuda(), caches, ints([list(range(pages))]), ints([cached]), ints([0, tokens]), out, scale=0.0))
+    want, bound = paged_model.attention(rows, keys.double(), values.double(), [list(range(pages))], [cached], [0, tokens], HEADS, DIM, PAGE, scale=0.0)
+    assert ((out.cpu().double() - want).abs() <= bound + 2.0 ** -9 * want.abs()).all()

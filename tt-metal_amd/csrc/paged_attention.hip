@@ -1320,8 +1320,8 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     p.pages = c.pages; p.kv_heads = c.kv_heads; p.page_blocks = c.page_size / 32;
     p.heads = x.heads; p.group = x.heads / c.kv_heads; p.window = x.window;
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
-    // a scale of zero stands for the smallest one: -inf, what is masked, has to stay -inf
-    p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 0x1p-126f);
+    // a scale of zero stands for the smallest number there is: -inf, what is masked, has to stay -inf, and the largest score is 2^-21
+    p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 0x1p-149f);
     p.flip = x.scale < 0.f ? 0x80008000u : 0u;
 
     const Route route = route_of(p.tokens, p.requests, p.heads, c);
