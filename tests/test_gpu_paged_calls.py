@@ -198,3 +198,25 @@ def test_a_scale_of_zero_weighs_all_alike(tokens):
     capi.check(attend(rows.cuda(), caches, ints([list(range(pages))]), ints([cached]), ints([0, tokens]), out, scale=0.0))
     want, bound = paged_model.attention(rows, keys.double(), values.double(), [list(range(pages))], [cached], [0, tokens], HEADS, DIM, PAGE, scale=0.0)
     assert ((out.cpu().double() - want).abs() <= bound + 2.0 ** -9 * want.abs()).all()
+
+
+# ---- lengths ------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("window", [0, 2 ** 31 - 40])
+@pytest.mark.parametrize("tokens", [4, 150])
+def test_positions_of_two_to_the_31_and_more(tokens, window):
+    """A request that has more tokens from before than its row of the page table holds, with new ones at 2^31: every one of them sees the tokens that have
+    a page, or, of those, what its window reaches (here: a window that ends before the first token from the 40th new one on)."""
+    torch.manual_seed(6)
+    caches, (keys, values) = caches_of(3)
+    rows = torch.randn(tokens, HEADS * DIM).bfloat16()
+    cached, out = 2 ** 31 - 3, torch.empty(tokens, HEADS * DIM, dtype=torch.bfloat16, device="cuda")
+    capi.check(attend(rows.cuda(), caches, ints([[2, 0, 1]]), ints([cached]), ints([0, tokens]), out, window=window))
+    k, v = (x[[2, 0, 1]].transpose(0, 1).reshape(KV_HEADS, 96, DIM) for x in (keys, values))
+    got = out.cpu().double().view(tokens, HEADS, DIM)
+    for t in range(tokens):
+        first = max(0, cached + t - window + 1) if window else 0
+        if first >= 96:
+            assert not got[t].any(), t
+            continue
+        want, bound = paged_model.attention(rows[t:t + 1], k[None, :, first:], v[None, :, first:], [[0]], [95 - first], [0, 1], HEADS, DIM, 96 - first)
+        assert ((got[t].flatten() - want[0]).abs() <= bound[0] + 2.0 ** -9 * want[0].abs()).all(), t

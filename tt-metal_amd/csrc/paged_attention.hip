@@ -79,6 +79,9 @@ __device__ __forceinline__ Request request_of(uint32_t start, uint32_t end, int3
     return {from, to - from, (uint32_t)max(cached, 0)};
 }
 __device__ __forceinline__ Request request_at(const AttentionDev &p, uint32_t r, uint32_t taken) { return request_of(start_at(p, r), start_at(p, r + 1), p.cached[r], taken); }
+// Positions in masks, which compare signed differences.  No page holds a token from 2^31 - 1 on: positions there, behind what the page table
+// can name, see what one at 2^31 - 1 sees of it.
+__device__ __forceinline__ uint32_t in_table(uint32_t position) { return min(position, 0x7fffffffu); }
 // first token that a row at `position` sees
 __device__ __forceinline__ uint32_t first_seen(const AttentionDev &p, uint32_t position) {
     return p.window && position >= p.window ? position - p.window + 1 : 0u;
@@ -565,7 +568,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 if (!all_seen) {
-                    const uint32_t pos = pc.q.cached + row_token[mt], first = first_seen(p, pos);
+                    const uint32_t pos = in_table(pc.q.cached + row_token[mt]), first = in_table(first_seen(p, pc.q.cached + row_token[mt]));
                     const int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
 #pragma unroll
                     for (int th = 0; th < 2; ++th)
@@ -606,7 +609,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
                         put_values(b.v);
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            const uint32_t pos = pc.q.cached + row_token[mt], first = first_seen(p, pos);
+                            const uint32_t pos = in_table(pc.q.cached + row_token[mt]), first = in_table(first_seen(p, pc.q.cached + row_token[mt]));
                             int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
                             asm volatile("" : "+v"(from), "+v"(to));            // compared here, not held in registers from before the loop
                             union { uint32_t words[4]; bf16x8 v; } seen;
@@ -844,7 +847,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-        const uint32_t pos = pc.q.cached + row_token, first = first_seen(p, pos);
+        const uint32_t pos = in_table(pc.q.cached + row_token), first = in_table(first_seen(p, pc.q.cached + row_token));
         // tokens that some row, and that every row, sees: of the unit and of this wavefront
         const uint32_t pos_max = pc.q.cached + pc.token1, first_min = first_seen(p, pc.q.cached + pc.token0);
         const uint32_t unit_pos_min = pc.q.cached + pc.token0, unit_first_max = first_seen(p, pos_max);
