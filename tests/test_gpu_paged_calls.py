@@ -220,3 +220,21 @@ def test_positions_of_two_to_the_31_and_more(tokens, window):
             continue
         want, bound = paged_model.attention(rows[t:t + 1], k[None, :, first:], v[None, :, first:], [[0]], [95 - first], [0, 1], HEADS, DIM, 96 - first)
         assert ((got[t].flatten() - want[0]).abs() <= bound[0] + 2.0 ** -9 * want[0].abs()).all(), t
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_lengths_and_page_numbers_that_are_none(tokens):
+    """Negative lengths are 0, lengths past the table's row see what it holds, numbers outside the cache are no pages: answers by the definition."""
+    torch.manual_seed(7)
+    pages, requests = 6, 3
+    caches, (keys, values) = caches_of(pages)
+    table = torch.tensor([[-2 ** 31, 5, 2 ** 31 - 1, 0], [6, -1, 7, 1 << 30], [3, 1, 4, 2]])
+    cached = [-2 ** 31, 50, 10 ** 6]
+    starts = [0, tokens - 2, tokens - 1, tokens]
+    rows, out = torch.randn(tokens, HEADS * DIM).bfloat16(), torch.ones(tokens + 8, HEADS * DIM, dtype=torch.bfloat16, device="cuda")
+    capi.check(attend(rows.cuda(), caches, table.to(torch.int32).cuda(), ints(cached), ints(starts), out))
+    assert (out[tokens:] == 1).all()
+    lengths = [0, 50, 4 * PAGE - 1]                                # the last one: its row sees all four pages
+    want, bound = paged_model.attention(rows, keys, values, table.tolist(), lengths, starts, HEADS, DIM, PAGE)
+    off = (out[:tokens].cpu().double() - want).abs()
+    assert (off <= bound + 2.0 ** -9 * want.abs()).all() and not out[tokens - 2].any() and out[tokens - 1].any()
