@@ -3,7 +3,8 @@
     python examples/paged_decoder.py                     # 8 users, prompts of up to 700 tokens, 64 tokens each, Mistral-7B's widths
 
 A step takes any number of new tokens of every user: whole prompts, chunks of them, single tokens, all in one call of each
-operator.  The weights are random block floats (there is no checkpoint here), the hidden states random numbers."""
+operator.  The weights are random block floats (there is no checkpoint here), the hidden states random numbers.  Queries and keys go into
+attention and cache as they are projected: a model with rotary positions rotates them in the qkv rows first, which is not done here."""
 from __future__ import annotations
 
 import os

@@ -277,7 +277,8 @@ TTMI_API int ttmi_eltwise_bf16(int op, const void *a, const void *b, float scala
  * table[p / page_size] * page_size + p % page_size, with the request's row of the page table.  Lengths, tables, slots and row
  * starts are int32 in device memory and never come to the host, so a step can be captured into a graph and replayed on other
  * lengths.  Whatever they hold, no call reads or writes outside the buffers whose sizes it is told: page numbers outside
- * [0, pages), -1 among them, mean that there is no page, negative lengths count as 0.  No
+ * [0, pages), -1 among them, mean that there is no page, negative lengths count as 0.  Block floats in a cache are read as finite
+ * numbers: an exponent byte of 255 (infinities or NaN were written) as 254, one below 7 (all 16 numbers under 2^-119) as 7.  No
  * counterpart on the reference's block-float path.
  *
  * ttmi_paged_tables: what a step needs, from its requests' lengths, one launch.  Request r has cached[r] tokens from before and adds
@@ -296,7 +297,8 @@ TTMI_API int ttmi_paged_tables(const int32_t *cached, const int32_t *added, uint
  *   rows      bf16 [tokens, width], layout TTMI_ROW_MAJOR or TTMI_TILE, e.g. the output of a fused qkv projection: the keys of token t
  *             are columns [key_column, key_column + kv_heads * head_dim) of row t, the values likewise; columns are multiples of 32,
  *             width is a multiple of 8 (TILE: of 32)
- *   slots     [tokens]; a token whose slot is negative or past the last page is left out.  A slot may be named once
+ *   slots     [tokens]; a token whose slot is negative or past the last page is left out.  A slot may be named once (named twice, it
+ *             holds parts of both tokens)
  * BFLOAT8_B caches get the codes that ttmi_typecast_tiles gives for the bf16 values (one exponent for 16 neighbours of a
  * token); no other token of the page changes. */
 TTMI_API int ttmi_paged_write(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t key_column, uint32_t value_column,

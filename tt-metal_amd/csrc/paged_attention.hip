@@ -23,7 +23,9 @@
 //              the second product, as the values are, and l is the sum of the rounded ones: what a row is divided by is what it
 //              was multiplied with, so a row of one token is that token's value (v_dot2_f32_bf16 adds two at a time).  Rows of
 //              few tokens have no others for the roundings to cancel against: in the block where a row ends what the rounding
-//              took off is a second product
+//              took off is a second product.  Elsewhere it is left out: results are 2.0e-3 to 2.2e-3 off 64 bits (2-norm over 2-norm, scores
+//              with a spread of 2), with it everywhere 1.7e-3, the rounding of the result alone.  It would cost 32 users x 2000 tokens in bf16 63.0 us
+//              instead of 61.8, drafts of 5 tokens 69.0 (66.6), 8 users x 16000 in BFLOAT8_B 124 (98), 512 tokens behind 7680 114 (86), prompts 691 (527)
 //   masks      a score that does not count becomes -inf, its weight 0.  bf16 values that no row of the unit sees (behind the last token,
 //              before the window) are zeroed on their way into LDS: 0 x NaN is NaN.  Where rows of a unit see different tokens, or one
 //              ends (what a rounding took off may have either sign), values that are not finite are taken out as well, and two
@@ -335,9 +337,10 @@ __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_
 //   keys     go from memory into the registers of the MFMA operand (16 bytes per lane, whole tiles); block floats are expanded there
 //   values   go through 32 tokens of LDS that belong to the wavefront (no barriers) for their transposition: ds_read_b64_tr_b16 for
 //            bf16; block floats as words of four columns, of which each of four products takes one byte
-// The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.  Nothing may spill in that loop: a reload
+// The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.  Nothing should spill in that loop: a reload
 // from scratch memory waits for all loads before it, the next block's among them (two row tiles of 128 elements in BFLOAT8_B with 66 spilled
-// registers: 185 us instead of 83).  Hence the scheduling barriers between products of different operands.
+// registers: 185 us instead of 83).  Hence the scheduling barriers between products of different operands.  One and two row tiles have no spilled
+// registers; five row tiles of 64 elements do not fit: 46 are spilled for BFLOAT8_B, 14 for bf16, and some are reloaded in every block.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int D, bool PACKED> struct StreamShape {
     static constexpr int SLABS = D / 32, TILE_BYTES = PACKED ? 1088 : 2048;
@@ -791,7 +794,8 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 //            prompts of 5000 tokens (BFLOAT8_B cache, window 4096, 32 heads on 8 key heads), 106 instead of 94 for 512 tokens behind 7680
 //            (bf16).  With the wavefronts in their matrix phase not preferred (s_setprio): 560 and 97.  The additions of the
 //            weights belong into the matrix phase, although v_dot2_f32_bf16 takes 20 cycles beside products: 566 and 102 us in the other
-//   rate     those prompts: 527 us = 0.82 PFLOP/s of what the masks leave, a large product reaches 1.22; matrix cores busy 44 % of the time,
+//   rate     those prompts: 527 us = 0.82 PFLOP/s of what the masks leave (the largest of several cards' rates: 590 us and 0.73 on another, and
+//            on any under a profiler), a large product reaches 1.22; matrix cores busy 44 % of the time,
 //            vector ALU 66 %: an instruction takes it 8 cycles while the matrix cores work, and a step of 32 products (1024 cycles) has 300
 //            of them for each wavefront, 140 for expanding block floats, 32 exponentials among the rest
 //   LDS      three buffers each for keys and values.  In vector phase i the keys of step i + 2 and the values of step i + 1 are written, read by
@@ -1264,6 +1268,9 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     // 300 rows of 64 elements 45 us (33), of 128 elements 69 (49); 1000 rows of 64 elements 51 (74); 1200 rows 47 (66).  From 256 rows per request on the
     // launch that has nothing to do costs more than single tokens among the prompts: 8 prompts of 500 tokens 54 us (56), 31 single tokens and
     // a prompt of 4000 257 (259).
+    // Both rules know averages only.  A chunk beside so many single tokens that it does not show in them goes to the kernel for few rows, which is right
+    // for short ones and not for long ones: 128 elements, bf16 (BFLOAT8_B), 64 single tokens behind 2000 and a chunk of 200 120 us (95), both kernels 144
+    // (101); 96 and 512 188 (176), both 204 (159); 127 and 895 behind 7680 411 (543), both 352 (295); 255 and 1500 494 (466), both 476 (344).
     r.tile = rows > limit || (requests > 1 && tokens > 8ull * requests && (uint64_t)tokens * group > 512);
     if (!r.tile) r.mt = tiles_for(rows);
     else if (requests > 1 && rows < 256 && group <= limit) r.mt = tiles_for(group);

@@ -120,7 +120,8 @@ int paged_tables(const int32_t *cached, const int32_t *added, uint32_t requests,
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Writes.  A lane moves a face row: 16 neighbouring elements of one token, 32 bytes of the activations, and 32 bytes of a bf16 cache
-// or 16 codes and their exponent of a BFLOAT8_B one (the host packers' arithmetic).  HBM-bound.  In TILE layout neighbouring
+// or 16 codes and their exponent of a BFLOAT8_B one (the host packers' arithmetic).  Bound by latency: two loads that wait for each other (slot, row), then
+// the stores; a copy moves twice as much in the time of the larger case below.  In TILE layout neighbouring
 // lanes take neighbouring tokens, in row-major rows neighbouring columns: 16 lanes read 512 contiguous bytes, and where tokens lie
 // next to each other in a page, as those of a prompt do, they write 512 (or 256) contiguous bytes too.  4100 tokens, 8 key heads of 128
 // elements, into BFLOAT8_B: 26 MB in 9.8 us = 2.6 TB/s with the launch; 32 tokens into bf16: 3.2 us, the launch.

@@ -49,7 +49,7 @@ def paged_tables(cached_lengths: Tensor, new_lengths: Tensor, page_table: Tensor
     and goes on with pages from free_pages, in order, request by request; entries without a page are 0xffffffff.  slots[t] is
     where token t of the step goes (num_tokens of them, 0xffffffff behind the last token and without a page), row_starts the
     first token of every request and the number of all, counts = (pages taken, pages wanted and not there).  The arguments do not
-    change.  At most 4096 requests."""
+    change.  At most 4096 requests.  The four share an allocation, which lives as long as any of them."""
     name = "ttnn.experimental.paged_tables"
     handles = _handles(name, cached_lengths=cached_lengths, new_lengths=new_lengths, page_table=page_table, free_pages=free_pages)
     return tuple(_wrap(t) for t in _m().paged_tables(*handles, _count(name, "page_size", page_size), _count(name, "num_tokens", num_tokens), name))
@@ -70,8 +70,12 @@ def attend_paged_cache(input_tensor: Tensor, key_cache: Tensor, value_cache: Ten
     further back than the last `window` tokens where one is given.  input_tensor: bfloat16 [1, 1, tokens, width] in either layout,
     num_heads queries of head_dim elements in every row from query_column on; head h looks at key head
     h // (num_heads // num_kv_heads).  scale: 1 / sqrt(head_dim) if not given.  Returns bfloat16 [1, 1, tokens, num_heads * head_dim]
-    in input_tensor's layout.  A request may have any number of new tokens; rows of no request, and rows with nothing to look at
-    (no page), are zeros."""
+    in input_tensor's layout.  A request may have any number of new tokens; rows of no request (before row_starts[0], behind the last
+    one's), and rows with nothing to look at (no page), are zeros.  Row starts ascend; one below an earlier one is read as that one.
+
+    Scores, maxima and sums are held in 32 bits; the weights of the softmax are rounded to bfloat16 for the product with the values.
+
+    While the stream is captured into a graph, the call takes memory of its own from torch's allocator, so replays may run on any stream."""
     name = "ttnn.experimental.attend_paged_cache"
     handles = _handles(name, input_tensor=input_tensor, key_cache=key_cache, value_cache=value_cache, page_table=page_table, cached_lengths=cached_lengths,
                        row_starts=row_starts)
