@@ -325,6 +325,67 @@ TTMI_API int ttmi_paged_attention(const void *rows, int layout, uint32_t tokens,
                          const int32_t *page_table, uint32_t requests, uint32_t max_pages, const int32_t *cached, const int32_t *row_starts,
                          uint32_t heads, float scale, uint32_t window, void *out, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ttmi_paged_attention with sinks: besides the last `window` tokens, the first `sinks` tokens of the request stay visible,
+ * j <= p and (j > p - window or j < sinks).  What lies between is not read, and needs no pages.  Without a window all tokens are seen, sinks among
+ * them.  The same workspace. */
+TTMI_API int ttmi_paged_attention_sinks(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t query_column, const void *key_cache,
+                         const void *value_cache, int cache_dtype, uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim,
+                         const int32_t *page_table, uint32_t requests, uint32_t max_pages, const int32_t *cached, const int32_t *row_starts,
+                         uint32_t heads, float scale, uint32_t window, uint32_t sinks, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- positions ------------------------------------------------------------------------------------------------------------
+ * Heads of the step's tokens by their positions, with their norm in the same pass.  Row row_starts[r] + i of `rows` is token
+ * p = cached[r] + i of request r (row starts as above).  For each head x, columns [column + h * head_dim, + head_dim):
+ *   y = norm * x / sqrt(mean(x^2) + epsilon)          where `norm` (head_dim values) is given, else y = x
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)  of the angle p * frequencies[i]
+ * for the pairs i < rotary_dim / 2 of its first rotary_dim elements: (y[i], y[i + rotary_dim / 2]), or neighbours (y[2 i], y[2 i + 1]) where
+ * `interleaved` is not 0.  The other elements are y.  fp32, rounded once; angles are reduced in 64 bits, positions count up to 2^32 - 1.
+ *   frequencies  rotary_dim / 2 floats, rotary_dim a multiple of 16 up to head_dim (0: nothing turns); norm: floats; both 16-byte aligned
+ *   head_dim     64, 96, 128 or 256
+ *   out          bf16 [tokens, heads * head_dim], layout as `rows`; rows of no request, padding rows among them, are zeros.  May not overlap `rows` */
+TTMI_API int ttmi_rotate_heads(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t column, uint32_t heads, uint32_t head_dim,
+                      const int32_t *cached, const int32_t *row_starts, uint32_t requests, const float *frequencies, uint32_t rotary_dim, int interleaved,
+                      const float *norm, float epsilon, float magnitude, void *out, void *stream);
+
+/* ttmi_rotate_heads for the queries, into `out`, and for the keys, which go straight into their slots, with the values beside them as
+ * ttmi_paged_write has them: one launch.  Keys of a bf16 cache are rounded once; those of a BFLOAT8_B cache go from fp32 to its codes (the
+ * codes that ttmi_pack_rowmajor_as_bfp_tiles gives for the fp32 values).  Tokens of no request, and tokens without a slot, are left out of the caches. */
+TTMI_API int ttmi_paged_rotate_write(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t query_column, uint32_t heads,
+                      uint32_t key_column, uint32_t value_column, const int32_t *slots, void *key_cache, void *value_cache, int cache_dtype,
+                      uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, const int32_t *cached, const int32_t *row_starts,
+                      uint32_t requests, const float *frequencies, uint32_t rotary_dim, int interleaved, const float *query_norm, const float *key_norm,
+                      float epsilon, float magnitude, void *out, void *stream);
+
+/* ---- pages that change hands ------------------------------------------------------------------------------------------------
+ * ttmi_paged_fork: page tables of requests that go on from others, one launch.  Row i continues request parents[i], with its length
+ * (a parent that is none, -1 among them: an empty row).  Full pages are shared: nobody writes into them any more.  The page begun, where
+ * page_size does not divide the length, stays with the first of a parent's continuations; every other one takes a page from free_pages, in the
+ * order of the continuations, into which it is to be copied.  At most 4096 requests and 4096 continuations.
+ *   page_table_out [children, max_pages], lengths_out [children]; neither may overlap the old ones.  -1 behind the length, and where free_pages ran out
+ *   sources, targets [children]: the page begun and the page taken where continuation i has a copy to make, else -1
+ *   counts         [2]: pages taken, and pages that were wanted and not there
+ *
+ * ttmi_paged_copy: page sources[i] to page targets[i], i < pairs, in each of `count` caches of one shape, e.g. the keys and values of all
+ * layers; one launch for up to 128 of them.  `caches` is host memory.  Pairs that name no page on either side are left out.  Pairs are moved at once: a
+ * target may be named once, and is no source.
+ *
+ * ttmi_paged_release: entries that no later token of their request can see become -1 (behind the length, numbers that are no pages and, with
+ * a window, pages that lie before the window of the token at `length` and hold none of the first `sinks` tokens), and the pages that no
+ * entry names any more are listed.
+ *   page_table_out as page_table (may be the same memory)
+ *   free_pages     [pages]: the pages of [0, pages) that no entry kept names, ascending, then -1
+ *   counts         [2]: pages free, pages in use
+ *   workspace      ttmi_paged_release_workspace_bytes() bytes, 256-byte aligned (0 bytes: none); nothing is kept in it between calls */
+TTMI_API int ttmi_paged_fork(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size,
+                      const int32_t *parents, uint32_t children, const int32_t *free_pages, uint32_t free_count, int32_t *page_table_out,
+                      int32_t *lengths_out, int32_t *sources, int32_t *targets, int32_t *counts, void *stream);
+TTMI_API int ttmi_paged_copy(void *const *caches, uint32_t count, int cache_dtype, uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim,
+                      const int32_t *sources, const int32_t *targets, uint32_t pairs, void *stream);
+TTMI_API size_t ttmi_paged_release_workspace_bytes(uint32_t requests, uint32_t max_pages, uint32_t pages);
+TTMI_API int ttmi_paged_release(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, uint32_t window,
+                      uint32_t sinks, uint32_t pages, int32_t *page_table_out, int32_t *free_pages, int32_t *counts, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

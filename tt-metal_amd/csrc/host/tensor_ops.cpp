@@ -887,7 +887,7 @@ void paged_write(const Tensor &rows, const Tensor &key_cache, const Tensor &valu
 }
 
 Tensor paged_attention(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &page_table, const Tensor &cached, const Tensor &row_starts,
-                       uint32_t heads, uint32_t query_column, std::optional<float> scale, uint32_t window, const std::string &op) {
+                       uint32_t heads, uint32_t query_column, std::optional<float> scale, uint32_t window, uint32_t sinks, const std::string &op) {
     const auto [tokens, width] = activation_rows(rows, op);
     const int device = rows.buffer.device;
     const CacheShape c = cache_shape(key_cache, value_cache, device, op);
@@ -908,9 +908,135 @@ Tensor paged_attention(const Tensor &rows, const Tensor &key_cache, const Tensor
     Buffer workspace;
     if (const size_t bytes = ttmi_paged_attention_workspace_bytes(tokens, requests, heads, (int)key_cache.dtype, c.kv_heads, c.head_dim); bytes && is_captured((hipStream_t)stream))
         workspace = allocate(bytes, device);
-    check(ttmi_paged_attention(rows.buffer.data, (int)rows.layout, tokens, width, query_column, key_cache.buffer.data, value_cache.buffer.data, (int)key_cache.dtype, c.pages, c.kv_heads,
+    check(ttmi_paged_attention_sinks(rows.buffer.data, (int)rows.layout, tokens, width, query_column, key_cache.buffer.data, value_cache.buffer.data, (int)key_cache.dtype, c.pages, c.kv_heads,
                                c.page_size, c.head_dim, ints(page_table), requests, page_table.padded.back(), ints(cached), ints(row_starts), heads,
-                               scale ? *scale : 1.f / std::sqrt((float)c.head_dim), window, out.buffer.data, workspace.data, workspace.nbytes, stream));
+                               scale ? *scale : 1.f / std::sqrt((float)c.head_dim), window, sinks, out.buffer.data, workspace.data, workspace.nbytes, stream));
+    return out;
+}
+
+namespace {
+// the step's lengths; how many requests they are
+uint32_t need_lengths(const Tensor &cached, const Tensor &row_starts, int device, const std::string &op) {
+    need_integers(cached, device, op, "cached_lengths");
+    need_integers(row_starts, device, op, "row_starts");
+    if (row_starts.volume() != cached.volume() + 1) raise("TT_FATAL: " + op + ": row_starts must have one element more than cached_lengths");
+    return (uint32_t)cached.volume();
+}
+const float *floats(const Tensor &t, int device, const std::string &op, const char *name) {
+    need_on_device(t, device, op, name);
+    if (t.dtype != DataType::FLOAT32 || t.layout != Layout::ROW_MAJOR) raise("TT_FATAL: " + op + ": " + name + " must be a FLOAT32 tensor in ROW_MAJOR layout, got " + name_of(t.dtype) + " " + name_of(t.layout));
+    return (const float *)t.buffer.data;
+}
+const float *norm_weights(const Tensor *t, uint32_t head_dim, int device, const std::string &op, const char *name) {
+    if (!t) return nullptr;
+    const float *values = floats(*t, device, op, name);
+    if (t->volume() != head_dim) raise("TT_FATAL: " + op + ": " + name + " must have " + std::to_string(head_dim) + " elements, got " + std::to_string(t->volume()));
+    return values;
+}
+// frequencies of pairs: twice as many elements of a head turn
+uint32_t rotary_dim_of(const Tensor &frequencies, uint32_t head_dim, const std::string &op) {
+    const uint64_t dim = 2 * (uint64_t)frequencies.volume();
+    if (dim > head_dim) raise("TT_FATAL: " + op + ": " + std::to_string(dim / 2) + " frequencies are more than heads of " + std::to_string(head_dim) + " elements have pairs");
+    return (uint32_t)dim;
+}
+// activations of another width beside `rows`
+Tensor rows_like(const Tensor &rows, uint64_t width, int device, const std::string &op) {
+    if (!width || width > rows.padded.back()) raise("TT_FATAL: " + op + ": the heads do not fit rows of " + std::to_string(rows.padded.back()));
+    Tensor out = rows;
+    out.shape.back() = out.padded.back() = (uint32_t)width;
+    out.buffer = allocate(storage_bytes(out.dtype, out.layout, out.padded), device);
+    return out;
+}
+uint32_t table_rows(const Tensor &page_table, const Tensor &lengths, const std::string &op) {
+    const uint32_t requests = (uint32_t)lengths.volume();
+    if (page_table.padded.size() < 2 || product(page_table.padded, 0, page_table.padded.size() - 1) != requests)
+        raise("TT_FATAL: " + op + ": page_table must be [requests, pages], got " + list_of(page_table.shape) + " for " + std::to_string(requests) + " requests");
+    return requests;
+}
+}  // namespace
+
+Tensor rotate_heads(const Tensor &rows, const Tensor &cached, const Tensor &row_starts, const Tensor &frequencies, uint32_t heads, uint32_t head_dim, uint32_t column, bool interleaved,
+                    const Tensor *norm, float epsilon, float magnitude, const std::string &op) {
+    const auto [tokens, width] = activation_rows(rows, op);
+    const int device = rows.buffer.device;
+    const uint32_t requests = need_lengths(cached, row_starts, device, op);
+    const float *const f = floats(frequencies, device, op, "frequencies"), *const w = norm_weights(norm, head_dim, device, op, "norm");
+    const uint32_t rotary_dim = rotary_dim_of(frequencies, head_dim, op);
+    DeviceGuard guard(device);
+    Tensor out = rows_like(rows, (uint64_t)heads * head_dim, device, op);
+    check(ttmi_rotate_heads(rows.buffer.data, (int)rows.layout, tokens, width, column, heads, head_dim, ints(cached), ints(row_starts), requests, f, rotary_dim, interleaved, w, epsilon,
+                            magnitude, out.buffer.data, stream_of(device)));
+    return out;
+}
+
+Tensor paged_rotate_write(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &slots, const Tensor &cached, const Tensor &row_starts,
+                          const Tensor &frequencies, uint32_t heads, uint32_t key_column, uint32_t value_column, uint32_t query_column, bool interleaved, const Tensor *query_norm,
+                          const Tensor *key_norm, float epsilon, float magnitude, const std::string &op) {
+    const auto [tokens, width] = activation_rows(rows, op);
+    const int device = rows.buffer.device;
+    const CacheShape c = cache_shape(key_cache, value_cache, device, op);
+    need_integers(slots, device, op, "slots");
+    if (slots.volume() != tokens) raise("TT_FATAL: " + op + ": " + std::to_string(slots.volume()) + " slots for " + std::to_string(tokens) + " tokens");
+    if (key_cache.buffer.data == value_cache.buffer.data) raise("TT_FATAL: " + op + ": key_cache and value_cache are the same memory");
+    const uint32_t requests = need_lengths(cached, row_starts, device, op);
+    const float *const f = floats(frequencies, device, op, "frequencies");
+    const float *const qw = norm_weights(query_norm, c.head_dim, device, op, "query_norm"), *const kw = norm_weights(key_norm, c.head_dim, device, op, "key_norm");
+    const uint32_t rotary_dim = rotary_dim_of(frequencies, c.head_dim, op);
+    DeviceGuard guard(device);
+    Tensor out = rows_like(rows, (uint64_t)heads * c.head_dim, device, op);
+    check(ttmi_paged_rotate_write(rows.buffer.data, (int)rows.layout, tokens, width, query_column, heads, key_column, value_column, ints(slots), key_cache.buffer.data, value_cache.buffer.data,
+                                  (int)key_cache.dtype, c.pages, c.kv_heads, c.page_size, c.head_dim, ints(cached), ints(row_starts), requests, f, rotary_dim, interleaved, qw, kw, epsilon,
+                                  magnitude, out.buffer.data, stream_of(device)));
+    return out;
+}
+
+std::vector<Tensor> paged_fork(const Tensor &page_table, const Tensor &lengths, const Tensor &parents, const Tensor &free_pages, uint32_t page_size, const std::string &op) {
+    const int device = page_table.buffer.device;
+    need_integers(page_table, device, op, "page_table");
+    need_integers(lengths, device, op, "lengths");
+    need_integers(parents, device, op, "parents");
+    need_integers(free_pages, device, op, "free_pages");
+    const uint32_t requests = table_rows(page_table, lengths, op), width = page_table.padded.back();
+    if (parents.volume() > 0x7fffffffu || free_pages.volume() > 0x7fffffffu) raise("TT_FATAL: " + op + ": too many parents or free pages");
+    const uint32_t children = (uint32_t)parents.volume();
+    DeviceGuard guard(device);
+    std::vector<Tensor> out = integers({{children, width}, {children}, {children}, {children}, {2}}, device);
+    check(ttmi_paged_fork(ints(page_table), ints(lengths), requests, width, page_size, ints(parents), children, ints(free_pages), (uint32_t)free_pages.volume(), ints(out[0]), ints(out[1]),
+                          ints(out[2]), ints(out[3]), ints(out[4]), stream_of(device)));
+    return out;
+}
+
+void paged_copy(const std::vector<const Tensor *> &caches, const Tensor &sources, const Tensor &targets, const std::string &op) {
+    if (caches.empty()) return;
+    const int device = caches[0]->buffer.device;
+    std::vector<void *> at;
+    CacheShape c{};
+    for (const Tensor *cache : caches) {
+        c = cache_shape(*caches[0], *cache, device, op);
+        for (void *other : at)
+            if (other == cache->buffer.data) raise("TT_FATAL: " + op + ": the same cache twice");
+        at.push_back(cache->buffer.data);
+    }
+    need_integers(sources, device, op, "sources");
+    need_integers(targets, device, op, "targets");
+    if (sources.volume() != targets.volume()) raise("TT_FATAL: " + op + ": " + std::to_string(sources.volume()) + " sources for " + std::to_string(targets.volume()) + " targets");
+    if (sources.volume() > 0x7fffffffu) raise("TT_FATAL: " + op + ": too many pages");
+    DeviceGuard guard(device);
+    check(ttmi_paged_copy(at.data(), (uint32_t)at.size(), (int)caches[0]->dtype, c.pages, c.kv_heads, c.page_size, c.head_dim, ints(sources), ints(targets), (uint32_t)sources.volume(), stream_of(device)));
+}
+
+std::vector<Tensor> paged_release(const Tensor &page_table, const Tensor &lengths, uint32_t page_size, uint32_t pages, uint32_t window, uint32_t sinks, const std::string &op) {
+    const int device = page_table.buffer.device;
+    need_integers(page_table, device, op, "page_table");
+    need_integers(lengths, device, op, "lengths");
+    const uint32_t requests = table_rows(page_table, lengths, op), width = page_table.padded.back();
+    DeviceGuard guard(device);
+    const size_t bytes = ttmi_paged_release_workspace_bytes(requests, width, pages);
+    // the workspace lies behind the results, in their allocation
+    std::vector<Tensor> out = integers({page_table.padded, {pages}, {2}, {(uint32_t)((bytes + 3) / 4)}}, device);
+    check(ttmi_paged_release(ints(page_table), ints(lengths), requests, width, page_size, window, sinks, pages, ints(out[0]), ints(out[1]), ints(out[2]), bytes ? ints(out[3]) : nullptr, bytes,
+                             stream_of(device)));
+    out.pop_back();
     return out;
 }
 

@@ -99,7 +99,19 @@ std::vector<Tensor> paged_tables(const Tensor &cached, const Tensor &added, cons
                                  const std::string &op);
 void paged_write(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &slots, uint32_t key_column, uint32_t value_column, const std::string &op);
 Tensor paged_attention(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &page_table, const Tensor &cached, const Tensor &row_starts,
-                       uint32_t heads, uint32_t query_column, std::optional<float> scale, uint32_t window, const std::string &op);
+                       uint32_t heads, uint32_t query_column, std::optional<float> scale, uint32_t window, uint32_t sinks, const std::string &op);
+// norms may be null; frequencies and norms are FLOAT32 tensors in ROW_MAJOR layout
+Tensor rotate_heads(const Tensor &rows, const Tensor &cached, const Tensor &row_starts, const Tensor &frequencies, uint32_t heads, uint32_t head_dim, uint32_t column, bool interleaved,
+                    const Tensor *norm, float epsilon, float magnitude, const std::string &op);
+// the queries
+Tensor paged_rotate_write(const Tensor &rows, const Tensor &key_cache, const Tensor &value_cache, const Tensor &slots, const Tensor &cached, const Tensor &row_starts,
+                          const Tensor &frequencies, uint32_t heads, uint32_t key_column, uint32_t value_column, uint32_t query_column, bool interleaved, const Tensor *query_norm,
+                          const Tensor *key_norm, float epsilon, float magnitude, const std::string &op);
+// {page table, lengths, sources, targets, counts}
+std::vector<Tensor> paged_fork(const Tensor &page_table, const Tensor &lengths, const Tensor &parents, const Tensor &free_pages, uint32_t page_size, const std::string &op);
+void paged_copy(const std::vector<const Tensor *> &caches, const Tensor &sources, const Tensor &targets, const std::string &op);
+// {page table, free pages, counts}
+std::vector<Tensor> paged_release(const Tensor &page_table, const Tensor &lengths, uint32_t page_size, uint32_t pages, uint32_t window, uint32_t sinks, const std::string &op);
 
 // ---- ttnn.from_torch / to_torch / to_layout / __getitem__ (ttnn/ttnn/operations/core.py) ------------------------------------
 // from_torch for block-float: data is host fp32 or bf16 (src_dtype), logical shape `shape`; one fused pad + tilize + pack.

@@ -3,7 +3,7 @@
 // Request r has cached_r tokens from before and n_r = row_starts[r + 1] - row_starts[r] new ones, all of them in the cache.  Row
 // row_starts[r] + i of the activations is token p = cached_r + i.  For each of its heads, with the key head that its group shares,
 //   out = sum_j softmax_j(scale q . k_j) v_j    over the tokens p - window < j <= p that have a page
-// and zeros where nothing is left.
+// and zeros where nothing is left.  With sinks (kernels of their own: SINKS) the first `sinks` tokens stay visible before the window: j <= p and j < sinks.
 //
 // Common to both kernels
 //   rows       the heads that share a key head are rows of one product: row rho of (request, key head) is token rho / group, head
@@ -52,7 +52,7 @@ struct AttentionDev {
     const int32_t *table, *cached, *starts;
     uint8_t *out;
     uint32_t tokens, out_rows, width, query_column, requests, max_pages;
-    uint32_t pages, kv_heads, page_blocks, heads, group, window;
+    uint32_t pages, kv_heads, page_blocks, heads, group, window, sinks;
     uint32_t least_rows, most_rows;        // requests of that many rows per key head are this launch's
     uint32_t target, slots;                // about how many pieces the step is cut into; partial results that fit
     uint32_t *counters;                    // pieces of a unit that are done, by the unit's first slot; all zero between launches
@@ -106,7 +106,12 @@ struct Rows {
     }
 };
 
-template <int ROWS> struct Extent {
+// Blocks of the sinks, in whole steps of the kernel.  What a unit sees is these and the ones of its window, counted as if they lay next to each other
+// wherever something lies between: a step never reaches over the gap.
+template <int SINKS> __device__ __forceinline__ uint32_t sink_blocks(const AttentionDev &p) { return ((p.sinks + 31) / 32 + SINKS - 1) / SINKS * SINKS; }
+
+// SINKS here and below: 0 without sinks, else the blocks that a step of the kernel has.
+template <int ROWS, int SINKS> struct Extent {
     uint32_t units, blocks;                // units of the request; 32-token blocks that one of them has at most
     __device__ __forceinline__ Extent(const AttentionDev &p, const Request &q) {
         const uint64_t rows = (uint64_t)q.added * p.group;
@@ -114,26 +119,11 @@ template <int ROWS> struct Extent {
         units = (uint32_t)((rows + ROWS - 1) / ROWS) * p.kv_heads;
         const uint32_t end = min((q.cached + q.added - 1) / 32 + 1, p.max_pages * p.page_blocks), begin = min(first_seen(p, q.cached) / 32, end);
         blocks = end - begin;
-        if (p.window) blocks = (uint32_t)min((uint64_t)blocks, ((uint64_t)p.window + ROWS / p.group + 2) / 32 + 2);
+        if constexpr (SINKS != 0) blocks = (uint32_t)min((uint64_t)end, ((uint64_t)p.window + ROWS / p.group + 2) / 32 + 2 + sink_blocks<SINKS>(p));
+        else if (p.window) blocks = (uint32_t)min((uint64_t)blocks, ((uint64_t)p.window + ROWS / p.group + 2) / 32 + 2);
         blocks = max(blocks, 1u);
     }
 };
-
-// Sums (maxima of numbers that are not negative) over the lanes up to and including this one, by DPP: no LDS and no barriers, the same in every wavefront.
-template <int CTRL, int ROWS, typename T> __device__ __forceinline__ T lane_from(T x) {           // 0 where there is none
-    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
-}
-template <typename T, typename Join> __device__ __forceinline__ T running(T v, Join join) {
-    v = join(v, lane_from<0x111, 0xf>(v));                      // 1, 2, 4, 8 lanes down within 16
-    v = join(v, lane_from<0x112, 0xf>(v));
-    v = join(v, lane_from<0x114, 0xf>(v));
-    v = join(v, lane_from<0x118, 0xf>(v));
-    v = join(v, lane_from<0x142, 0xa>(v));                      // lane 15 of each 16 to the next
-    return join(v, lane_from<0x143, 0xc>(v));                   // lane 31 to the upper half
-}
-template <typename T> __device__ __forceinline__ T running_sum(T v) { return running(v, [](T a, T b) { return a + b; }); }
-__device__ __forceinline__ uint32_t running_max(uint32_t v) { return running(v, [](uint32_t a, uint32_t b) { return max(a, b); }); }
-template <typename T> __device__ __forceinline__ T last_lane(T v) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
 
 // The pieces of the step.  Every wavefront makes the plan for itself: a lane has `each` requests, one where there are at most 64.
 struct Plan {
@@ -142,7 +132,7 @@ struct Plan {
     uint32_t begin, end;                   // first row of the first request, end of the last one's rows
     Request q;                             // this lane's first request
 };
-template <int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const AttentionDev &p) {
+template <int ROWS, int STEP, int SINKS> __device__ __forceinline__ Plan make_plan(const AttentionDev &p) {
     const uint32_t lane = threadIdx.x & 63;
     Plan plan;
     plan.each = (p.requests + 63) / 64;
@@ -161,7 +151,7 @@ template <int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const At
     Request q = plan.q;
     for (uint32_t r = r0; r < r1; ++r) {
         if (r > r0) q = request_at(p, r, q.start + q.added);
-        const Extent<ROWS> e(p, q);
+        const Extent<ROWS, SINKS> e(p, q);
         work += (float)e.units * (float)e.blocks;
         units += (float)e.units;
     }
@@ -174,7 +164,7 @@ template <int ROWS, int STEP> __device__ __forceinline__ Plan make_plan(const At
     q = plan.q;
     for (uint32_t r = r0; r < r1; ++r) {
         if (r > r0) q = request_at(p, r, q.start + q.added);
-        const Extent<ROWS> e(p, q);
+        const Extent<ROWS, SINKS> e(p, q);
         const uint32_t parts = (e.blocks + plan.piece - 1) / plan.piece;
         pieces += e.units * parts;
         if (parts > 1) slots += e.units * parts;
@@ -191,16 +181,18 @@ struct Piece {
     Request q;
     uint32_t r, kv, row0, rows, begin, end, parts, part, slot;
     uint32_t token0, token1;               // first and last token of the unit, counted from the request's first new one
+    uint32_t skip_from, skip;              // with sinks: blocks from skip_from on lie `skip` further back
+    __device__ __forceinline__ uint32_t block(uint32_t b) const { return b >= skip_from ? b + skip : b; }
 };
 // False where the unit has fewer pieces than others of its request, and this is none of them.
-template <int ROWS> __device__ __forceinline__ bool piece_at(const AttentionDev &p, const Plan &plan, uint32_t index, Piece &x) {
+template <int ROWS, int SINKS> __device__ __forceinline__ bool piece_at(const AttentionDev &p, const Plan &plan, uint32_t index, Piece &x) {
     const uint32_t owner = __popcll(__ballot(plan.first_piece <= index)) - 1;
     uint32_t at = __builtin_amdgcn_readlane(plan.first_piece, owner), most, units;
     x.slot = __builtin_amdgcn_readlane(plan.first_slot, owner);
     x.r = owner * plan.each;
     x.q = {(uint32_t)__builtin_amdgcn_readlane(plan.q.start, owner), (uint32_t)__builtin_amdgcn_readlane(plan.q.added, owner), (uint32_t)__builtin_amdgcn_readlane(plan.q.cached, owner)};
     for (uint32_t i = 0;; ++i) {
-        const Extent<ROWS> e(p, x.q);
+        const Extent<ROWS, SINKS> e(p, x.q);
         units = e.units;
         most = (e.blocks + plan.piece - 1) / plan.piece;
         if (index < at + units * most || i + 1 >= plan.each || x.r + 1 >= p.requests) break;
@@ -218,7 +210,17 @@ template <int ROWS> __device__ __forceinline__ bool piece_at(const AttentionDev 
     x.rows = min((uint32_t)ROWS, all_rows - x.row0);
     x.token0 = x.row0 / p.group;
     x.token1 = (x.row0 + x.rows - 1) / p.group;
-    const uint32_t end = min((x.q.cached + x.token1) / 32 + 1, p.max_pages * p.page_blocks), begin = min(first_seen(p, x.q.cached + x.token0) / 32, end);
+    uint32_t end = min((x.q.cached + x.token1) / 32 + 1, p.max_pages * p.page_blocks);
+    const uint32_t first = min(first_seen(p, x.q.cached + x.token0) / 32, end);
+    uint32_t begin = first;
+    x.skip_from = 0xffffffffu;
+    x.skip = 0;
+    if constexpr (SINKS != 0) {
+        x.skip_from = sink_blocks<SINKS>(p);
+        x.skip = first > x.skip_from ? first - x.skip_from : 0;
+        begin = 0;
+        end -= x.skip;
+    }
     x.parts = max((end - begin + plan.piece - 1) / plan.piece, 1u);
     x.begin = min(begin + x.part * plan.piece, end);
     x.end = min(x.begin + plan.piece, end);
@@ -228,12 +230,12 @@ template <int ROWS> __device__ __forceinline__ bool piece_at(const AttentionDev 
 
 // Where the blocks first, first + STRIDE, ... of a piece lie, 64 at a time: lane i has the byte at which the keys, and the values, of entry i
 // start, 0 (page 0) for what has no page or lies past the end.
-template <int STRIDE, int BLOCK_BYTES> struct Blocks {
+template <int STRIDE, int BLOCK_BYTES, int SINKS> struct Blocks {
     uint32_t low, high;
     uint64_t pages;                        // bit i: entry i has a page
     __device__ __forceinline__ void load(const AttentionDev &p, const Piece &x, uint32_t first) {
-        const uint32_t b = first + (threadIdx.x & 63) * STRIDE, column = b / p.page_blocks;
-        const int32_t page = b < x.end ? p.table[(uint64_t)x.r * p.max_pages + column] : -1;
+        const uint32_t n = first + (threadIdx.x & 63) * STRIDE, b = SINKS ? x.block(n) : n, column = b / p.page_blocks;
+        const int32_t page = n < x.end ? p.table[(uint64_t)x.r * p.max_pages + column] : -1;
         const bool there = (uint32_t)page < p.pages;
         const uint64_t at = there ? (((uint64_t)page * p.kv_heads + x.kv) * p.page_blocks + (b - column * p.page_blocks)) * BLOCK_BYTES : 0;
         low = (uint32_t)at;
@@ -378,7 +380,7 @@ template <int D, bool PACKED> struct StreamBlock {
     }
 };
 
-template <int D, int MT, bool PACKED>
+template <int D, int MT, bool PACKED, int SINKS>
 __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void paged_attention_stream_kernel(const AttentionDev p) {
     using S = StreamShape<D, PACKED>;
     constexpr int ROWS = MT * 16, NACC = MT * S::COLS;          // NACC quads of accumulators
@@ -390,7 +392,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
     __shared__ uint32_t flag;
     const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Plan plan = make_plan<ROWS, 4>(p);
+    const Plan plan = make_plan<ROWS, 4, SINKS>(p);
 
     typedef __attribute__((address_space(3))) uint8_t lds_byte;
     lds_byte *const stage = (lds_byte *)lds + wave * S::STAGE;
@@ -404,10 +406,10 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 
     for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
         Piece pc;
-        if (!piece_at<ROWS>(p, plan, index, pc)) continue;
+        if (!piece_at<ROWS, SINKS>(p, plan, index, pc)) continue;
         // this wavefront's blocks: pc.begin + wave, + 4, ...; the first one is asked for before the queries
         const uint32_t mine = pc.end > pc.begin + wave ? (pc.end - pc.begin - wave + 3) / 4 : 0;
-        Blocks<4, S::SLABS * S::TILE_BYTES> blocks;
+        Blocks<4, S::SLABS * S::TILE_BYTES, SINKS> blocks;
         StreamBlock<D, PACKED> b;
         uint64_t at = 0;
         bool there = false;
@@ -458,12 +460,12 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
                 if (n + 1 < S::LOADS || S::CHUNKS % 64 == 0 || n * 64 + lane < S::CHUNKS) *(__attribute__((address_space(3))) u32x4 *)(stage + to[n]) = v[n];
             lanes_in_order();
         };
-        // bf16 values: zeros for the tokens outside [low, high]
+        // bf16 values: zeros for the tokens outside [low, high] that are no sinks
         auto clear_values = [&](u32x4 (&v)[S::LOADS], uint32_t token0, uint32_t low, uint32_t high) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < S::LOADS; ++n) {
                 const uint32_t t = token0 + (n & 1) * 16 + (lane >> 1 & 15);               // 64 pieces are a face row of a tile
-                if (t < low || t > high) v[n] = u32x4{0, 0, 0, 0};
+                if ((t < low && (!SINKS || t >= p.sinks)) || t > high) v[n] = u32x4{0, 0, 0, 0};
             }
         };
         auto value_operand = [&](int c) __attribute__((always_inline)) {
@@ -517,10 +519,11 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
         // `next` is called once the block's registers are free
         auto work_on = [&](StreamBlock<D, PACKED> &b, uint32_t block, uint64_t at, auto &&next) __attribute__((always_inline)) {
             const uint32_t token0 = block * 32;
-            const bool all_seen = token0 >= first_max && token0 + 31 <= pos_min;
+            const bool all_sinks = SINKS && token0 + 31 < p.sinks;
+            const bool all_seen = (token0 >= first_max || all_sinks) && token0 + 31 <= pos_min;
             bool odd = false;                                   // values that are not finite, where rows see different tokens or one ends
             if constexpr (!PACKED) {
-                if (__builtin_expect(!(token0 >= first_min && token0 + 31 <= pos_max), 0)) clear_values(b.v, token0, first_min, pos_max);
+                if (__builtin_expect(!((token0 >= first_min || all_sinks) && token0 + 31 <= pos_max), 0)) clear_values(b.v, token0, first_min, pos_max);
                 if (__builtin_expect(token0 + 31 >= pos_min || (!all_seen && pc.token0 != pc.token1), 0)) {
                     uint32_t any = 0;
 #pragma unroll
@@ -572,12 +575,12 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
             for (int mt = 0; mt < MT; ++mt) {
                 if (!all_seen) {
                     const uint32_t pos = in_table(pc.q.cached + row_token[mt]), first = in_table(first_seen(p, pc.q.cached + row_token[mt]));
-                    const int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
+                    const int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4, sinks = (int)(in_table(p.sinks) - token0) - g * 4;
 #pragma unroll
                     for (int th = 0; th < 2; ++th)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (th * 16 + i < from || th * 16 + i > to) s[th][mt][i] = -INFINITY;
+                            if ((th * 16 + i < from && (!SINKS || th * 16 + i >= sinks)) || th * 16 + i > to) s[th][mt][i] = -INFINITY;
                 }
                 top[mt] = fmaxf(fmaxf(s[0][mt][0], s[0][mt][1]), fmaxf(s[0][mt][2], s[0][mt][3]));
                 top[mt] = fmaxf(top[mt], fmaxf(fmaxf(s[1][mt][0], s[1][mt][1]), fmaxf(s[1][mt][2], s[1][mt][3])));
@@ -615,11 +618,13 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
                             const uint32_t pos = in_table(pc.q.cached + row_token[mt]), first = in_table(first_seen(p, pc.q.cached + row_token[mt]));
                             int from = (int)(first - token0) - g * 4, to = (int)(pos - token0) - g * 4;
                             asm volatile("" : "+v"(from), "+v"(to));            // compared here, not held in registers from before the loop
+                            const int sinks = (int)(in_table(p.sinks) - token0) - g * 4;
+                            auto sees = [&](int t) { return (t >= from || (SINKS && t < sinks)) && t <= to; };
                             union { uint32_t words[4]; bf16x8 v; } seen;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const int t = (i >> 1) * 16 + (i & 1) * 2;
-                                seen.words[i] = (t >= from && t <= to ? 0x3f80u : 0u) | (t + 1 >= from && t + 1 <= to ? 0x3f800000u : 0u);
+                                seen.words[i] = (sees(t) ? 0x3f80u : 0u) | (sees(t + 1) ? 0x3f800000u : 0u);
                             }
 #pragma unroll
                             for (int c = 0; c < S::COLS; ++c) {
@@ -638,7 +643,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 
         if (Q_IN_LDS) __syncthreads();
         for (uint32_t i = 0; i < mine; ++i) {
-            if (there) work_on(b, pc.begin + wave + i * 4, at, [&]() __attribute__((always_inline)) { request(i + 1); });
+            if (there) work_on(b, SINKS ? pc.block(pc.begin + wave + i * 4) : pc.begin + wave + i * 4, at, [&]() __attribute__((always_inline)) { request(i + 1); });
             else request(i + 1);
         }
 
@@ -819,22 +824,22 @@ __device__ __forceinline__ void end_phase() {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-template <int D, bool PACKED>
+template <int D, bool PACKED, bool WITH_SINKS>
 __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_attention_tile_kernel(const AttentionDev p) {
     using S = TileShape<D, PACKED>;
-    constexpr int WAVES = S::WAVES, THREADS = WAVES * 64, ROWS = WAVES * 32, NB = S::NB, SLABS = D / 16, DB = D / 32;
+    constexpr int WAVES = S::WAVES, THREADS = WAVES * 64, ROWS = WAVES * 32, NB = S::NB, SLABS = D / 16, DB = D / 32, SINKS = WITH_SINKS ? NB : 0;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[6 * S::HALF];                // keys, then values, three buffers each
     __shared__ uint32_t flag;
     const int lane = threadIdx.x & 63, c = lane & 31, kh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool second = WAVES == 8 && wave >= 4;                // the half that runs a phase behind
     typedef __attribute__((address_space(3))) uint8_t lds_byte;
-    const Plan plan = make_plan<ROWS, NB>(p);
+    const Plan plan = make_plan<ROWS, NB, SINKS>(p);
     const uint32_t out_width = p.heads * D;
 
     for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
         Piece pc;
-        if (!piece_at<ROWS>(p, plan, index, pc)) continue;
+        if (!piece_at<ROWS, SINKS>(p, plan, index, pc)) continue;
         const bool idle = (uint32_t)wave * 32 >= pc.rows;       // a wavefront without rows only moves keys and values
         uint32_t row_token, head;
         Rows(pc.token0, p.group).at(pc.row0 + min((uint32_t)(wave * 32 + c), pc.rows - 1), row_token, head);
@@ -858,15 +863,17 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         const uint32_t wave_pos_min = pc.q.cached + (pc.row0 + min((uint32_t)wave * 32, pc.rows - 1)) / p.group, wave_pos_max = pc.q.cached + (pc.row0 + min((uint32_t)wave * 32 + 31, pc.rows - 1)) / p.group;
         const uint32_t wave_first_min = first_seen(p, wave_pos_min), wave_first_max = first_seen(p, wave_pos_max);
         const uint32_t steps = (pc.end - pc.begin + NB - 1) / NB;
-        auto token_of = [&](uint32_t step) { return (pc.begin + step * NB) * 32; };
+        auto token_of = [&](uint32_t step) { return (SINKS ? pc.block(pc.begin + step * NB) : pc.begin + step * NB) * 32; };
+        auto all_sinks = [&](uint32_t token0) { return SINKS && token0 + NB * 32 - 1 < p.sinks; };
         // steps [step_from, step_to) have something for this wavefront
-        const uint32_t step_to = idle || wave_pos_max < token_of(0) ? 0 : min((wave_pos_max / 32 - pc.begin) / NB + 1, steps);
-        const uint32_t step_from = wave_first_min / 32 > pc.begin ? min((wave_first_min / 32 - pc.begin) / NB, step_to) : 0;
+        const uint32_t last_block = wave_pos_max / 32 - (SINKS ? pc.skip : 0), first_block = SINKS && pc.begin < pc.skip_from ? 0 : wave_first_min / 32 - (SINKS ? pc.skip : 0);
+        const uint32_t step_to = idle || last_block < pc.begin ? 0 : min((last_block - pc.begin) / NB + 1, steps);
+        const uint32_t step_from = first_block > pc.begin ? min((first_block - pc.begin) / NB, step_to) : 0;
         // rows of the unit see different parts of the step, or one ends in it
-        auto uneven = [&](uint32_t step) { return !(token_of(step) >= unit_first_max && token_of(step) + NB * 32 - 1 < unit_pos_min); };
+        auto uneven = [&](uint32_t step) { return !((token_of(step) >= unit_first_max || all_sinks(token_of(step))) && token_of(step) + NB * 32 - 1 < unit_pos_min); };
 
         // ---- keys and values: memory -> registers -> LDS ------------------------------------------------------------------------------
-        Blocks<1, S::ROW_BYTES> blocks;
+        Blocks<1, S::ROW_BYTES, SINKS> blocks;
         uint64_t keys_at[NB], values_at[NB];                    // of the step whose keys, and whose values, are asked for next
         uint32_t have = 0;                                      // which blocks of four steps, from the current one on, have pages: bit NB * step + block
         u32x4 kreg[S::EACH], vreg[S::EACH];
@@ -935,14 +942,14 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                 uint32_t block, from, token, exponent;
                 place(i, block, from, token, exponent);
                 const uint32_t t = token0 + block * 32 + token;
-                if (t < first_min || t > pos_max || !(pages >> block & 1)) vreg[i] = u32x4{0, 0, 0, 0};
+                if ((t < first_min && (!SINKS || t >= p.sinks)) || t > pos_max || !(pages >> block & 1)) vreg[i] = u32x4{0, 0, 0, 0};
             }
         };
         uint32_t odd = 0;                                       // values that are not finite, in uneven steps
         auto put_values = [&](uint32_t to, uint32_t step, int ahead) __attribute__((always_inline)) {
             if constexpr (!PACKED) {
                 const uint32_t token0 = token_of(step), pages = have >> (ahead * NB) & ((1u << NB) - 1);
-                if (__builtin_expect(!(token0 >= first_min && token0 + NB * 32 - 1 <= pos_max && pages == (1u << NB) - 1), 0)) clear_values(token0, pages);
+                if (__builtin_expect(!((token0 >= first_min || all_sinks(token0)) && token0 + NB * 32 - 1 <= pos_max && pages == (1u << NB) - 1), 0)) clear_values(token0, pages);
                 if (__builtin_expect(uneven(step), 0)) {
 #pragma unroll
                     for (int i = 0; i < S::EACH; ++i) {
@@ -1082,15 +1089,15 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) ring[i] = value_operand(buffer[0], i);
             keep_order();
-            if (__builtin_expect(!(token0 >= wave_first_max && last <= wave_pos_min && (have & ((1u << NB) - 1)) == (1u << NB) - 1), 0)) {
+            if (__builtin_expect(!((token0 >= wave_first_max || all_sinks(token0)) && last <= wave_pos_min && (have & ((1u << NB) - 1)) == (1u << NB) - 1), 0)) {
                 // against constants: the tokens' numbers would be held in registers over all steps
-                const int from = (int)(first - token0) - kh * 4, to = (int)(pos - token0) - kh * 4;
+                const int from = (int)(first - token0) - kh * 4, to = (int)(pos - token0) - kh * 4, sinks = (int)(in_table(p.sinks) - token0) - kh * 4;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int t = b * 32 + (i >> 2) * 8 + (i & 3);
-                        if (t < from || t > to || !(have >> b & 1)) s[b][i] = -INFINITY;
+                        if ((t < from && (!SINKS || t >= sinks)) || t > to || !(have >> b & 1)) s[b][i] = -INFINITY;
                     }
             }
             float top = s[0][0];
@@ -1138,8 +1145,8 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                     uint32_t pages = 0;
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        const uint32_t block = pc.begin + step * NB + b;
-                        int32_t page = block < pc.end ? p.table[(uint64_t)pc.r * p.max_pages + block / p.page_blocks] : -1;
+                        const uint32_t n = pc.begin + step * NB + b, block = SINKS ? pc.block(n) : n;
+                        int32_t page = n < pc.end ? p.table[(uint64_t)pc.r * p.max_pages + block / p.page_blocks] : -1;
                         pages |= (uint32_t)((uint32_t)page < p.pages) << b;
                         if ((uint32_t)page >= p.pages) page = 0;
                         values_at[b] = (((uint64_t)page * p.kv_heads + pc.kv) * p.page_blocks + block % p.page_blocks) * S::ROW_BYTES;
@@ -1155,6 +1162,8 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                         if (step < step_from || step >= step_to) continue;
                         int from = (int)(first - token_of(step)) - kh * 4, to = (int)(pos - token_of(step)) - kh * 4;
                         asm volatile("" : "+v"(from), "+v"(to));                // compared here, not held in registers from before the loop
+                        const int sinks = (int)(in_table(p.sinks) - token_of(step)) - kh * 4;
+                        auto sees = [&](int t) { return (t >= from || (SINKS && t < sinks)) && t <= to; };
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -1163,7 +1172,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
                                     const int t = b * 32 + h * 16 + (i >> 1) * 8 + (i & 1) * 2;
-                                    seen.words[i] = (t >= from && t <= to ? 0x3f80u : 0u) | (t + 1 >= from && t + 1 <= to ? 0x3f800000u : 0u);
+                                    seen.words[i] = (sees(t) ? 0x3f80u : 0u) | (sees(t + 1) ? 0x3f800000u : 0u);
                                 }
 #pragma unroll
                                 for (int d = 0; d < DB; ++d) {
@@ -1297,8 +1306,9 @@ int clear_counters(void *at, hipStream_t st) {
 }
 
 template <int D, int MT> void launch_stream(const AttentionDev &p, uint32_t grid, bool packed, hipStream_t st) {
-    if (packed) hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, true>), dim3(grid), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((paged_attention_stream_kernel<D, MT, false>), dim3(grid), dim3(256), 0, st, p);
+    auto launch = [&](auto plain, auto sinks) { hipLaunchKernelGGL(p.sinks ? sinks : plain, dim3(grid), dim3(256), 0, st, p); };
+    if (packed) launch(paged_attention_stream_kernel<D, MT, true, 0>, paged_attention_stream_kernel<D, MT, true, 1>);
+    else launch(paged_attention_stream_kernel<D, MT, false, 0>, paged_attention_stream_kernel<D, MT, false, 1>);
 }
 template <int D, int MOST> void launch_stream(const AttentionDev &p, const Route &route, bool packed, hipStream_t st) {
     if (route.mt == 1) launch_stream<D, 1>(p, route.grid, packed, st);
@@ -1309,8 +1319,9 @@ template <int D, int MOST> void launch_stream(const AttentionDev &p, const Route
 }
 template <int D> void launch_tile(const AttentionDev &p, bool packed, hipStream_t st) {
     constexpr uint32_t threads = TileShape<D, false>::WAVES * 64;
-    if (packed) hipLaunchKernelGGL((paged_attention_tile_kernel<D, true>), dim3(TILE_TARGET), dim3(threads), 0, st, p);
-    else hipLaunchKernelGGL((paged_attention_tile_kernel<D, false>), dim3(TILE_TARGET), dim3(threads), 0, st, p);
+    auto launch = [&](auto plain, auto sinks) { hipLaunchKernelGGL(p.sinks ? sinks : plain, dim3(TILE_TARGET), dim3(threads), 0, st, p); };
+    if (packed) launch(paged_attention_tile_kernel<D, true, false>, paged_attention_tile_kernel<D, true, true>);
+    else launch(paged_attention_tile_kernel<D, false, false>, paged_attention_tile_kernel<D, false, true>);
 }
 }  // namespace
 
@@ -1329,6 +1340,7 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     p.width = x.rows.width; p.query_column = x.query_column; p.requests = x.step.requests; p.max_pages = x.step.max_pages;
     p.pages = c.pages; p.kv_heads = c.kv_heads; p.page_blocks = c.page_size / 32;
     p.heads = x.heads; p.group = x.heads / c.kv_heads; p.window = x.window;
+    p.sinks = x.window ? x.sinks : 0;      // without a window they are seen anyway
     const bool packed = c.dtype == TTMI_BFLOAT8_B;
     // a scale of zero stands for the smallest number there is: -inf, what is masked, has to stay -inf, and the largest score is 2^-21
     p.scale = std::max(std::fabs(x.scale) * 1.4426950408889634f, 0x1p-149f);

@@ -1,0 +1,241 @@
+// Pages of a key/value cache that several requests have in common, that change hands, and that nobody needs any longer.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "bfp_dequant.h"
+#include "paged_cache.h"
+#include "ttmi_internal.h"
+
+namespace ttmi {
+
+__device__ __forceinline__ uint32_t tokens_of(int32_t length) { return (uint32_t)max(length, 0); }
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Forks.  Row i of the new table goes on from row parent_i of the old one.  With n tokens of the parent and pages of S,
+//   entry j = the parent's for j S < n, else -1
+// but for the page begun, j = n / S where S does not divide n: the first of a parent's continuations keeps it, each other one takes the next
+// page from the list, in the order of the continuations, into which the one begun is to be copied.
+// As the tables of a step are made: every workgroup finds the first continuations (LDS, atomic minimum) and makes the prefix sum for itself,
+// then the entries are dealt out.  Bound by the launch and three loads that wait for each other (parents, lengths, the page begun).
+// ---------------------------------------------------------------------------------------------------------------------------------
+struct ForkDev {
+    const int32_t *table, *lengths, *parents, *free_pages;
+    int32_t *table_out, *lengths_out, *sources, *targets, *counts;
+    uint32_t requests, max_pages, page_size, children, free_count;
+};
+
+__global__ __launch_bounds__(256) void paged_fork_kernel(const ForkDev p) {
+    extern __shared__ uint32_t lds[];                          // first[requests], taken[children]: pages taken up to and by a continuation, bit 31: one by itself
+    uint32_t *const first = lds, *const taken = lds + p.requests;
+    __shared__ uint32_t wave_sum[4];
+    constexpr uint32_t COPIES = 0x80000000u;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    auto parent_of = [&](uint32_t i) { return (uint32_t)p.parents[i]; };
+    for (uint32_t r = threadIdx.x; r < p.requests; r += 256) first[r] = 0xffffffffu;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < p.children; i += 256)
+        if (const uint32_t r = parent_of(i); r < p.requests) atomicMin(first + r, i);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < p.children; i += 256) {
+        const uint32_t r = parent_of(i);
+        bool copies = false;
+        if (r < p.requests && first[r] != i) {
+            const uint32_t n = tokens_of(p.lengths[r]), j = n / p.page_size;
+            copies = n % p.page_size && j < p.max_pages && p.table[(uint64_t)r * p.max_pages + j] >= 0;
+        }
+        taken[i] = copies ? COPIES : 0;
+    }
+    __syncthreads();
+    const uint32_t each = (p.children + 255) / 256, i0 = min(threadIdx.x * each, p.children), i1 = min(i0 + each, p.children);
+    uint32_t sum = 0;
+    for (uint32_t i = i0; i < i1; ++i) sum += taken[i] >> 31;
+    uint32_t to = running_sum(sum);
+    if (lane == 63) wave_sum[wave] = to;
+    __syncthreads();
+    to -= sum;
+    for (uint32_t w = 0; w < wave; ++w) to += wave_sum[w];
+    for (uint32_t i = i0; i < i1; ++i) {
+        const uint32_t flag = taken[i];
+        taken[i] = flag | to;
+        to += flag >> 31;
+    }
+    const uint32_t all = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+    __syncthreads();
+
+    auto fresh = [&](uint32_t i) {                             // the page that continuation i copies into
+        const uint32_t at = taken[i] & ~COPIES;
+        return at < p.free_count ? p.free_pages[at] : -1;
+    };
+    const uint64_t entries = (uint64_t)p.children * p.max_pages, step = (uint64_t)gridDim.x * 256, id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    for (uint64_t e = id; e < entries; e += step) {
+        const uint32_t i = (uint32_t)(e / p.max_pages), j = (uint32_t)(e - (uint64_t)i * p.max_pages), r = parent_of(i);
+        int32_t page = -1;
+        if (r < p.requests) {
+            const uint32_t n = tokens_of(p.lengths[r]);
+            if ((taken[i] & COPIES) && j == n / p.page_size) page = fresh(i);
+            else if ((uint64_t)j * p.page_size < n) page = p.table[(uint64_t)r * p.max_pages + j];
+        }
+        p.table_out[e] = page;
+    }
+    for (uint64_t e = id; e < p.children; e += step) {
+        const uint32_t i = (uint32_t)e, r = parent_of(i), n = r < p.requests ? tokens_of(p.lengths[r]) : 0;
+        p.lengths_out[i] = (int32_t)n;
+        const int32_t target = taken[i] & COPIES ? fresh(i) : -1;
+        p.targets[i] = target >= 0 ? target : -1;
+        p.sources[i] = target >= 0 ? p.table[(uint64_t)r * p.max_pages + n / p.page_size] : -1;
+    }
+    if (id == 0) {
+        const uint32_t got = min(all, p.free_count);
+        p.counts[0] = (int32_t)got;
+        p.counts[1] = (int32_t)(all - got);
+    }
+}
+
+int paged_fork(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, const int32_t *parents, uint32_t children,
+               const int32_t *free_pages, uint32_t free_count, int32_t *table_out, int32_t *lengths_out, int32_t *sources, int32_t *targets, int32_t *counts, hipStream_t st) {
+    const ForkDev p{page_table, lengths, parents, free_pages, table_out, lengths_out, sources, targets, counts, requests, max_pages, page_size, children, free_count};
+    const uint64_t work = std::max<uint64_t>((uint64_t)children * max_pages, children);
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((work + 255) / 256, 1), 512);
+    hipLaunchKernelGGL(paged_fork_kernel, dim3(blocks), dim3(256), ((size_t)requests + children) * 4, st, p);
+    return check_launch("paged_fork_kernel");
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Copies of whole pages, the same ones in every cache of a model.  A page is contiguous: a workgroup moves 16 KB of one.
+// ---------------------------------------------------------------------------------------------------------------------------------
+constexpr uint32_t CACHES = 128;           // of one launch: their addresses are kernel arguments
+struct CopyDev {
+    uint8_t *caches[CACHES];
+    const int32_t *sources, *targets;
+    uint64_t page_bytes, items;
+    uint32_t count, pages, pairs, pieces;  // pieces of a page
+};
+constexpr uint32_t COPY_LOADS = 4, COPY_PIECE = 256 * 16 * COPY_LOADS;
+
+__global__ __launch_bounds__(256) void paged_copy_kernel(const CopyDev p) {
+    for (uint64_t item = blockIdx.x; item < p.items; item += gridDim.x) {
+        const uint32_t piece = (uint32_t)(item % p.pieces);
+        const uint64_t rest = item / p.pieces;
+        const uint32_t which = (uint32_t)(rest % p.count), pair = (uint32_t)(rest / p.count);
+        const uint32_t source = (uint32_t)p.sources[pair], target = (uint32_t)p.targets[pair];
+        if (source >= p.pages || target >= p.pages || source == target) continue;
+        uint8_t *const cache = p.caches[which];
+        const uint64_t at = (uint64_t)piece * COPY_PIECE + threadIdx.x * 16;
+        const uint8_t *const from = cache + source * p.page_bytes + at;
+        uint8_t *const to = cache + target * p.page_bytes + at;
+        u32x4 v[COPY_LOADS];
+#pragma unroll
+        for (uint32_t i = 0; i < COPY_LOADS; ++i)
+            if (at + i * 4096 < p.page_bytes) v[i] = *reinterpret_cast<const u32x4 *>(from + i * 4096);
+#pragma unroll
+        for (uint32_t i = 0; i < COPY_LOADS; ++i)
+            if (at + i * 4096 < p.page_bytes) *reinterpret_cast<u32x4 *>(to + i * 4096) = v[i];
+    }
+}
+
+int paged_copy(void *const *caches, uint32_t count, const PagedCache &c, const int32_t *sources, const int32_t *targets, uint32_t pairs, hipStream_t st) {
+    CopyDev p{};
+    p.sources = sources; p.targets = targets; p.pages = c.pages; p.pairs = pairs;
+    p.page_bytes = (uint64_t)c.kv_heads * (c.page_size / 32) * (c.head_dim / 32) * (c.dtype == TTMI_BFLOAT8_B ? 1088 : 2048);
+    p.pieces = (uint32_t)((p.page_bytes + COPY_PIECE - 1) / COPY_PIECE);
+    for (uint32_t first = 0; first < count; first += CACHES) {
+        p.count = std::min(CACHES, count - first);
+        for (uint32_t i = 0; i < p.count; ++i) p.caches[i] = (uint8_t *)caches[first + i];
+        p.items = (uint64_t)p.pieces * p.count * pairs;
+        if (!p.items) return TTMI_OK;
+        hipLaunchKernelGGL(paged_copy_kernel, dim3((uint32_t)std::min<uint64_t>(p.items, 1u << 20)), dim3(256), 0, st, p);
+        if (int rc = check_launch("paged_copy_kernel")) return rc;
+    }
+    return TTMI_OK;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Release.  With n tokens of a request, pages of S and a window of W (0: none) behind K sinks, entry j is kept where
+//   j S < n   and   (W = 0, or j S + S > n + 1 - W: the next token sees a token of it, or j S < K)
+// and is -1 elsewhere.  The pages that no entry kept names, in ascending order, are the new list of free pages.
+// A bit for every page says whether it is in use; the place of a free page in the list is the number of free ones before it.
+// ---------------------------------------------------------------------------------------------------------------------------------
+struct ReleaseDev {
+    const int32_t *table, *lengths;
+    int32_t *table_out, *free_pages, *counts;
+    uint32_t *bits;                        // of the pages in use, [words]
+    uint64_t entries;
+    uint32_t requests, max_pages, page_size, window, sinks, pages, words;
+};
+// Entry e of the table, if it is kept and a page, else -1.
+__device__ __forceinline__ int32_t kept_entry(const ReleaseDev &p, uint64_t e) {
+    const uint32_t r = (uint32_t)(e / p.max_pages), j = (uint32_t)(e - (uint64_t)r * p.max_pages);
+    const uint64_t n = tokens_of(p.lengths[r]), first = (uint64_t)j * p.page_size;
+    const bool kept = first < n && (!p.window || first + p.page_size + p.window > n + 1 || first < p.sinks);
+    const int32_t page = kept ? p.table[e] : -1;
+    return (uint32_t)page < p.pages ? page : -1;
+}
+// The free pages among words [word0, word1) go into the list from `place` on, a wavefront two words at a time.
+__device__ __forceinline__ uint32_t list_free(const ReleaseDev &p, const uint32_t *bits, uint32_t word0, uint32_t word1, uint32_t place) {
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t w = word0; w < word1; w += 2) {
+        const uint32_t word = w + (lane >> 5), page = word * 32 + (lane & 31);
+        const bool free = word < word1 && page < p.pages && !(bits[word] >> (lane & 31) & 1);
+        const uint64_t all = __ballot(free);
+        if (free) p.free_pages[place + __popcll(all & ((1ull << lane) - 1))] = (int32_t)page;
+        place += __popcll(all);
+    }
+    return place;
+}
+
+__global__ __launch_bounds__(256) void paged_release_clear_kernel(uint32_t *bits, uint32_t words) {
+    for (uint32_t w = blockIdx.x * 256 + threadIdx.x; w < words; w += gridDim.x * 256) bits[w] = 0;
+}
+__global__ __launch_bounds__(256) void paged_release_mark_kernel(const ReleaseDev p) {
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < p.entries; e += (uint64_t)gridDim.x * 256) {
+        const int32_t page = kept_entry(p, e);
+        p.table_out[e] = page;
+        if (page >= 0) atomicOr(p.bits + (page >> 5), 1u << (page & 31));
+    }
+}
+// A workgroup lists the free pages of 64 words after counting those in use before them.
+constexpr uint32_t LIST_WORDS = 64;
+__global__ __launch_bounds__(256) void paged_release_list_kernel(const ReleaseDev p) {
+    __shared__ uint32_t counted[4][2];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t word0 = blockIdx.x * LIST_WORDS, word1 = min(word0 + LIST_WORDS, p.words);
+    uint32_t before = 0, all = 0;          // pages in use
+    for (uint32_t w = threadIdx.x; w < p.words; w += 256) {
+        const uint32_t n = __popc(p.bits[w]);
+        all += n;
+        if (w < word0) before += n;
+    }
+    before = last_lane(running_sum(before));
+    all = last_lane(running_sum(all));
+    if (lane == 0) { counted[wave][0] = before; counted[wave][1] = all; }
+    __syncthreads();
+    before = counted[0][0] + counted[1][0] + counted[2][0] + counted[3][0];
+    all = counted[0][1] + counted[1][1] + counted[2][1] + counted[3][1];
+    // the wavefront's quarter of the words
+    uint32_t place = word0 * 32 - before;
+    const uint32_t mine = min(word0 + wave * (LIST_WORDS / 4), word1), end = min(mine + LIST_WORDS / 4, word1);
+    for (uint32_t w = word0; w < mine; ++w) place += 32 - __popc(p.bits[w]);
+    list_free(p, p.bits, mine, end, place);
+    const uint32_t free = p.pages - all;
+    for (uint64_t i = free + (uint64_t)blockIdx.x * 256 + threadIdx.x; i < p.pages; i += (uint64_t)gridDim.x * 256) p.free_pages[i] = -1;
+    if (blockIdx.x == 0 && threadIdx.x == 0) { p.counts[0] = (int32_t)free; p.counts[1] = (int32_t)all; }
+}
+
+size_t paged_release_workspace_bytes(uint32_t, uint32_t, uint32_t pages) { return ((size_t)pages + 31) / 32 * 4; }
+
+int paged_release(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, uint32_t window, uint32_t sinks, uint32_t pages,
+                  int32_t *table_out, int32_t *free_pages, int32_t *counts, void *workspace, hipStream_t st) {
+    ReleaseDev p{page_table, lengths, table_out, free_pages, counts, (uint32_t *)workspace, (uint64_t)requests * max_pages, requests, max_pages, page_size, window, sinks, pages, (pages + 31) / 32};
+    hipLaunchKernelGGL(paged_release_clear_kernel, dim3(std::min((p.words + 255) / 256, 1024u)), dim3(256), 0, st, p.bits, p.words);
+    if (int rc = check_launch("paged_release_clear_kernel")) return rc;
+    if (p.entries) {
+        hipLaunchKernelGGL(paged_release_mark_kernel, dim3((uint32_t)std::min<uint64_t>((p.entries + 255) / 256, 4096)), dim3(256), 0, st, p);
+        if (int rc = check_launch("paged_release_mark_kernel")) return rc;
+    }
+    hipLaunchKernelGGL(paged_release_list_kernel, dim3((p.words + LIST_WORDS - 1) / LIST_WORDS), dim3(256), 0, st, p);
+    return check_launch("paged_release_list_kernel");
+}
+
+}  // namespace ttmi

@@ -72,6 +72,11 @@ static int validate_paged_rows(const PagedRows &r) {
     return TTMI_OK;
 }
 static bool misaligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) & (to - 1); }
+static bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+static uint64_t bytes_of_rows(const PagedRows &r, uint64_t width) { return (r.layout == TTMI_TILE ? ((uint64_t)r.tokens + 31) / 32 * 32 : r.tokens) * width * 2; }
 
 }  // namespace ttmi
 
@@ -289,6 +294,14 @@ int ttmi_paged_attention(const void *rows, int layout, uint32_t tokens, uint32_t
                          uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, const int32_t *page_table, uint32_t requests, uint32_t max_pages,
                          const int32_t *cached, const int32_t *row_starts, uint32_t heads, float scale, uint32_t window, void *out, void *workspace, size_t workspace_bytes,
                          void *stream) {
+    return ttmi_paged_attention_sinks(rows, layout, tokens, width, query_column, key_cache, value_cache, cache_dtype, pages, kv_heads, page_size, head_dim, page_table, requests, max_pages,
+                                      cached, row_starts, heads, scale, window, 0, out, workspace, workspace_bytes, stream);
+}
+
+int ttmi_paged_attention_sinks(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t query_column, const void *key_cache, const void *value_cache, int cache_dtype,
+                               uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, const int32_t *page_table, uint32_t requests, uint32_t max_pages,
+                               const int32_t *cached, const int32_t *row_starts, uint32_t heads, float scale, uint32_t window, uint32_t sinks, void *out, void *workspace,
+                               size_t workspace_bytes, void *stream) {
     const PagedCache c{cache_dtype, pages, kv_heads, page_size, head_dim};
     const PagedRows r{rows, layout, tokens, width};
     if (int rc = validate_paged_cache(c)) return rc;
@@ -300,14 +313,109 @@ int ttmi_paged_attention(const void *rows, int layout, uint32_t tokens, uint32_t
     if (requests > PAGED_MAX_REQUESTS) return fail(TTMI_ERR_UNSUPPORTED, "paged attention: %u requests, at most %u", requests, PAGED_MAX_REQUESTS);
     if ((uint64_t)max_pages * page_size > 0x7fffffffull) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: %u pages of %u tokens are more than an int32 counts", max_pages, page_size);
     if (!(scale == scale) || scale - scale != 0.f) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: scale must be finite");
+    if (sinks > 0x7fffffffu) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: more than 2^31 - 1 sinks");
     if (!key_cache || !value_cache || !row_starts || (requests && !cached) || ((uint64_t)requests * max_pages && !page_table) || (tokens && (!rows || !out)))
         return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: null pointer");
     if (misaligned(rows, 16) || misaligned(key_cache, 16) || misaligned(value_cache, 16) || misaligned(out, 16) || misaligned(page_table, 4) || misaligned(cached, 4) || misaligned(row_starts, 4))
         return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: rows, caches and out must be 16-byte aligned, the rest 4-byte aligned");
     if (workspace && (misaligned(workspace, 256) || workspace_bytes < ttmi_paged_attention_workspace_bytes(tokens, requests, heads, cache_dtype, kv_heads, head_dim)))
         return fail(TTMI_ERR_INVALID_ARGUMENT, "paged attention: workspace of %zu bytes, 256-byte aligned, expected", ttmi_paged_attention_workspace_bytes(tokens, requests, heads, cache_dtype, kv_heads, head_dim));
-    const PagedAttentionArgs args{r, query_column, key_cache, value_cache, c, PagedStep{page_table, requests, max_pages, cached, row_starts}, heads, scale, window, out, workspace, workspace_bytes};
+    const PagedAttentionArgs args{r, query_column, key_cache, value_cache, c, PagedStep{page_table, requests, max_pages, cached, row_starts}, heads, scale, window, sinks, out, workspace, workspace_bytes};
     return paged_attention(args, (hipStream_t)stream);
+}
+
+// what both entry points ask of a rotation and of the step's lengths
+static int validate_rotation(const char *what, uint32_t heads, uint32_t head_dim, const int32_t *cached, const int32_t *row_starts, uint32_t requests, const float *frequencies,
+                             uint32_t rotary_dim, float epsilon, float magnitude) {
+    if (head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 256) return fail(TTMI_ERR_UNSUPPORTED, "%s: head dimension %u (64, 96, 128 or 256)", what, head_dim);
+    if (!heads || heads > 0x7fffffffu / head_dim) return fail(TTMI_ERR_INVALID_ARGUMENT, "%s: %u heads", what, heads);
+    if (rotary_dim > head_dim || (rotary_dim & 15)) return fail(TTMI_ERR_INVALID_ARGUMENT, "%s: rotary dimension (%u) must be a multiple of 16 and at most the head's %u", what, rotary_dim, head_dim);
+    if (requests > PAGED_MAX_REQUESTS) return fail(TTMI_ERR_UNSUPPORTED, "%s: %u requests, at most %u", what, requests, PAGED_MAX_REQUESTS);
+    if (!row_starts || (requests && !cached) || (rotary_dim && !frequencies)) return fail(TTMI_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+    if (misaligned(row_starts, 4) || misaligned(cached, 4) || misaligned(frequencies, 16)) return fail(TTMI_ERR_INVALID_ARGUMENT, "%s: frequencies must be 16-byte aligned, lengths 4-byte aligned", what);
+    if (!(epsilon >= 0.f) || epsilon - epsilon != 0.f || magnitude - magnitude != 0.f) return fail(TTMI_ERR_INVALID_ARGUMENT, "%s: epsilon must be finite and not negative, magnitude finite", what);
+    return TTMI_OK;
+}
+
+int ttmi_rotate_heads(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t column, uint32_t heads, uint32_t head_dim, const int32_t *cached, const int32_t *row_starts,
+                      uint32_t requests, const float *frequencies, uint32_t rotary_dim, int interleaved, const float *norm, float epsilon, float magnitude, void *out, void *stream) {
+    const PagedRows r{rows, layout, tokens, width};
+    if (int rc = validate_rotation("paged rotation", heads, head_dim, cached, row_starts, requests, frequencies, rotary_dim, epsilon, magnitude)) return rc;
+    if (int rc = validate_paged_rows(r)) return rc;
+    if (int rc = validate_paged_columns(r, column, (uint64_t)heads * head_dim, "head")) return rc;
+    if (tokens && (!rows || !out)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged rotation: null pointer");
+    if (misaligned(rows, 16) || misaligned(out, 16) || misaligned(norm, 16)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged rotation: rows, norm and out must be 16-byte aligned");
+    if (overlap(rows, bytes_of_rows(r, width), out, bytes_of_rows(r, (uint64_t)heads * head_dim))) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged rotation: out overlaps the rows");
+    PagedRotationArgs args{};
+    args.rows = r; args.query_column = column; args.heads = heads; args.head_dim = head_dim;
+    args.step.cached = cached; args.step.row_starts = row_starts; args.step.requests = requests;
+    args.frequencies = frequencies; args.rotary_dim = rotary_dim; args.interleaved = interleaved != 0;
+    args.query_norm = norm; args.epsilon = epsilon; args.magnitude = magnitude; args.out = out;
+    return paged_rotate(args, (hipStream_t)stream);
+}
+
+int ttmi_paged_rotate_write(const void *rows, int layout, uint32_t tokens, uint32_t width, uint32_t query_column, uint32_t heads, uint32_t key_column, uint32_t value_column,
+                            const int32_t *slots, void *key_cache, void *value_cache, int cache_dtype, uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim,
+                            const int32_t *cached, const int32_t *row_starts, uint32_t requests, const float *frequencies, uint32_t rotary_dim, int interleaved, const float *query_norm,
+                            const float *key_norm, float epsilon, float magnitude, void *out, void *stream) {
+    const PagedRows r{rows, layout, tokens, width};
+    const PagedCache c{cache_dtype, pages, kv_heads, page_size, head_dim};
+    if (int rc = validate_paged_cache(c)) return rc;
+    if (int rc = validate_rotation("paged rotation", heads, head_dim, cached, row_starts, requests, frequencies, rotary_dim, epsilon, magnitude)) return rc;
+    if (int rc = validate_paged_rows(r)) return rc;
+    if (int rc = validate_paged_columns(r, query_column, (uint64_t)heads * head_dim, "query")) return rc;
+    if (int rc = validate_paged_columns(r, key_column, (uint64_t)kv_heads * head_dim, "key")) return rc;
+    if (int rc = validate_paged_columns(r, value_column, (uint64_t)kv_heads * head_dim, "value")) return rc;
+    if (!key_cache || !value_cache || (tokens && (!rows || !slots || !out))) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged rotation: null pointer");
+    if (misaligned(rows, 16) || misaligned(out, 16) || misaligned(key_cache, 16) || misaligned(value_cache, 16) || misaligned(query_norm, 16) || misaligned(key_norm, 16) || misaligned(slots, 4))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged rotation: rows, caches, norms and out must be 16-byte aligned, slots 4-byte aligned");
+    if (overlap(rows, bytes_of_rows(r, width), out, bytes_of_rows(r, (uint64_t)heads * head_dim))) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged rotation: out overlaps the rows");
+    const PagedRotationArgs args{r, query_column, heads, head_dim, key_column, value_column, slots, key_cache, value_cache, c, PagedStep{nullptr, requests, 0, cached, row_starts},
+                                 frequencies, rotary_dim, interleaved != 0, query_norm, key_norm, epsilon, magnitude, out};
+    return paged_rotate(args, (hipStream_t)stream);
+}
+
+int ttmi_paged_fork(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, const int32_t *parents, uint32_t children,
+                    const int32_t *free_pages, uint32_t free_count, int32_t *page_table_out, int32_t *lengths_out, int32_t *sources, int32_t *targets, int32_t *counts, void *stream) {
+    if (!page_size || (page_size & 31)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged fork: page size (%u) must be a multiple of 32", page_size);
+    if (requests > PAGED_MAX_REQUESTS || children > PAGED_MAX_REQUESTS) return fail(TTMI_ERR_UNSUPPORTED, "paged fork: %u requests and %u continuations, at most %u of each", requests, children, PAGED_MAX_REQUESTS);
+    if (free_count > 0x7fffffffu) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged fork: more than 2^31 - 1 free pages");
+    if (!counts || (requests && !lengths) || ((uint64_t)requests * max_pages && !page_table) || (children && (!parents || !lengths_out || !sources || !targets)) ||
+        ((uint64_t)children * max_pages && !page_table_out) || (free_count && !free_pages))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged fork: null pointer");
+    const void *all[] = {page_table, lengths, parents, free_pages, page_table_out, lengths_out, sources, targets, counts};
+    for (const void *p : all)
+        if (misaligned(p, 4)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged fork: pointers must be 4-byte aligned");
+    if (overlap(page_table, (uint64_t)requests * max_pages * 4, page_table_out, (uint64_t)children * max_pages * 4) || overlap(lengths, (uint64_t)requests * 4, lengths_out, (uint64_t)children * 4))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged fork: the new table or lengths overlap the old ones");
+    return paged_fork(page_table, lengths, requests, max_pages, page_size, parents, children, free_pages, free_count, page_table_out, lengths_out, sources, targets, counts, (hipStream_t)stream);
+}
+
+int ttmi_paged_copy(void *const *caches, uint32_t count, int cache_dtype, uint32_t pages, uint32_t kv_heads, uint32_t page_size, uint32_t head_dim, const int32_t *sources,
+                    const int32_t *targets, uint32_t pairs, void *stream) {
+    const PagedCache c{cache_dtype, pages, kv_heads, page_size, head_dim};
+    if (int rc = validate_paged_cache(c)) return rc;
+    if ((count && !caches) || (pairs && (!sources || !targets))) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged copy: null pointer");
+    if (pairs > 0x7fffffffu) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged copy: more than 2^31 - 1 pairs");
+    if (misaligned(sources, 4) || misaligned(targets, 4)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged copy: sources and targets must be 4-byte aligned");
+    for (uint32_t i = 0; i < count; ++i)
+        if (!caches[i] || misaligned(caches[i], 16)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged copy: caches must be 16-byte aligned and not null");
+    return paged_copy(caches, count, c, sources, targets, pairs, (hipStream_t)stream);
+}
+
+size_t ttmi_paged_release_workspace_bytes(uint32_t requests, uint32_t max_pages, uint32_t pages) { return paged_release_workspace_bytes(requests, max_pages, pages); }
+
+int ttmi_paged_release(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, uint32_t window, uint32_t sinks, uint32_t pages,
+                       int32_t *page_table_out, int32_t *free_pages, int32_t *counts, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!page_size || (page_size & 31)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: page size (%u) must be a multiple of 32", page_size);
+    if (!pages || pages > 0x7fffffffu) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: %u pages", pages);
+    if (!counts || !free_pages || (requests && !lengths) || ((uint64_t)requests * max_pages && (!page_table || !page_table_out))) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: null pointer");
+    const void *all[] = {page_table, lengths, page_table_out, free_pages, counts};
+    for (const void *p : all)
+        if (misaligned(p, 4)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: pointers must be 4-byte aligned");
+    if (const size_t bytes = ttmi_paged_release_workspace_bytes(requests, max_pages, pages); bytes && (!workspace || misaligned(workspace, 256) || workspace_bytes < bytes))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: workspace of %zu bytes, 256-byte aligned, expected", bytes);
+    return paged_release(page_table, lengths, requests, max_pages, page_size, window, sinks, pages, page_table_out, free_pages, counts, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -174,6 +174,23 @@ void bind_tensor_layer(py::module_ &m) {
     m.def("paged_tables", &host::paged_tables, no_gil);
     m.def("paged_write", &host::paged_write, no_gil);
     m.def("paged_attention", &host::paged_attention, no_gil);
+    m.def("rotate_heads", [](const host::Tensor &rows, const host::Tensor &cached, const host::Tensor &row_starts, const host::Tensor &frequencies, uint32_t heads, uint32_t head_dim,
+                             uint32_t column, bool interleaved, const py::object &norm, float epsilon, float magnitude, const std::string &op) {
+        const host::Tensor *const w = optional_tensor(norm);
+        return unlocked([&] { return host::rotate_heads(rows, cached, row_starts, frequencies, heads, head_dim, column, interleaved, w, epsilon, magnitude, op); });
+    });
+    m.def("paged_rotate_write", [](const host::Tensor &rows, const host::Tensor &key_cache, const host::Tensor &value_cache, const host::Tensor &slots, const host::Tensor &cached,
+                                   const host::Tensor &row_starts, const host::Tensor &frequencies, uint32_t heads, uint32_t key_column, uint32_t value_column, uint32_t query_column,
+                                   bool interleaved, const py::object &query_norm, const py::object &key_norm, float epsilon, float magnitude, const std::string &op) {
+        const host::Tensor *const qw = optional_tensor(query_norm), *const kw = optional_tensor(key_norm);
+        return unlocked([&] {
+            return host::paged_rotate_write(rows, key_cache, value_cache, slots, cached, row_starts, frequencies, heads, key_column, value_column, query_column, interleaved, qw, kw, epsilon,
+                                            magnitude, op);
+        });
+    });
+    m.def("paged_fork", &host::paged_fork, no_gil);
+    m.def("paged_copy", &host::paged_copy, no_gil);
+    m.def("paged_release", &host::paged_release, no_gil);
     m.def("ttnn_from_torch_block_float",
           [](uintptr_t data, int src_dtype, host::Dims shape, int dtype, int device) {
               return unlocked([&] { return host::ttnn_from_torch_block_float(reinterpret_cast<const void *>(data), (host::DataType)src_dtype, shape, (host::DataType)dtype, device); });

@@ -30,6 +30,7 @@ SYMBOLS = (
     "ttmi_release_scratch", "ttmi_matmul_bfp_ab_supported", "ttmi_matmul_bfp_ab", "ttmi_matmul_bfp_plan",
     "ttmi_matmul_bias_tiles", "ttmi_matmul_bias_tiles_supported",
     "ttmi_paged_tables", "ttmi_paged_write", "ttmi_paged_attention", "ttmi_paged_attention_workspace_bytes",
+    "ttmi_paged_attention_sinks", "ttmi_rotate_heads", "ttmi_paged_rotate_write", "ttmi_paged_fork", "ttmi_paged_copy", "ttmi_paged_release", "ttmi_paged_release_workspace_bytes",
 )
 
 _lib = None
@@ -123,6 +124,21 @@ def _load(path: str) -> ctypes.CDLL:
         L.ttmi_paged_attention_workspace_bytes.argtypes = [u32, u32, u32, i32, u32, u32]
         L.ttmi_paged_attention.restype = i32
         L.ttmi_paged_attention.argtypes = [vp, i32, u32, u32, u32, vp, vp, i32, u32, u32, u32, u32, vp, u32, u32, vp, vp, u32, ctypes.c_float, u32, vp, vp, sz, vp]
+        f32 = ctypes.c_float
+        L.ttmi_paged_attention_sinks.restype = i32
+        L.ttmi_paged_attention_sinks.argtypes = [vp, i32, u32, u32, u32, vp, vp, i32, u32, u32, u32, u32, vp, u32, u32, vp, vp, u32, f32, u32, u32, vp, vp, sz, vp]
+        L.ttmi_rotate_heads.restype = i32
+        L.ttmi_rotate_heads.argtypes = [vp, i32, u32, u32, u32, u32, u32, vp, vp, u32, vp, u32, i32, vp, f32, f32, vp, vp]
+        L.ttmi_paged_rotate_write.restype = i32
+        L.ttmi_paged_rotate_write.argtypes = [vp, i32, u32, u32, u32, u32, u32, u32, vp, vp, vp, i32, u32, u32, u32, u32, vp, vp, u32, vp, u32, i32, vp, vp, f32, f32, vp, vp]
+        L.ttmi_paged_fork.restype = i32
+        L.ttmi_paged_fork.argtypes = [vp, vp, u32, u32, u32, vp, u32, vp, u32, vp, vp, vp, vp, vp, vp]
+        L.ttmi_paged_copy.restype = i32
+        L.ttmi_paged_copy.argtypes = [vp, u32, i32, u32, u32, u32, u32, vp, vp, u32, vp]
+        L.ttmi_paged_release_workspace_bytes.restype = sz
+        L.ttmi_paged_release_workspace_bytes.argtypes = [u32, u32, u32]
+        L.ttmi_paged_release.restype = i32
+        L.ttmi_paged_release.argtypes = [vp, vp, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, sz, vp]
         _loaded[path] = L
     return _loaded[path]
 

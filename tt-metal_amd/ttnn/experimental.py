@@ -2,4 +2,5 @@
 from __future__ import annotations
 
 from .matmul import gated_linear  # noqa: F401
-from .paged import allocate_paged_cache, attend_paged_cache, paged_tables, write_paged_cache  # noqa: F401
+from .paged import (allocate_paged_cache, attend_paged_cache, copy_paged_pages, fork_paged_tables, paged_tables, release_paged_pages,  # noqa: F401
+                    rotary_frequencies, rotate_heads, rotate_write_paged_cache, write_paged_cache)
