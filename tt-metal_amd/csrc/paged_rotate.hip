@@ -28,20 +28,20 @@ struct RotateDev {
     uint32_t each;                             // heads of an item
     uint32_t pages, page_size, turning;
     float epsilon, magnitude;
-    int tiled, interleaved, packed;
+    int tiled;
 };
 
-// Position of row t0 + r, r = 0 .. 15, false where it is no request's.  A row belongs to the request before the first start behind it, and
+// Position of row t0 + r, r < ROWS, false where it is no request's.  A row belongs to the request before the first start behind it, and
 // the request's rows begin at the largest start up to its own: row starts that do not ascend are read through their running maximum.
-__device__ __forceinline__ bool position_of(const RotateDev &p, uint32_t t0, uint32_t r, uint32_t &position) {
+template <uint32_t ROWS> __device__ __forceinline__ bool position_of(const RotateDev &p, uint32_t t0, uint32_t r, uint32_t &position) {
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t owner = 0xffffffffu, from = 0, top = 0, open = 0xffffu;      // rows whose request is still looked for
+    uint32_t owner = 0xffffffffu, from = 0, top = 0, open = (1u << ROWS) - 1;      // rows whose request is still looked for
     for (uint32_t base = 0; base <= p.requests && open; base += 64) {
         const uint32_t v = base + lane <= p.requests ? min((uint32_t)max(p.starts[base + lane], 0), p.tokens) : 0xffffffffu;
         const uint32_t to = max(running_max(v), top);
         if (__ballot(to > t0))
 #pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
+            for (uint32_t i = 0; i < ROWS; ++i) {
                 const uint64_t behind = __ballot(to > t0 + i);
                 if (!(open >> i & 1) || !behind) continue;
                 open &= ~(1u << i);
@@ -58,180 +58,216 @@ __device__ __forceinline__ bool position_of(const RotateDev &p, uint32_t t0, uin
     return true;
 }
 
-// An item is up to `each` heads of 16 tokens.  Four lanes share a token; a lane has SLOTS pairs of chunks of 8 elements, chosen such that partners of
-// the rotation are in one lane: chunks k and k + R/16, or neighbours.
-template <int SLABS, bool NORM>
+// Codes of 8 of a face row's 16 numbers, lowest element in the lowest byte.  Ordinary rows (shared exponent 32 <= E < 255, or nothing but zeros):
+// floor(v + 1/2) = trunc(fma(|x|, 2^(133 - E), 1/2 - 2^-25)) with v = |x| 2^(133 - E), for every 24-bit mantissa; 2^7 becomes 2^7 - 1, zeros lose their sign.
+__device__ __forceinline__ uint32_t ordinary_codes(const float *x, float scale) {
+    constexpr uint32_t TOP = 0x80808080u, LOW = 0x7f7f7f7fu;
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m |= (uint32_t)fmaf(fabsf(x[e]), scale, 0.5f - 0x1p-25f) << (8 * e);
+    const uint32_t signs = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x0c0c0703u) | __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07030c0cu);
+    m -= (m & TOP) >> 7;
+    return (signs & (m + LOW) & TOP) | m;
+}
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t shared, bool ordinary) {
+    if (ordinary) {
+        const float scale = shared < 32u ? 0.f : __uint_as_float((260u - shared) << 23);
+        return make_uint2(ordinary_codes(x, scale), ordinary_codes(x + 4, scale));
+    }
+    uint32_t words[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) words[i >> 2] |= to_code<7>(__float_as_uint(x[i]), shared) << (8 * (i & 3));
+    return make_uint2(words[0], words[1]);
+}
+
+// An item is up to `each` heads of a few tokens.  LANES lanes share a token; each has two chunks of 8 elements of a head, chosen such that partners
+// of the rotation are in one lane: chunks k and k + R/16, or neighbours.  Angles are computed once for all heads of the item.
+template <int SLABS, bool NORM, bool INTERLEAVED, bool PACKED>
 __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
-    constexpr uint32_t D = SLABS * 32, PAIRS = SLABS * 2, SLOTS = (PAIRS + 3) / 4;
-    __shared__ uint32_t tops[4][16 * 4 * SLABS];               // largest exponent of every chunk
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t r = p.tiled ? lane >> 1 & 15 : lane >> 2, q = p.tiled ? (lane >> 5) * 2 + (lane & 1) : lane & 3;
+    constexpr uint32_t D = SLABS * 32, PAIRS = SLABS * 2, LANES = PAIRS <= 4 ? 4 : PAIRS <= 8 ? 8 : 16, ROWS = 64 / LANES;
+    __shared__ uint32_t tops[4][ROWS * 4 * SLABS];             // largest exponent of every chunk
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t r = p.tiled ? lane >> 1 & (ROWS - 1) : lane / LANES, q = p.tiled ? lane / (2 * ROWS) * 2 + (lane & 1) : lane % LANES;
     const uint32_t per_band = p.blocks[0] + p.blocks[1] + p.blocks[2];
+    const bool mine = LANES == PAIRS || q < PAIRS;
 
     for (uint64_t item = (uint64_t)blockIdx.x * 4 + wave; item < p.items; item += (uint64_t)gridDim.x * 4) {
         const uint32_t band = (uint32_t)(item / per_band);
         uint32_t block = (uint32_t)(item - (uint64_t)band * per_band), kind = QUERIES;
         while (block >= p.blocks[kind]) block -= p.blocks[kind++];
         const uint32_t head0 = block * p.each, head1 = min(head0 + p.each, p.heads[kind]);
-        const uint32_t t0 = band * 16, t = t0 + r, column = p.column[kind];
+        const uint32_t t0 = band * ROWS, t = t0 + r;
         const uint32_t turning16 = kind == VALUES ? 0 : p.turning / 16;
+        const bool turns = q < turning16, apart = turns && !INTERLEAVED;
+        const uint32_t at[2] = {apart ? q : 2 * q, apart ? q + turning16 : 2 * q + 1};
 
-        uint32_t at[SLOTS][2];                                 // chunks of a head; this lane has none where the first is past the head
+        // what this lane reads, head by head
+        const uint32_t head_step = p.tiled ? SLABS * 2048 : D * 2;
+        const bool exists = t < p.tokens && mine;
+        const uint8_t *from[2];
 #pragma unroll
-        for (uint32_t s = 0; s < SLOTS; ++s) {
-            const uint32_t k = s * 4 + q;
-            const bool apart = k < turning16 && !p.interleaved;
-            at[s][0] = apart ? k : 2 * k;
-            at[s][1] = apart ? k + turning16 : 2 * k + 1;
-        }
-        u32x4 raw[SLOTS][2];
-        auto load = [&](uint32_t head) __attribute__((always_inline)) {
+        for (int h = 0; h < 2; ++h) from[h] = p.rows + row_bytes_at(t, p.width, p.column[kind] + head0 * D + at[h] * 8, p.tiled);
+        u32x4 raw[2][2];
+        auto load = [&](u32x4 (&v)[2]) __attribute__((always_inline)) {
 #pragma unroll
-            for (uint32_t s = 0; s < SLOTS; ++s)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    raw[s][h] = t < p.tokens && s * 4 + q < PAIRS ? *reinterpret_cast<const u32x4 *>(p.rows + row_bytes_at(t, p.width, column + head * D + at[s][h] * 8, p.tiled)) : u32x4{0, 0, 0, 0};
+            for (int h = 0; h < 2; ++h) {
+                v[h] = exists ? *reinterpret_cast<const u32x4 *>(from[h]) : u32x4{0, 0, 0, 0};
+                from[h] += head_step;
+            }
         };
-        load(head0);
-        uint32_t position = 0;
-        const bool owned = position_of(p, t0, r, position);
-
-        // where this lane's token goes
-        uint32_t page = 0, within = 0;
-        bool stored = t < p.out_rows;
-        if (kind != QUERIES) {
-            const int32_t slot = owned ? p.slots[t] : -1;
-            page = (uint32_t)max(slot, 0) / p.page_size;
-            within = (uint32_t)max(slot, 0) - page * p.page_size;
-            stored = slot >= 0 && page < p.pages;
+        load(raw[0]);
+        if (head0 + 1 < head1) load(raw[1]);
+        const float *const norm = NORM && kind != VALUES ? p.norm[kind] : nullptr;
+        float weight[2][8], cosine[8], sine[8];
+        if (NORM && norm && mine) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) weight[h][i] = norm[at[h] * 8 + i];
         }
-        float cosine[SLOTS][8], sine[SLOTS][8], weight[SLOTS][2][8];
+        if (turns) {
 #pragma unroll
-        for (uint32_t s = 0; s < SLOTS; ++s) {
-            const uint32_t k = s * 4 + q;
-            if (k < turning16) {
+            for (int i = 0; i < 8; ++i) cosine[i] = p.frequencies[q * 8 + i];
+        }
+        uint32_t position = 0;
+        const bool owned = position_of<ROWS>(p, t0, r, position);
+        // where this lane's chunks go
+        bool stored = t < p.out_rows && mine;
+        uint8_t *to[2], *exponent[2];
+        uint64_t to_step = head_step;
+        if (kind == QUERIES) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    double turns = (double)position * ((double)p.frequencies[k * 8 + i] * 0.15915494309189533577);
-                    turns -= rint(turns);
-                    cosine[s][i] = __builtin_amdgcn_cosf((float)turns) * p.magnitude;
-                    sine[s][i] = __builtin_amdgcn_sinf((float)turns) * p.magnitude;
-                }
+            for (int h = 0; h < 2; ++h) to[h] = p.out + row_bytes_at(t, p.heads[QUERIES] * D, head0 * D + at[h] * 8, p.tiled);
+        } else {
+            const int32_t slot = owned ? p.slots[t] : -1;
+            const uint32_t page = (uint32_t)max(slot, 0) / p.page_size, within = (uint32_t)max(slot, 0) - page * p.page_size;
+            stored = slot >= 0 && page < p.pages && mine;
+            const uint32_t tile_bytes = PACKED ? 1088 : 2048;
+            to_step = (uint64_t)(p.page_size / 32) * SLABS * tile_bytes;
+            uint8_t *const token = p.cache[kind - KEYS] + ((uint64_t)page * p.heads[kind] + head0) * to_step + (uint64_t)(within / 32) * SLABS * tile_bytes;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t c = at[h], face = (within >> 4 & 1) * 2 + (c >> 1 & 1), row = face * 16 + (within & 15);
+                uint8_t *const tile = token + c / 4 * tile_bytes;
+                to[h] = tile + (PACKED ? 64 + row * 16 + (c & 1) * 8 : row * 32 + (c & 1) * 16);
+                exponent[h] = tile + row;
             }
-            if (NORM && kind != VALUES && p.norm[kind] && k < PAIRS) {
+        }
+        if (turns) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                double turn = (double)position * ((double)cosine[i] * 0.15915494309189533577);
+                turn -= rint(turn);
+                cosine[i] = __builtin_amdgcn_cosf((float)turn) * p.magnitude;
+                sine[i] = __builtin_amdgcn_sinf((float)turn) * p.magnitude;
+                __builtin_amdgcn_sched_barrier(0);             // one after the other: eight at once are 40 registers more
+            }
+        }
+
+        auto work = [&](const u32x4 (&v)[2]) __attribute__((always_inline)) {
+            if (kind == VALUES && !PACKED) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) weight[s][h][i] = p.norm[kind][at[s][h] * 8 + i];
+                    if (stored) *reinterpret_cast<u32x4 *>(to[h]) = v[h];
+                return;
             }
-        }
-
-        for (uint32_t head = head0; head < head1; ++head) {
-            float x[SLOTS][2][8];
-            u32x4 kept[SLOTS][2];
+            float x[2][8];
 #pragma unroll
-            for (uint32_t s = 0; s < SLOTS; ++s)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    kept[s][h] = raw[s][h];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[s][h][2 * i] = __uint_as_float(raw[s][h][i] << 16);
-                        x[s][h][2 * i + 1] = __uint_as_float(raw[s][h][i] & 0xffff0000u);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    x[h][2 * i] = __uint_as_float(v[h][i] << 16);
+                    x[h][2 * i + 1] = __uint_as_float(v[h][i] & 0xffff0000u);
                 }
-            if (head + 1 < head1) load(head + 1);
-            if (NORM && kind != VALUES && p.norm[kind]) {
+            if (NORM && norm) {
                 float sum = 0.f;
 #pragma unroll
-                for (uint32_t s = 0; s < SLOTS; ++s)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) sum = fmaf(x[s][h][i], x[s][h][i], sum);
+                    for (int i = 0; i < 8; ++i) sum = fmaf(x[h][i], x[h][i], sum);
                 sum += __shfl_xor(sum, 1);
-                sum += __shfl_xor(sum, p.tiled ? 32 : 2);
+#pragma unroll
+                for (uint32_t d = 2; d < LANES; d <<= 1) sum += __shfl_xor(sum, p.tiled ? d * ROWS : d);
                 const float by = rsqrtf(sum * (1.f / D) + p.epsilon);
 #pragma unroll
-                for (uint32_t s = 0; s < SLOTS; ++s)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[s][h][i] *= by * weight[s][h][i];
+                    for (int i = 0; i < 8; ++i) x[h][i] *= by * weight[h][i];
             }
-#pragma unroll
-            for (uint32_t s = 0; s < SLOTS; ++s) {
-                if (s * 4 + q >= turning16) continue;
+            if (turns) {
                 auto turn = [&](float &a, float &b, int i) __attribute__((always_inline)) {
-                    const float c = cosine[s][i], d = sine[s][i], old = a;
+                    const float c = cosine[i], d = sine[i], old = a;
                     a = fmaf(a, c, -(b * d));
                     b = fmaf(b, c, old * d);
                 };
-                if (p.interleaved) {
+                if (INTERLEAVED) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) turn(x[s][i >> 2][(i & 3) * 2], x[s][i >> 2][(i & 3) * 2 + 1], i);
+                    for (int i = 0; i < 8; ++i) turn(x[i >> 2][(i & 3) * 2], x[i >> 2][(i & 3) * 2 + 1], i);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) turn(x[s][0][i], x[s][1][i], i);
+                    for (int i = 0; i < 8; ++i) turn(x[0][i], x[1][i], i);
                 }
             }
-            auto rounded = [&](const float (&v)[8]) __attribute__((always_inline)) {
-                return u32x4{f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]), f32x2_to_bf16x2_rne(v[4], v[5]), f32x2_to_bf16x2_rne(v[6], v[7])};
-            };
-            if (kind == QUERIES) {
+            if (kind == QUERIES || !PACKED) {
 #pragma unroll
-                for (uint32_t s = 0; s < SLOTS; ++s)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (stored && s * 4 + q < PAIRS)
-                            *reinterpret_cast<u32x4 *>(p.out + row_bytes_at(t, p.heads[QUERIES] * D, head * D + at[s][h] * 8, p.tiled)) = owned ? rounded(x[s][h]) : u32x4{0, 0, 0, 0};
-                continue;
-            }
-            uint8_t *const cache = p.cache[kind - KEYS];
-            const uint64_t tile0 = (((uint64_t)page * p.heads[kind] + head) * (p.page_size / 32) + within / 32) * SLABS;
-            if (!p.packed) {
-#pragma unroll
-                for (uint32_t s = 0; s < SLOTS; ++s)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t c = at[s][h];
-                        if (stored && s * 4 + q < PAIRS)
-                            *reinterpret_cast<u32x4 *>(cache + (tile0 + c / 4) * 2048 + ((within >> 4 & 1) * 2 + (c >> 1 & 1)) * 512 + (within & 15) * 32 + (c & 1) * 16) = kind == VALUES ? kept[s][h] : rounded(x[s][h]);
-                    }
-                continue;
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4 rounded = {f32x2_to_bf16x2_rne(x[h][0], x[h][1]), f32x2_to_bf16x2_rne(x[h][2], x[h][3]), f32x2_to_bf16x2_rne(x[h][4], x[h][5]), f32x2_to_bf16x2_rne(x[h][6], x[h][7])};
+                    if (stored) *reinterpret_cast<u32x4 *>(to[h]) = owned ? rounded : u32x4{0, 0, 0, 0};
+                }
+                return;
             }
             // block floats: two neighbouring chunks share an exponent, and lie in one lane or in two
             uint32_t *const top = tops[wave] + r * (4 * SLABS);
-            uint32_t own[SLOTS][2];
+            uint32_t shared[2];
+            bool odd = false;
 #pragma unroll
-            for (uint32_t s = 0; s < SLOTS; ++s)
+            for (int h = 0; h < 2; ++h) {
+                shared[h] = 0;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    own[s][h] = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) own[s][h] = max(own[s][h], __float_as_uint(x[s][h][i]) >> 23 & 0xffu);
-                    if (s * 4 + q < PAIRS) top[at[s][h]] = own[s][h];
-                }
+                for (int i = 0; i < 8; ++i) shared[h] = max(shared[h], __float_as_uint(x[h][i]) & 0x7fffffffu);
+                if (mine) top[at[h]] = shared[h];
+            }
             __builtin_amdgcn_wave_barrier();
             asm volatile("" ::: "memory");
 #pragma unroll
-            for (uint32_t s = 0; s < SLOTS; ++s)
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t largest = mine ? max(shared[h], top[at[h] ^ 1]) : 0;
+                shared[h] = largest >> 23;
+                odd |= (shared[h] < 32u && largest != 0) || shared[h] == 255u;
+            }
+            const bool ordinary = __ballot(odd) == 0;          // asked once for the wavefront
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t c = at[s][h];
-                    if (!stored || s * 4 + q >= PAIRS) continue;
-                    const uint32_t shared = max(own[s][h], top[c ^ 1]), face = (within >> 4 & 1) * 2 + (c >> 1 & 1);
-                    uint32_t words[2] = {0, 0};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) words[i >> 2] |= to_code<7>(__float_as_uint(x[s][h][i]), shared) << (8 * (i & 3));
-                    uint8_t *const to = cache + (tile0 + c / 4) * 1088;
-                    *reinterpret_cast<uint2 *>(to + 64 + face * 256 + (within & 15) * 16 + (c & 1) * 8) = make_uint2(words[0], words[1]);
-                    if (!(c & 1)) to[face * 16 + (within & 15)] = (uint8_t)shared;
+            for (int h = 0; h < 2; ++h) {
+                const uint2 codes = codes_of(x[h], shared[h], ordinary);
+                if (stored) {
+                    *reinterpret_cast<uint2 *>(to[h]) = codes;
+                    if (!(at[h] & 1)) *exponent[h] = (uint8_t)shared[h];
                 }
+            }
             __builtin_amdgcn_wave_barrier();
             asm volatile("" ::: "memory");
+        };
+        for (uint32_t head = head0; head < head1; ++head) {
+            const u32x4 v[2] = {raw[0][0], raw[0][1]};
+            raw[0][0] = raw[1][0]; raw[0][1] = raw[1][1];
+            if (head + 2 < head1) load(raw[1]);
+            work(v);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { to[h] += to_step; exponent[h] += to_step; }
         }
     }
+}
+
+template <int SLABS, bool NORM, bool INTERLEAVED> static void launch(const RotateDev &p, bool packed, dim3 grid, hipStream_t st) {
+    if (packed) hipLaunchKernelGGL((paged_rotate_kernel<SLABS, NORM, INTERLEAVED, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_rotate_kernel<SLABS, NORM, INTERLEAVED, false>), grid, dim3(256), 0, st, p);
+}
+template <int SLABS> static void launch(const RotateDev &p, const PagedRotationArgs &x, dim3 grid, hipStream_t st) {
+    const bool norm = x.query_norm || x.key_norm, packed = x.key_cache && x.cache.dtype == TTMI_BFLOAT8_B;
+    if (norm && x.interleaved) launch<SLABS, true, true>(p, packed, grid, st);
+    else if (norm) launch<SLABS, true, false>(p, packed, grid, st);
+    else if (x.interleaved) launch<SLABS, false, true>(p, packed, grid, st);
+    else launch<SLABS, false, false>(p, packed, grid, st);
 }
 
 int paged_rotate(const PagedRotationArgs &x, hipStream_t st) {
@@ -248,21 +284,19 @@ int paged_rotate(const PagedRotationArgs &x, hipStream_t st) {
     p.heads[0] = x.heads;
     if (x.key_cache) p.heads[1] = p.heads[2] = x.cache.kv_heads;
     p.pages = x.cache.pages; p.page_size = std::max(x.cache.page_size, 32u);
-    p.turning = x.rotary_dim; p.interleaved = x.interleaved;
+    p.turning = x.rotary_dim;
     p.epsilon = x.epsilon; p.magnitude = x.magnitude;
-    p.packed = x.cache.dtype == TTMI_BFLOAT8_B;
-    const uint64_t bands = ((uint64_t)p.out_rows + 15) / 16, heads = (uint64_t)p.heads[0] + p.heads[1] + p.heads[2];
-    p.each = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(bands * heads / 8192, 1), 8);
+    const uint32_t rows = x.head_dim == 64 ? 16 : x.head_dim == 256 ? 4 : 8;       // tokens of an item
+    const uint64_t bands = ((uint64_t)p.out_rows + rows - 1) / rows, heads = (uint64_t)p.heads[0] + p.heads[1] + p.heads[2];
+    p.each = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(bands * heads / 8192, 1), 4);
     for (int k = 0; k < 3; ++k) p.blocks[k] = (p.heads[k] + p.each - 1) / p.each;
     p.items = bands * (p.blocks[0] + p.blocks[1] + p.blocks[2]);
     const dim3 grid((uint32_t)std::min<uint64_t>((p.items + 3) / 4, 1u << 20));
-    const bool norm = x.query_norm || x.key_norm;
-    auto launch = [&](auto plain, auto normed) { hipLaunchKernelGGL(norm ? normed : plain, grid, dim3(256), 0, st, p); };
     switch (x.head_dim) {
-        case 64: launch(paged_rotate_kernel<2, false>, paged_rotate_kernel<2, true>); break;
-        case 96: launch(paged_rotate_kernel<3, false>, paged_rotate_kernel<3, true>); break;
-        case 128: launch(paged_rotate_kernel<4, false>, paged_rotate_kernel<4, true>); break;
-        default: launch(paged_rotate_kernel<8, false>, paged_rotate_kernel<8, true>); break;
+        case 64: launch<2>(p, x, grid, st); break;
+        case 96: launch<3>(p, x, grid, st); break;
+        case 128: launch<4>(p, x, grid, st); break;
+        default: launch<8>(p, x, grid, st); break;
     }
     return check_launch("paged_rotate_kernel");
 }
