@@ -154,87 +154,146 @@ int paged_copy(void *const *caches, uint32_t count, const PagedCache &c, const i
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Release.  With n tokens of a request, pages of S and a window of W (0: none) behind K sinks, entry j is kept where
 //   j S < n   and   (W = 0, or j S + S > n + 1 - W: the next token sees a token of it, or j S < K)
-// and is -1 elsewhere.  The pages that no entry kept names, in ascending order, are the new list of free pages.
-// A bit for every page says whether it is in use; the place of a free page in the list is the number of free ones before it.
+// and is -1 elsewhere.  The pages that no entry kept names, in ascending order, are the new list of free pages: the place of a free page in
+// it is the number of free ones before it.
+// Small tables and pools: one launch, in which every workgroup marks the pages in use in its own LDS from the whole table and writes its share of
+// the results.  Large ones: a byte of memory for every page, which is cleared, set by plain stores (all of them store the same, so nothing has to be
+// atomic: 1000 requests with a common page would wait for each other), and counted by every workgroup up to its share.
 // ---------------------------------------------------------------------------------------------------------------------------------
 struct ReleaseDev {
     const int32_t *table, *lengths;
     int32_t *table_out, *free_pages, *counts;
-    uint32_t *bits;                        // of the pages in use, [words]
-    uint64_t entries;
-    uint32_t requests, max_pages, page_size, window, sinks, pages, words;
+    uint8_t *used;                         // one byte for every page, whole 256 of them
+    uint32_t requests, max_pages, page_size, window, sinks, pages, share;
 };
-// Entry e of the table, if it is kept and a page, else -1.
-__device__ __forceinline__ int32_t kept_entry(const ReleaseDev &p, uint64_t e) {
-    const uint32_t r = (uint32_t)(e / p.max_pages), j = (uint32_t)(e - (uint64_t)r * p.max_pages);
+// Entry j of request r, if it is kept and a page, else -1.
+__device__ __forceinline__ int32_t kept_entry(const ReleaseDev &p, uint32_t r, uint32_t j, uint64_t e) {
     const uint64_t n = tokens_of(p.lengths[r]), first = (uint64_t)j * p.page_size;
     const bool kept = first < n && (!p.window || first + p.page_size + p.window > n + 1 || first < p.sinks);
-    const int32_t page = kept ? p.table[e] : -1;
-    return (uint32_t)page < p.pages ? page : -1;
+    const int32_t page = p.table[e];
+    return kept && (uint32_t)page < p.pages ? page : -1;
 }
-// The free pages among words [word0, word1) go into the list from `place` on, a wavefront two words at a time.
-__device__ __forceinline__ uint32_t list_free(const ReleaseDev &p, const uint32_t *bits, uint32_t word0, uint32_t word1, uint32_t place) {
-    const uint32_t lane = threadIdx.x & 63;
-    for (uint32_t w = word0; w < word1; w += 2) {
+// sum of v over the workgroup
+template <uint32_t WAVES> __device__ __forceinline__ uint32_t sum_over_all(uint32_t v, uint32_t *lds) {
+    v = last_lane(running_sum(v));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w) v += lds[w];
+    return v;
+}
+__device__ __forceinline__ void finish_list(const ReleaseDev &p, uint32_t used) {
+    const uint32_t free = p.pages - used;
+    for (uint64_t i = (uint64_t)free + blockIdx.x * blockDim.x + threadIdx.x; i < p.pages; i += (uint64_t)gridDim.x * blockDim.x) p.free_pages[i] = -1;
+    if (blockIdx.x == 0 && threadIdx.x == 0) { p.counts[0] = (int32_t)free; p.counts[1] = (int32_t)used; }
+}
+
+constexpr uint32_t SMALL_TABLE = 1u << 16, SMALL_POOL = 1u << 18;                 // entries, pages
+__global__ __launch_bounds__(1024) void paged_release_small_kernel(const ReleaseDev p) {
+    extern __shared__ uint32_t bits[];                         // of the pages in use
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t words = (p.pages + 31) / 32, entries = p.requests * p.max_pages;
+    for (uint32_t w = threadIdx.x; w < words; w += 1024) bits[w] = 0;
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < entries; e += 1024) {
+        const uint32_t r = e / p.max_pages;
+        const int32_t page = kept_entry(p, r, e - r * p.max_pages, e);
+        if (page >= 0) atomicOr(bits + (page >> 5), 1u << (page & 31));
+        if (e / 1024 % gridDim.x == blockIdx.x) p.table_out[e] = page;
+    }
+    __syncthreads();
+    // words of this wavefront: its part of the workgroup's share, in whole pairs
+    const uint32_t all_waves = gridDim.x * 16, each = ((words + all_waves - 1) / all_waves + 1) / 2 * 2;
+    const uint32_t first = min((blockIdx.x * 16 + wave) * each, words), end = min(first + each, words);
+    uint32_t before = 0, used = 0;
+    for (uint32_t w = lane; w < words; w += 64) {              // each wavefront for itself: LDS, and no barrier
+        const uint32_t n = __popc(bits[w]);
+        used += n;
+        if (w < first) before += n;
+    }
+    before = last_lane(running_sum(before));
+    used = last_lane(running_sum(used));
+    uint32_t place = first * 32 - before;
+    for (uint32_t w = first; w < end; w += 2) {
         const uint32_t word = w + (lane >> 5), page = word * 32 + (lane & 31);
-        const bool free = word < word1 && page < p.pages && !(bits[word] >> (lane & 31) & 1);
+        const bool free = word < end && page < p.pages && !(bits[word] >> (lane & 31) & 1);
         const uint64_t all = __ballot(free);
         if (free) p.free_pages[place + __popcll(all & ((1ull << lane) - 1))] = (int32_t)page;
         place += __popcll(all);
     }
-    return place;
+    finish_list(p, used);
 }
 
-__global__ __launch_bounds__(256) void paged_release_clear_kernel(uint32_t *bits, uint32_t words) {
-    for (uint32_t w = blockIdx.x * 256 + threadIdx.x; w < words; w += gridDim.x * 256) bits[w] = 0;
+__global__ __launch_bounds__(256) void paged_release_clear_kernel(u32x4 *used, uint32_t quads) {
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < quads; i += gridDim.x * 256) used[i] = u32x4{0, 0, 0, 0};
 }
 __global__ __launch_bounds__(256) void paged_release_mark_kernel(const ReleaseDev p) {
-    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < p.entries; e += (uint64_t)gridDim.x * 256) {
-        const int32_t page = kept_entry(p, e);
+    const uint32_t across = (p.max_pages + 255) / 256;         // workgroups of a row
+    for (uint64_t i = blockIdx.x; i < (uint64_t)p.requests * across; i += gridDim.x) {
+        const uint32_t r = (uint32_t)(i / across), j = (uint32_t)(i - (uint64_t)r * across) * 256 + threadIdx.x;
+        if (j >= p.max_pages) continue;
+        const uint64_t e = (uint64_t)r * p.max_pages + j;
+        const int32_t page = kept_entry(p, r, j, e);
         p.table_out[e] = page;
-        if (page >= 0) atomicOr(p.bits + (page >> 5), 1u << (page & 31));
+        if (page >= 0) p.used[page] = 1;
     }
 }
-// A workgroup lists the free pages of 64 words after counting those in use before them.
-constexpr uint32_t LIST_WORDS = 64;
-__global__ __launch_bounds__(256) void paged_release_list_kernel(const ReleaseDev p) {
-    __shared__ uint32_t counted[4][2];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t word0 = blockIdx.x * LIST_WORDS, word1 = min(word0 + LIST_WORDS, p.words);
-    uint32_t before = 0, all = 0;          // pages in use
-    for (uint32_t w = threadIdx.x; w < p.words; w += 256) {
-        const uint32_t n = __popc(p.bits[w]);
-        all += n;
-        if (w < word0) before += n;
+// `share` pages (whole 1024) for each workgroup.
+constexpr uint32_t LIST_WAVES = 16;
+__global__ __launch_bounds__(LIST_WAVES * 64) void paged_release_list_kernel(const ReleaseDev p) {
+    __shared__ uint32_t sums[LIST_WAVES];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t first = blockIdx.x * p.share, mine = first + wave * (p.share / LIST_WAVES);         // of the workgroup, of the wavefront
+    const u32x4 *const used = reinterpret_cast<const u32x4 *>(p.used);
+    const uint32_t quads = (p.pages + 255) / 256 * 16;
+    auto count = [&](uint32_t from, uint32_t to, uint32_t id, uint32_t step) __attribute__((always_inline)) {
+        uint32_t n = 0;
+        for (uint32_t i = from + id; i < to; i += 4 * step) {
+            u32x4 v[4];                                        // on their way together
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) v[k] = used[min(i + k * step, quads - 1)];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (i + k * step < to) n += __popc(v[k][0]) + __popc(v[k][1]) + __popc(v[k][2]) + __popc(v[k][3]);
+        }
+        return n;
+    };
+    const uint32_t ahead = count(first / 16, min(mine / 16, quads), lane, 64);     // of the wavefronts before, in this workgroup's share
+    const uint32_t before = sum_over_all<LIST_WAVES>(count(0, first / 16, threadIdx.x, LIST_WAVES * 64), sums);
+    const uint32_t all = before + sum_over_all<LIST_WAVES>(count(first / 16, quads, threadIdx.x, LIST_WAVES * 64), sums);
+    uint32_t place = mine - before - last_lane(running_sum(ahead));
+    for (uint32_t page0 = mine; page0 < min(mine + p.share / LIST_WAVES, p.pages); page0 += 64) {
+        const bool free = page0 + lane < p.pages && !p.used[page0 + lane];
+        const uint64_t them = __ballot(free);
+        if (free) p.free_pages[place + __popcll(them & ((1ull << lane) - 1))] = (int32_t)(page0 + lane);
+        place += __popcll(them);
     }
-    before = last_lane(running_sum(before));
-    all = last_lane(running_sum(all));
-    if (lane == 0) { counted[wave][0] = before; counted[wave][1] = all; }
-    __syncthreads();
-    before = counted[0][0] + counted[1][0] + counted[2][0] + counted[3][0];
-    all = counted[0][1] + counted[1][1] + counted[2][1] + counted[3][1];
-    // the wavefront's quarter of the words
-    uint32_t place = word0 * 32 - before;
-    const uint32_t mine = min(word0 + wave * (LIST_WORDS / 4), word1), end = min(mine + LIST_WORDS / 4, word1);
-    for (uint32_t w = word0; w < mine; ++w) place += 32 - __popc(p.bits[w]);
-    list_free(p, p.bits, mine, end, place);
-    const uint32_t free = p.pages - all;
-    for (uint64_t i = free + (uint64_t)blockIdx.x * 256 + threadIdx.x; i < p.pages; i += (uint64_t)gridDim.x * 256) p.free_pages[i] = -1;
-    if (blockIdx.x == 0 && threadIdx.x == 0) { p.counts[0] = (int32_t)free; p.counts[1] = (int32_t)all; }
+    finish_list(p, all);
 }
 
-size_t paged_release_workspace_bytes(uint32_t, uint32_t, uint32_t pages) { return ((size_t)pages + 31) / 32 * 4; }
+static bool small_release(uint32_t requests, uint32_t max_pages, uint32_t pages) { return (uint64_t)requests * max_pages <= SMALL_TABLE && pages <= SMALL_POOL; }
+size_t paged_release_workspace_bytes(uint32_t requests, uint32_t max_pages, uint32_t pages) { return small_release(requests, max_pages, pages) ? 0 : ((size_t)pages + 255) / 256 * 256; }
 
 int paged_release(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, uint32_t window, uint32_t sinks, uint32_t pages,
                   int32_t *table_out, int32_t *free_pages, int32_t *counts, void *workspace, hipStream_t st) {
-    ReleaseDev p{page_table, lengths, table_out, free_pages, counts, (uint32_t *)workspace, (uint64_t)requests * max_pages, requests, max_pages, page_size, window, sinks, pages, (pages + 31) / 32};
-    hipLaunchKernelGGL(paged_release_clear_kernel, dim3(std::min((p.words + 255) / 256, 1024u)), dim3(256), 0, st, p.bits, p.words);
+    ReleaseDev p{page_table, lengths, table_out, free_pages, counts, (uint8_t *)workspace, requests, max_pages, page_size, window, sinks, pages, 0};
+    if (small_release(requests, max_pages, pages)) {
+        const uint32_t blocks = std::min(std::max(std::max(requests * max_pages, pages) / 8192, 1u), 32u);
+        hipLaunchKernelGGL(paged_release_small_kernel, dim3(blocks), dim3(1024), (pages + 31) / 32 * 4, st, p);
+        return check_launch("paged_release_small_kernel");
+    }
+    const uint32_t quads = (uint32_t)(((uint64_t)pages + 255) / 256 * 16);
+    hipLaunchKernelGGL(paged_release_clear_kernel, dim3(std::min((quads + 255) / 256, 1024u)), dim3(256), 0, st, (u32x4 *)workspace, quads);
     if (int rc = check_launch("paged_release_clear_kernel")) return rc;
-    if (p.entries) {
-        hipLaunchKernelGGL(paged_release_mark_kernel, dim3((uint32_t)std::min<uint64_t>((p.entries + 255) / 256, 4096)), dim3(256), 0, st, p);
+    if ((uint64_t)requests * max_pages) {
+        hipLaunchKernelGGL(paged_release_mark_kernel, dim3((uint32_t)std::min<uint64_t>((uint64_t)requests * ((max_pages + 255) / 256), 1u << 16)), dim3(256), 0, st, p);
         if (int rc = check_launch("paged_release_mark_kernel")) return rc;
     }
-    hipLaunchKernelGGL(paged_release_list_kernel, dim3((p.words + LIST_WORDS - 1) / LIST_WORDS), dim3(256), 0, st, p);
+    const uint32_t most = (uint32_t)std::min<uint64_t>(((uint64_t)pages + 2047) / 2048, 256);
+    p.share = (uint32_t)((((uint64_t)pages + most - 1) / most + 1023) / 1024 * 1024);
+    hipLaunchKernelGGL(paged_release_list_kernel, dim3((uint32_t)(((uint64_t)pages + p.share - 1) / p.share)), dim3(LIST_WAVES * 64), 0, st, p);
     return check_launch("paged_release_list_kernel");
 }
 

@@ -165,8 +165,10 @@ def copy_paged_pages(caches: Sequence[Tensor], sources: Tensor, targets: Tensor)
     """Page sources[i] to page targets[i] in every one of the caches, in place: the keys and the values of all layers, of one shape and dtype.
     Pairs in which either is no page are left out.  All are moved at once: a target may be named once, and is not a source."""
     name = "ttnn.experimental.copy_paged_pages"
-    handles = _handles(name, **{f"caches[{i}]": t for i, t in enumerate(caches)})
-    _m().paged_copy(handles, *_handles(name, sources=sources, targets=targets), name)
+    for t in caches:
+        if not isinstance(t, Tensor) or t._t is None:
+            raise RuntimeError(f"{name}: caches must be ttnn.Tensors that have not been deallocated")
+    _m().paged_copy([t._t for t in caches], *_handles(name, sources=sources, targets=targets), name)
 
 
 def release_paged_pages(page_table: Tensor, lengths: Tensor, *, page_size: int, num_pages: int, window: Optional[int] = None, sinks: int = 0) -> Tuple[Tensor, Tensor, Tensor]:
