@@ -114,6 +114,14 @@ def test_long_contexts_are_cut_and_joined(oracle, device, dtype):
     sinks_case(oracle, device, cached=[6100], new=[290], heads=2, kv_heads=1, head_dim=64, page_size=128, dtype=dtype, calls=2, window=1500, sinks=50)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "bfloat8_b"])
+@pytest.mark.parametrize("head_dim,page_size", [(64, 64), (256, 32)])
+def test_more_pieces_than_workgroups(oracle, device, dtype, head_dim, page_size):
+    """Whole prompts: workgroups ask for further pieces, the second call finds the counter as the first one found it."""
+    kv_heads = 8 if head_dim == 64 else 4
+    sinks_case(oracle, device, cached=[0, 500], new=[1290, 1270], heads=4 * kv_heads, kv_heads=kv_heads, head_dim=head_dim, page_size=page_size, dtype=dtype, calls=2, window=60, sinks=20)
+
+
 @pytest.mark.parametrize("new", [1, 200])
 def test_sinks_without_a_window_or_within_it(device, new):
     """All tokens are seen: bit for bit the attention without a window; and without sinks, that with the window alone."""

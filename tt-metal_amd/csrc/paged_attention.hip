@@ -63,6 +63,7 @@ struct AttentionDev {
 };
 
 constexpr uint32_t COUNTERS = 4096;        // at most 2 `target` slots, each could be a unit's first
+constexpr uint32_t NEXT_PIECE = COUNTERS - 1;          // pieces that workgroups of the kernel for many rows have asked for
 constexpr float LAZY = 8.f;                // how far (log2) a score may pass the running maximum
 
 // Operands go from LDS through a ring of this many, so that a product finds its own in registers.  Four took 537 us where two take 527 (two prompts of
@@ -829,7 +830,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
     using S = TileShape<D, PACKED>;
     constexpr int WAVES = S::WAVES, THREADS = WAVES * 64, ROWS = WAVES * 32, NB = S::NB, SLABS = D / 16, DB = D / 32, SINKS = WITH_SINKS ? NB : 0;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[6 * S::HALF];                // keys, then values, three buffers each
-    __shared__ uint32_t flag;
+    __shared__ uint32_t flag, queue;
     const int lane = threadIdx.x & 63, c = lane & 31, kh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool second = WAVES == 8 && wave >= 4;                // the half that runs a phase behind
@@ -837,9 +838,26 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
     const Plan plan = make_plan<ROWS, NB, SINKS>(p);
     const uint32_t out_width = p.heads * D;
 
-    for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
+    // The first piece is the workgroup's own, others are those that come next when it is done: units see different numbers of tokens.  Whoever asks
+    // last, all ask once too often, leaves the counter at zero.
+    uint32_t ticket = 0;
+    auto take_ticket = [&]() __attribute__((always_inline)) {
+        if (plan.pieces > gridDim.x && threadIdx.x == 0) {
+            ticket = __hip_atomic_fetch_add(p.counters + NEXT_PIECE, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (ticket == plan.pieces - 1) __hip_atomic_store(p.counters + NEXT_PIECE, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    };
+    auto next_piece = [&]() __attribute__((always_inline)) {
+        if (plan.pieces <= gridDim.x) return 0xffffffffu;
+        if (threadIdx.x == 0) queue = gridDim.x + ticket;
+        __syncthreads();
+        const uint32_t next = __builtin_amdgcn_readfirstlane(queue);
+        __syncthreads();
+        return next;
+    };
+    for (uint32_t index = blockIdx.x; index < plan.pieces; index = next_piece()) {
         Piece pc;
-        if (!piece_at<ROWS, SINKS>(p, plan, index, pc)) continue;
+        if (!piece_at<ROWS, SINKS>(p, plan, index, pc)) { take_ticket(); continue; }
         const bool idle = (uint32_t)wave * 32 >= pc.rows;       // a wavefront without rows only moves keys and values
         uint32_t row_token, head;
         Rows(pc.token0, p.group).at(pc.row0 + min((uint32_t)(wave * 32 + c), pc.rows - 1), row_token, head);
@@ -1191,6 +1209,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
             }
         }
 
+        take_ticket();
         l = sum_over_halves(l);
         if (pc.parts > 1) {
             constexpr uint32_t PART = (DB * 4 + 1) * 1024, SLOT = WAVES * PART;        // of a wavefront, of a workgroup
