@@ -58,6 +58,26 @@ template <uint32_t ROWS> __device__ __forceinline__ bool position_of(const Rotat
     return true;
 }
 
+// Sum over the lanes of a token, in each of them: lanes 2 ROWS apart and pairs in TILE layout, neighbours in rows.  By DPP and lane swaps: LDS permutes take 4 us
+// of 49 for the prompts below.
+template <int CTRL> __device__ __forceinline__ float add_lane(float v) { return v + __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, false)); }
+template <uint32_t LANES> __device__ __forceinline__ float sum_over_token(float v, int tiled) {
+    v = add_lane<0xb1>(v);                                     // the other of a pair
+    if (tiled) {
+        if (LANES == 16) v = add_lane<0x128>(v);               // 8 lanes on, of 16
+        if (LANES >= 8) {
+            const auto o = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+        }
+        const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(o[0]) + __uint_as_float(o[1]);
+    }
+    v = add_lane<0x4e>(v);                                     // the other pair of four
+    if (LANES >= 8) v = add_lane<0x141>(v);                    // mirrored in 8: the other four
+    if (LANES == 16) v = add_lane<0x140>(v);                   // mirrored in 16: the other eight
+    return v;
+}
+
 // Codes of 8 of a face row's 16 numbers, lowest element in the lowest byte.  Ordinary rows (shared exponent 32 <= E < 255, or nothing but zeros):
 // floor(v + 1/2) = trunc(fma(|x|, 2^(133 - E), 1/2 - 2^-25)) with v = |x| 2^(133 - E), for every 24-bit mantissa; 2^7 becomes 2^7 - 1, zeros lose their sign.
 __device__ __forceinline__ uint32_t ordinary_codes(const float *x, float scale) {
@@ -84,7 +104,7 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t shared, 
 // of the rotation are in one lane: chunks k and k + R/16, or neighbours.  Angles are computed once for all heads of the item.
 template <int SLABS, bool NORM, bool INTERLEAVED, bool PACKED>
 __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
-    constexpr uint32_t D = SLABS * 32, PAIRS = SLABS * 2, LANES = PAIRS <= 4 ? 4 : PAIRS <= 8 ? 8 : 16, ROWS = 64 / LANES;
+    constexpr uint32_t D = SLABS * 32, PAIRS = SLABS * 2, LANES = PAIRS <= 4 ? 4 : PAIRS <= 8 ? 8 : 16, ROWS = 64 / LANES, AHEAD = 3;
     __shared__ uint32_t tops[4][ROWS * 4 * SLABS];             // largest exponent of every chunk
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = p.tiled ? lane >> 1 & (ROWS - 1) : lane / LANES, q = p.tiled ? lane / (2 * ROWS) * 2 + (lane & 1) : lane % LANES;
@@ -107,7 +127,7 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
         const uint8_t *from[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) from[h] = p.rows + row_bytes_at(t, p.width, p.column[kind] + head0 * D + at[h] * 8, p.tiled);
-        u32x4 raw[2][2];
+        u32x4 raw[AHEAD][2];
         auto load = [&](u32x4 (&v)[2]) __attribute__((always_inline)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -115,8 +135,9 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
                 from[h] += head_step;
             }
         };
-        load(raw[0]);
-        if (head0 + 1 < head1) load(raw[1]);
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+            if (head0 + i < head1) load(raw[i]);
         const float *const norm = NORM && kind != VALUES ? p.norm[kind] : nullptr;
         float weight[2][8], cosine[8], sine[8];
         if (NORM && norm && mine) {
@@ -185,9 +206,7 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sum = fmaf(x[h][i], x[h][i], sum);
-                sum += __shfl_xor(sum, 1);
-#pragma unroll
-                for (uint32_t d = 2; d < LANES; d <<= 1) sum += __shfl_xor(sum, p.tiled ? d * ROWS : d);
+                sum = sum_over_token<LANES>(sum, p.tiled);
                 const float by = rsqrtf(sum * (1.f / D) + p.epsilon);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -249,8 +268,9 @@ __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
         };
         for (uint32_t head = head0; head < head1; ++head) {
             const u32x4 v[2] = {raw[0][0], raw[0][1]};
-            raw[0][0] = raw[1][0]; raw[0][1] = raw[1][1];
-            if (head + 2 < head1) load(raw[1]);
+#pragma unroll
+            for (uint32_t i = 0; i + 1 < AHEAD; ++i) { raw[i][0] = raw[i + 1][0]; raw[i][1] = raw[i + 1][1]; }
+            if (head + AHEAD < head1) load(raw[AHEAD - 1]);
             work(v);
 #pragma unroll
             for (int h = 0; h < 2; ++h) { to[h] += to_step; exponent[h] += to_step; }

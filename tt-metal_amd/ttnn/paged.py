@@ -26,12 +26,14 @@ from .core import to_device
 
 
 def _handles(operation_name, **tensors):
+    handles = []
     for name, t in tensors.items():
         if not isinstance(t, Tensor):
             raise RuntimeError(f"{operation_name}: {name} must be a ttnn.Tensor")
-        if not t.is_allocated():
+        if t._t is None:
             raise RuntimeError(f"{operation_name}: {name} has been deallocated")
-    return [t._t for t in tensors.values()]
+        handles.append(t._t)
+    return handles
 
 
 def _count(operation_name, name, value, least=0):
