@@ -296,6 +296,9 @@ __device__ __forceinline__ bool last_of(const AttentionDev &p, const Piece &x, u
     return true;
 }
 
+// ones for the bits below x: none for x <= 0, all from 32 on
+__device__ __forceinline__ uint32_t bits_below(int x) { return x >= 32 ? 0xffffffffu : (1u << max(x, 0)) - 1; }
+
 // LDS that lanes of one wavefront hand each other: the hardware keeps a wavefront's accesses in order, this keeps the compiler to it.
 __device__ __forceinline__ void lanes_in_order() {
     __builtin_amdgcn_wave_barrier();
@@ -850,9 +853,9 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
     auto next_piece = [&]() __attribute__((always_inline)) {
         if (plan.pieces <= gridDim.x) return 0xffffffffu;
         if (threadIdx.x == 0) queue = gridDim.x + ticket;
-        __syncthreads();
+        end_phase();
         const uint32_t next = __builtin_amdgcn_readfirstlane(queue);
-        __syncthreads();
+        end_phase();
         return next;
     };
     for (uint32_t index = blockIdx.x; index < plan.pieces; index = next_piece()) {
@@ -862,6 +865,9 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         uint32_t row_token, head;
         Rows(pc.token0, p.group).at(pc.row0 + min((uint32_t)(wave * 32 + c), pc.rows - 1), row_token, head);
         head += pc.kv * p.group;
+        // the first pages are looked up ahead of the queries: keys and values wait for them
+        Blocks<1, S::ROW_BYTES, SINKS> blocks;
+        blocks.load(p, pc, pc.begin);
         bf16x8 q[SLABS];
 #pragma unroll
         for (int s = 0; s < SLABS; ++s) {
@@ -891,7 +897,6 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         auto uneven = [&](uint32_t step) { return !((token_of(step) >= unit_first_max || all_sinks(token_of(step))) && token_of(step) + NB * 32 - 1 < unit_pos_min); };
 
         // ---- keys and values: memory -> registers -> LDS ------------------------------------------------------------------------------
-        Blocks<1, S::ROW_BYTES, SINKS> blocks;
         uint64_t keys_at[NB], values_at[NB];                    // of the step whose keys, and whose values, are asked for next
         uint32_t have = 0;                                      // which blocks of four steps, from the current one on, have pages: bit NB * step + block
         u32x4 kreg[S::EACH], vreg[S::EACH];
@@ -1049,7 +1054,6 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
         if (steps) {
             u32x4 k1[S::EACH];
             uint32_t e1[S::EACH];
-            refill(0);
             look_up(0, 0);
             load(p.keys, keys_at, kreg, kexp);
             load(p.values, keys_at, vreg, vexp);
@@ -1111,12 +1115,17 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                 // against constants: the tokens' numbers would be held in registers over all steps
                 const int from = (int)(first - token0) - kh * 4, to = (int)(pos - token0) - kh * 4, sinks = (int)(in_table(p.sinks) - token0) - kh * 4;
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t seen = ~bits_below(from - b * 32);
+                    if (SINKS) seen |= bits_below(sinks - b * 32);
+                    const uint32_t hidden = have >> b & 1 ? ~(seen & bits_below(to + 1 - b * 32)) : 0xffffffffu;
+                    if (!__ballot(hidden != 0)) continue;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int t = b * 32 + (i >> 2) * 8 + (i & 3);
-                        if ((t < from && (!SINKS || t >= sinks)) || t > to || !(have >> b & 1)) s[b][i] = -INFINITY;
+                        const uint32_t gone = (uint32_t)__builtin_amdgcn_sbfe(hidden, (i >> 2) * 8 + (i & 3), 1);
+                        s[b][i] = __uint_as_float((gone & 0xff800000u) | (~gone & __float_as_uint(s[b][i])));      // -inf
                     }
+                }
             }
             float top = s[0][0];
 #pragma unroll
@@ -1264,7 +1273,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                 const auto w1 = __builtin_amdgcn_permlane32_swap(f32x2_to_bf16x2_rne(acc[d][i + 2] * by, acc[d][i + 3] * by), f32x2_to_bf16x2_rne(acc[d][i + 6] * by, acc[d][i + 7] * by), false, false);
                 if (stored) *reinterpret_cast<u32x4 *>(p.out + row_bytes_at(pc.q.start + row_token, out_width, head * D + d * 32 + f * 16 + kh * 8, p.tiled)) = u32x4{w0[0], w1[0], w0[1], w1[1]};
             }
-        __syncthreads();                                        // LDS is the next piece's
+        end_phase();                                            // LDS is the next piece's
     }
     if (p.zero_rows) clear_rows(p, D, plan.begin, plan.end);
 }
