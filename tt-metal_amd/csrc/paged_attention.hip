@@ -1116,9 +1116,9 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
                 const int from = (int)(first - token0) - kh * 4, to = (int)(pos - token0) - kh * 4, sinks = (int)(in_table(p.sinks) - token0) - kh * 4;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    uint32_t seen = ~bits_below(from - b * 32);
-                    if (SINKS) seen |= bits_below(sinks - b * 32);
-                    const uint32_t hidden = have >> b & 1 ? ~(seen & bits_below(to + 1 - b * 32)) : 0xffffffffu;
+                    uint32_t seen = ~bits_below(max(from, 0) - b * 32);
+                    if (SINKS) seen |= bits_below(max(sinks, 0) - b * 32);
+                    const uint32_t hidden = have >> b & 1 ? ~(seen & bits_below(min(to, 64) + 1 - b * 32)) : 0xffffffffu;
                     if (!__ballot(hidden != 0)) continue;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
