@@ -358,12 +358,13 @@ TTMI_API int ttmi_paged_rotate_write(const void *rows, int layout, uint32_t toke
 
 /* ---- pages that change hands ------------------------------------------------------------------------------------------------
  * ttmi_paged_fork: page tables of requests that go on from others, one launch.  Row i continues request parents[i], with its length
- * (a parent that is none, -1 among them: an empty row).  Full pages are shared: nobody writes into them any more.  The page begun, where
+ * (a parent that is none, -1 among them: an empty row).  Full pages are shared: nobody writes into them any more, unless a length goes back behind the
+ * fork, which is the caller's to rule out.  The page begun, where
  * page_size does not divide the length, stays with the first of a parent's continuations; every other one takes a page from free_pages, in the
  * order of the continuations, into which it is to be copied.  At most 4096 requests and 4096 continuations.
  *   page_table_out [children, max_pages], lengths_out [children]; neither may overlap the old ones.  -1 behind the length, and where free_pages ran out
  *   sources, targets [children]: the page begun and the page taken where continuation i has a copy to make, else -1
- *   counts         [2]: pages taken, and pages that were wanted and not there
+ *   counts         [2]: entries taken from free_pages, and pages that were wanted when it was at its end
  *
  * ttmi_paged_copy: page sources[i] to page targets[i], i < pairs, in each of `count` caches of one shape, e.g. the keys and values of all
  * layers; one launch for up to 128 of them.  `caches` is host memory.  Pairs that name no page on either side are left out.  Pairs are moved at once: a
@@ -374,7 +375,8 @@ TTMI_API int ttmi_paged_rotate_write(const void *rows, int layout, uint32_t toke
  * entry names any more are listed.
  *   page_table_out as page_table (may be the same memory)
  *   free_pages     [pages]: the pages of [0, pages) that no entry kept names, ascending, then -1
- *   counts         [2]: pages free, pages in use
+ *   counts         [2]: pages free, pages in use.  The calls that take from the whole list count its entries: a step that takes more than are free
+ *                  has run out, and leaves rows without a page
  *   workspace      ttmi_paged_release_workspace_bytes() bytes, 256-byte aligned (0 bytes: none); nothing is kept in it between calls */
 TTMI_API int ttmi_paged_fork(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size,
                       const int32_t *parents, uint32_t children, const int32_t *free_pages, uint32_t free_count, int32_t *page_table_out,

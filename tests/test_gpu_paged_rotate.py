@@ -246,6 +246,29 @@ def test_keys_are_those_of_rotate_heads(device, rotary_dim):
     assert torch.equal(keys, alone) and torch.equal(values.contiguous().view(torch.int16), odd.view(torch.int16))
 
 
+@pytest.mark.parametrize("layout", ["TILE_LAYOUT", "ROW_MAJOR_LAYOUT"])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -90, 2.0 ** -100, 2.0 ** -122, 2.0 ** -133, 2.0 ** 127])
+def test_numbers_at_the_ends_of_the_range_are_packed_as_elsewhere(device, layout, scale):
+    """Without frequencies and norms a BFLOAT8_B cache holds the bits that write_paged_cache gives: tiny and huge numbers, infinities and NaN, rows of zeros, among ordinary ones."""
+    import ttnn
+
+    torch.manual_seed(10)
+    E, tokens, kv_heads, dim = ttnn.experimental, 45, 2, 96
+    wide = kv_heads * dim
+    rows = (torch.randn(tokens, 3 * wide) * scale).bfloat16()
+    rows[3], rows[4, ::2], rows[5:9] = 0.0, -0.0, torch.randn(4, 3 * wide).bfloat16()
+    rows[10, ::37], rows[11, ::41], rows[12, 5::16] = float("inf"), float("nan"), -float("inf")
+    given, slots = activations(device, rows, layout), integers(device, torch.randperm(96)[:tokens])
+    caches = [[E.allocate_paged_cache(3, kv_heads, 32, dim, dtype=ttnn.bfloat8_b, device=device) for _ in range(2)] for _ in range(2)]
+    for pair in caches:
+        for cache in pair:
+            cache._buf.zero_()
+    E.write_paged_cache(given, *caches[0], slots, key_column=wide, value_column=2 * wide)
+    E.rotate_write_paged_cache(given, *caches[1], slots, integers(device, [7]), integers(device, [0, tokens]), floats(device, frequencies_of(0)), num_heads=kv_heads, key_column=wide, value_column=2 * wide)
+    for a, b in zip(*caches):
+        assert torch.equal(a._buf, b._buf)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "bfloat8_b"])
 def test_a_graph_replayed_on_other_lengths_and_streams(device, dtype):
     import ttnn

@@ -92,7 +92,7 @@ RELEASE = dict(page_table=SOMEWHERE, lengths=SOMEWHERE, requests=3, max_pages=4,
 
 
 @pytest.mark.parametrize("change", [dict(page_size=0), dict(page_size=48), dict(pages=0), dict(pages=1 << 31), dict(page_table=None), dict(lengths=None), dict(page_table_out=None),
-                                    dict(free_pages=None), dict(counts=None), dict(lengths=SOMEWHERE + 2)])
+                                    dict(free_pages=None), dict(counts=None), dict(lengths=SOMEWHERE + 2), dict(page_table_out=SOMEWHERE + 4)])
 def test_releases_refuse(capi, change):
     refused(capi, "ttmi_paged_release", RELEASE, change)
 

@@ -413,6 +413,8 @@ int ttmi_paged_release(const int32_t *page_table, const int32_t *lengths, uint32
     const void *all[] = {page_table, lengths, page_table_out, free_pages, counts};
     for (const void *p : all)
         if (misaligned(p, 4)) return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: pointers must be 4-byte aligned");
+    if (page_table_out != page_table && overlap(page_table, (uint64_t)requests * max_pages * 4, page_table_out, (uint64_t)requests * max_pages * 4))
+        return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: the new table overlaps the old one without being the same memory");
     if (const size_t bytes = ttmi_paged_release_workspace_bytes(requests, max_pages, pages); bytes && (!workspace || misaligned(workspace, 256) || workspace_bytes < bytes))
         return fail(TTMI_ERR_INVALID_ARGUMENT, "paged release: workspace of %zu bytes, 256-byte aligned, expected", bytes);
     return paged_release(page_table, lengths, requests, max_pages, page_size, window, sinks, pages, page_table_out, free_pages, counts, workspace, (hipStream_t)stream);

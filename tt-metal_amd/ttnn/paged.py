@@ -154,9 +154,10 @@ def rotate_write_paged_cache(input_tensor: Tensor, key_cache: Tensor, value_cach
 def fork_paged_tables(page_table: Tensor, lengths: Tensor, parents: Tensor, free_pages: Tensor, *, page_size: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """Requests that go on from others (several answers to one prompt, beams): (page_table, lengths, sources, targets, counts).
 
-    Row i of the new table continues request parents[i] (0xffffffff: an empty row) with its length.  They share its full pages.  The
+    Row i of the new table continues request parents[i] (0xffffffff: an empty row) with its length.  They share its full pages, which nobody writes into as
+    long as no length goes back behind the fork.  The
     page that it is about to go on in stays with the first of them; each other one takes a page from free_pages, in order, and
-    copy_paged_pages(caches, sources, targets) has to copy it before the next write.  counts = (pages taken, pages wanted and not there); a row that
+    copy_paged_pages(caches, sources, targets) has to copy it before the next write.  counts = (entries taken, pages wanted at the end of the list); a row that
     got none has no page there.  The arguments do not change.  At most 4096 requests and as many continuations.  The five share an allocation."""
     name = "ttnn.experimental.fork_paged_tables"
     handles = _handles(name, page_table=page_table, lengths=lengths, parents=parents, free_pages=free_pages)
@@ -178,7 +179,7 @@ def release_paged_pages(page_table: Tensor, lengths: Tensor, *, page_size: int, 
 
     Entries behind a request's length become 0xffffffff (a request that is over has length 0), and, with a window, those that no later token will see: before
     the window of the token at `length`, without one of the first `sinks` tokens.  Pages may be shared.  free_pages: those of the num_pages that no entry names, ascending, then
-    0xffffffff; counts = (free, in use).  The arguments do not change.  The three share an allocation."""
+    0xffffffff; counts = (free, in use): a later step that takes more than `free` entries of the list has run out of pages.  The arguments do not change.  The three share an allocation."""
     name = "ttnn.experimental.release_paged_pages"
     handles = _handles(name, page_table=page_table, lengths=lengths)
     return tuple(_wrap(t) for t in _m().paged_release(*handles, _count(name, "page_size", page_size), _count(name, "num_pages", num_pages, 1),
