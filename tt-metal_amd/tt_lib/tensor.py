@@ -153,10 +153,7 @@ class Tensor:
     """
 
     def __init__(self, data, data_type: Optional[DataType] = None, device: Optional[Device] = None,
-                 layout: Optional[Layout] = None, mem_config: Optional[MemoryConfig] = None, *, _raw=None, _handle=None):
-        if _handle is not None:
-            self._t = _handle
-            return
+                 layout: Optional[Layout] = None, mem_config: Optional[MemoryConfig] = None, *, _raw=None):
         if _raw is not None:      # (torch buffer, logical shape, padded shape, dtype, layout, device): memory that torch already holds
             buf, shape, padded, dtype, lay, dev = _raw
             storage = buf.contiguous().reshape(-1).view(torch.uint8)
@@ -304,7 +301,9 @@ def _bytes_of(handle) -> "torch.Tensor":
 
 
 def _wrap(handle) -> Tensor:
-    return Tensor(None, _handle=handle)
+    tensor = Tensor.__new__(Tensor)                    # past the constructor and its arguments: every operation makes one or more
+    tensor._t = handle
+    return tensor
 
 
 def _as_torch(host_handle) -> "torch.Tensor":

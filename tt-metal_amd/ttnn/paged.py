@@ -37,6 +37,8 @@ def _handles(operation_name, **tensors):
 
 
 def _count(operation_name, name, value, least=0):
+    if type(value) is int and least <= value <= 0x7FFFFFFF:
+        return value
     if int(value) != value or not least <= value <= 0x7FFFFFFF:
         raise RuntimeError(f"{operation_name}: {name} must be a whole number of at least {least}, got {value}")
     return int(value)
