@@ -137,7 +137,7 @@ def test_windows(device, window, sinks):
     release_case(device, table, [3 * n for n in lengths], 96, 90, window, sinks)
 
 
-@pytest.mark.parametrize("requests,width,pages", [(1, 5000, 9000), (900, 70, 70000), (4096, 20, 300000), (5000, 3, 20000)])
+@pytest.mark.parametrize("requests,width,pages", [(1, 5000, 9000), (900, 70, 70000), (4096, 20, 300000), (5000, 3, 20000), (256, 64, 65536), (255, 64, 65535), (256, 64, 65537), (257, 64, 60000), (1024, 16, 3000), (4096, 4, 65536)])
 def test_large_tables(device, requests, width, pages):
     g = torch.Generator().manual_seed(3)
     table = torch.randint(0, pages, (requests, width), generator=g)

@@ -346,7 +346,7 @@ __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_
 // The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.  Nothing should spill in that loop: a reload
 // from scratch memory waits for all loads before it, the next block's among them (two row tiles of 128 elements in BFLOAT8_B with 66 spilled
 // registers: 185 us instead of 83).  Hence the scheduling barriers between products of different operands.  One and two row tiles have no spilled
-// registers; five row tiles of 64 elements do not fit: 46 are spilled for BFLOAT8_B, 14 for bf16, and some are reloaded in every block.
+// registers; five row tiles of 64 elements do not fit: 46 are spilled for BFLOAT8_B, 12 for bf16, and some are reloaded in every block.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int D, bool PACKED> struct StreamShape {
     static constexpr int SLABS = D / 32, TILE_BYTES = PACKED ? 1088 : 2048;
@@ -803,8 +803,13 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 //            prompts of 5000 tokens (BFLOAT8_B cache, window 4096, 32 heads on 8 key heads), 106 instead of 94 for 512 tokens behind 7680
 //            (bf16).  With the wavefronts in their matrix phase not preferred (s_setprio): 560 and 97.  The additions of the
 //            weights belong into the matrix phase, although v_dot2_f32_bf16 takes 20 cycles beside products: 566 and 102 us in the other
-//   rate     those prompts: 527 us = 0.82 PFLOP/s of what the masks leave (the largest of several cards' rates: 590 us and 0.73 on another, and
-//            on any under a profiler), a large product reaches 1.22; matrix cores busy 44 % of the time,
+//   pieces   workgroups ask a counter for what comes next: units of a prompt see different numbers of tokens, and every 256th piece for each came to 524 us
+//            for those prompts where it is 460 now (527 in the figures above and below, which are of the time before).  Bits of a mask are taken as signed
+//            fields and select -inf, two instructions for a score: with comparisons a step with a boundary in it took 7700 cycles, now 5700, others 4300.
+//            The last barrier of a piece waits for LDS only, not for the stores.  A piece of 38 blocks (a window of 1024, 100 sinks, BFLOAT8_B) is 90,000 cycles of steps and
+//            20,000 around them: 8200 until the first keys lie in LDS, 2000 for the second half's last phase, 5000 for stores
+//   rate     those prompts: 460 us = 0.94 PFLOP/s of what the masks leave (a tenth more or less from card to card, and more
+//            under a profiler), a large product reaches 1.22; with 527 us, the matrix cores busy 44 % of the time,
 //            vector ALU 66 %: an instruction takes it 8 cycles while the matrix cores work, and a step of 32 products (1024 cycles) has 300
 //            of them for each wavefront, 140 for expanding block floats, 32 exponentials among the rest
 //   LDS      three buffers each for keys and values.  In vector phase i the keys of step i + 2 and the values of step i + 1 are written, read by

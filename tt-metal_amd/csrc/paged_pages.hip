@@ -18,7 +18,8 @@ __device__ __forceinline__ uint32_t tokens_of(int32_t length) { return (uint32_t
 // but for the page begun, j = n / S where S does not divide n: the first of a parent's continuations keeps it, each other one takes the next
 // page from the list, in the order of the continuations, into which the one begun is to be copied.
 // As the tables of a step are made: every workgroup finds the first continuations (LDS, atomic minimum) and makes the prefix sum for itself,
-// then the entries are dealt out.  Bound by the launch and three loads that wait for each other (parents, lengths, the page begun).
+// then the entries are dealt out.  Bound by the launch and three loads that wait for each other (parents, lengths, the page begun): 3.4 us for
+// four continuations, 4.5 for 96.
 // ---------------------------------------------------------------------------------------------------------------------------------
 struct ForkDev {
     const int32_t *table, *lengths, *parents, *free_pages;
@@ -103,7 +104,8 @@ int paged_fork(const int32_t *page_table, const int32_t *lengths, uint32_t reque
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Copies of whole pages, the same ones in every cache of a model.  A page is contiguous: a workgroup moves 16 KB of one.
+// Copies of whole pages, the same ones in every cache of a model.  A page is contiguous: a workgroup moves 16 KB of one, four loads of a lane on their way
+// together.  12 pages of 128 KB in each of 16 caches, among 96 pairs of which the others copy nothing: 50 MB in 11.2 us with the launch = 4.5 TB/s.
 // ---------------------------------------------------------------------------------------------------------------------------------
 constexpr uint32_t CACHES = 128;           // of one launch: their addresses are kernel arguments
 struct CopyDev {
@@ -156,9 +158,11 @@ int paged_copy(void *const *caches, uint32_t count, const PagedCache &c, const i
 //   j S < n   and   (W = 0, or j S + S > n + 1 - W: the next token sees a token of it, or j S < K)
 // and is -1 elsewhere.  The pages that no entry kept names, in ascending order, are the new list of free pages: the place of a free page in
 // it is the number of free ones before it.
-// Small tables and pools: one launch, in which every workgroup marks the pages in use in its own LDS from the whole table and writes its share of
-// the results.  Large ones: a byte of memory for every page, which is cleared, set by plain stores (all of them store the same, so nothing has to be
-// atomic: 1000 requests with a common page would wait for each other), and counted by every workgroup up to its share.
+// A byte for every page says whether it is in use.  Small tables and pools: one launch, in which every workgroup marks them in its own LDS from the whole
+// table and writes its share of the results.  Large ones: in memory, cleared, set by plain stores (all of them store the same, so nothing has to be
+// atomic: 1000 requests with common pages would wait for each other, 22 us instead of 5), and counted by every workgroup up to its share.
+// 32 rows of 64 entries, 4096 pages: 4.4 us, the launch, two passes and their barriers; 1000 rows of 512, 300,000 pages: 2.2 + 5.1 + 8.0 us, the last of them for reading
+// the bytes once per workgroup (256 lanes with one load at a time 24 us, 1024 with four 8).
 // ---------------------------------------------------------------------------------------------------------------------------------
 struct ReleaseDev {
     const int32_t *table, *lengths;
@@ -166,13 +170,19 @@ struct ReleaseDev {
     uint8_t *used;                         // one byte for every page, whole 256 of them
     uint32_t requests, max_pages, page_size, window, sinks, pages, share;
 };
-// Entry j of request r, if it is kept and a page, else -1.
-__device__ __forceinline__ int32_t kept_entry(const ReleaseDev &p, uint32_t r, uint32_t j, uint64_t e) {
-    const uint64_t n = tokens_of(p.lengths[r]), first = (uint64_t)j * p.page_size;
-    const bool kept = first < n && (!p.window || first + p.page_size + p.window > n + 1 || first < p.sinks);
-    const int32_t page = p.table[e];
-    return kept && (uint32_t)page < p.pages ? page : -1;
-}
+// Which entries of a request's row are kept: j < held and (j >= from or j < sinks).  j S + S > n + 1 - W is j >= floor((n + 1 - W) / S).
+struct Kept {
+    uint32_t held, from, sinks;
+    __device__ __forceinline__ Kept(uint32_t held, uint32_t from, uint32_t sinks) : held(held), from(from), sinks(sinks) {}
+    __device__ __forceinline__ Kept(const ReleaseDev &p, int32_t length) {
+        const uint32_t n = tokens_of(length);
+        auto pages = [&](uint32_t tokens) { return tokens / p.page_size + (tokens % p.page_size != 0); };
+        held = pages(n);
+        from = p.window && n + 1 > p.window ? (n + 1 - p.window) / p.page_size : 0;
+        sinks = pages(p.sinks);
+    }
+    __device__ __forceinline__ int32_t operator()(const ReleaseDev &p, uint32_t j, int32_t page) const { return j < held && (j >= from || j < sinks) && (uint32_t)page < p.pages ? page : -1; }
+};
 // sum of v over the workgroup
 template <uint32_t WAVES> __device__ __forceinline__ uint32_t sum_over_all(uint32_t v, uint32_t *lds) {
     v = last_lane(running_sum(v));
@@ -184,46 +194,69 @@ template <uint32_t WAVES> __device__ __forceinline__ uint32_t sum_over_all(uint3
     for (uint32_t w = 0; w < WAVES; ++w) v += lds[w];
     return v;
 }
-__device__ __forceinline__ void finish_list(const ReleaseDev &p, uint32_t used) {
-    const uint32_t free = p.pages - used;
+// The free pages of [first, first + share), share a multiple of 1024, go to their places in the list, in a workgroup of LIST_WAVES wavefronts: what is in use before them is counted, and
+// in the parts of the wavefronts before this one.
+constexpr uint32_t LIST_WAVES = 16;
+__device__ __forceinline__ void list_free(const ReleaseDev &p, const uint8_t *used, uint32_t first, uint32_t share, uint32_t *sums) {
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t mine = first + wave * (share / LIST_WAVES), quads = (p.pages + 255) / 256 * 16;
+    auto count = [&](uint32_t from, uint32_t to, uint32_t id, uint32_t step) __attribute__((always_inline)) {
+        uint32_t n = 0;
+        for (uint32_t i = from + id; i < to; i += 4 * step) {
+            u32x4 v[4];                                        // on their way together
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) v[k] = reinterpret_cast<const u32x4 *>(used)[min(i + k * step, quads - 1)];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (i + k * step < to) n += __popc(v[k][0]) + __popc(v[k][1]) + __popc(v[k][2]) + __popc(v[k][3]);
+        }
+        return n;
+    };
+    const uint32_t ahead = count(first / 16, min(mine / 16, quads), lane, 64);
+    const uint32_t before = sum_over_all<LIST_WAVES>(count(0, first / 16, threadIdx.x, LIST_WAVES * 64), sums);
+    const uint32_t all = before + sum_over_all<LIST_WAVES>(count(first / 16, quads, threadIdx.x, LIST_WAVES * 64), sums), free = p.pages - all;
+    uint32_t place = mine - before - last_lane(running_sum(ahead));
+    for (uint32_t page0 = mine; page0 < min(mine + share / LIST_WAVES, p.pages); page0 += 64) {
+        const bool is_free = page0 + lane < p.pages && !used[page0 + lane];
+        const uint64_t them = __ballot(is_free);
+        if (is_free) p.free_pages[place + __popcll(them & ((1ull << lane) - 1))] = (int32_t)(page0 + lane);
+        place += __popcll(them);
+    }
     for (uint64_t i = (uint64_t)free + blockIdx.x * blockDim.x + threadIdx.x; i < p.pages; i += (uint64_t)gridDim.x * blockDim.x) p.free_pages[i] = -1;
-    if (blockIdx.x == 0 && threadIdx.x == 0) { p.counts[0] = (int32_t)free; p.counts[1] = (int32_t)used; }
+    if (blockIdx.x == 0 && threadIdx.x == 0) { p.counts[0] = (int32_t)free; p.counts[1] = (int32_t)all; }
 }
 
-constexpr uint32_t SMALL_TABLE = 1u << 16, SMALL_POOL = 1u << 18;                 // entries, pages
-__global__ __launch_bounds__(1024) void paged_release_small_kernel(const ReleaseDev p) {
-    extern __shared__ uint32_t bits[];                         // of the pages in use
+__global__ __launch_bounds__(LIST_WAVES * 64) void paged_release_small_kernel(const ReleaseDev p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t in_use[];               // a byte for every page, whole 256 of them
+    __shared__ uint32_t sums[LIST_WAVES];
+    const uint32_t quads = (p.pages + 255) / 256 * 16;
+    for (uint32_t i = threadIdx.x; i < quads; i += LIST_WAVES * 64) reinterpret_cast<u32x4 *>(in_use)[i] = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    // A wavefront has every 64th group of four rows: its lanes find what is kept of 16 groups, one row each, then the entries of four rows are on their way together
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t words = (p.pages + 31) / 32, entries = p.requests * p.max_pages;
-    for (uint32_t w = threadIdx.x; w < words; w += 1024) bits[w] = 0;
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < entries; e += 1024) {
-        const uint32_t r = e / p.max_pages;
-        const int32_t page = kept_entry(p, r, e - r * p.max_pages, e);
-        if (page >= 0) atomicOr(bits + (page >> 5), 1u << (page & 31));
-        if (e / 1024 % gridDim.x == blockIdx.x) p.table_out[e] = page;
+    constexpr uint32_t ROWS = 4, STRIDE = LIST_WAVES * ROWS;
+    for (uint32_t base = wave * ROWS; base < p.requests; base += 16 * STRIDE) {
+        const Kept row(p, p.lengths[min(base + lane / ROWS * STRIDE + lane % ROWS, p.requests - 1)]);
+        for (uint32_t g = 0; g < 16 && base + g * STRIDE < p.requests; ++g) {
+            const uint32_t r0 = base + g * STRIDE;
+            const bool mine = r0 / ROWS % gridDim.x == blockIdx.x;
+            for (uint32_t j = lane; j < p.max_pages; j += 64) {
+                int32_t page[ROWS];
+#pragma unroll
+                for (uint32_t k = 0; k < ROWS; ++k) page[k] = p.table[min(r0 + k, p.requests - 1) * p.max_pages + j];
+#pragma unroll
+                for (uint32_t k = 0; k < ROWS; ++k) {
+                    if (r0 + k >= p.requests) break;
+                    const Kept of{(uint32_t)__builtin_amdgcn_readlane(row.held, g * ROWS + k), (uint32_t)__builtin_amdgcn_readlane(row.from, g * ROWS + k), (uint32_t)__builtin_amdgcn_readlane(row.sinks, g * ROWS + k)};
+                    const int32_t kept = of(p, j, page[k]);
+                    if (kept >= 0) in_use[kept] = 1;
+                    if (mine) p.table_out[(r0 + k) * p.max_pages + j] = kept;
+                }
+            }
+        }
     }
     __syncthreads();
-    // words of this wavefront: its part of the workgroup's share, in whole pairs
-    const uint32_t all_waves = gridDim.x * 16, each = ((words + all_waves - 1) / all_waves + 1) / 2 * 2;
-    const uint32_t first = min((blockIdx.x * 16 + wave) * each, words), end = min(first + each, words);
-    uint32_t before = 0, used = 0;
-    for (uint32_t w = lane; w < words; w += 64) {              // each wavefront for itself: LDS, and no barrier
-        const uint32_t n = __popc(bits[w]);
-        used += n;
-        if (w < first) before += n;
-    }
-    before = last_lane(running_sum(before));
-    used = last_lane(running_sum(used));
-    uint32_t place = first * 32 - before;
-    for (uint32_t w = first; w < end; w += 2) {
-        const uint32_t word = w + (lane >> 5), page = word * 32 + (lane & 31);
-        const bool free = word < end && page < p.pages && !(bits[word] >> (lane & 31) & 1);
-        const uint64_t all = __ballot(free);
-        if (free) p.free_pages[place + __popcll(all & ((1ull << lane) - 1))] = (int32_t)page;
-        place += __popcll(all);
-    }
-    finish_list(p, used);
+    list_free(p, in_use, blockIdx.x * p.share, p.share, sums);
 }
 
 __global__ __launch_bounds__(256) void paged_release_clear_kernel(u32x4 *used, uint32_t quads) {
@@ -235,53 +268,30 @@ __global__ __launch_bounds__(256) void paged_release_mark_kernel(const ReleaseDe
         const uint32_t r = (uint32_t)(i / across), j = (uint32_t)(i - (uint64_t)r * across) * 256 + threadIdx.x;
         if (j >= p.max_pages) continue;
         const uint64_t e = (uint64_t)r * p.max_pages + j;
-        const int32_t page = kept_entry(p, r, j, e);
+        const int32_t page = Kept(p, p.lengths[r])(p, j, p.table[e]);
         p.table_out[e] = page;
         if (page >= 0) p.used[page] = 1;
     }
 }
-// `share` pages (whole 1024) for each workgroup.
-constexpr uint32_t LIST_WAVES = 16;
 __global__ __launch_bounds__(LIST_WAVES * 64) void paged_release_list_kernel(const ReleaseDev p) {
     __shared__ uint32_t sums[LIST_WAVES];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t first = blockIdx.x * p.share, mine = first + wave * (p.share / LIST_WAVES);         // of the workgroup, of the wavefront
-    const u32x4 *const used = reinterpret_cast<const u32x4 *>(p.used);
-    const uint32_t quads = (p.pages + 255) / 256 * 16;
-    auto count = [&](uint32_t from, uint32_t to, uint32_t id, uint32_t step) __attribute__((always_inline)) {
-        uint32_t n = 0;
-        for (uint32_t i = from + id; i < to; i += 4 * step) {
-            u32x4 v[4];                                        // on their way together
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) v[k] = used[min(i + k * step, quads - 1)];
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-                if (i + k * step < to) n += __popc(v[k][0]) + __popc(v[k][1]) + __popc(v[k][2]) + __popc(v[k][3]);
-        }
-        return n;
-    };
-    const uint32_t ahead = count(first / 16, min(mine / 16, quads), lane, 64);     // of the wavefronts before, in this workgroup's share
-    const uint32_t before = sum_over_all<LIST_WAVES>(count(0, first / 16, threadIdx.x, LIST_WAVES * 64), sums);
-    const uint32_t all = before + sum_over_all<LIST_WAVES>(count(first / 16, quads, threadIdx.x, LIST_WAVES * 64), sums);
-    uint32_t place = mine - before - last_lane(running_sum(ahead));
-    for (uint32_t page0 = mine; page0 < min(mine + p.share / LIST_WAVES, p.pages); page0 += 64) {
-        const bool free = page0 + lane < p.pages && !p.used[page0 + lane];
-        const uint64_t them = __ballot(free);
-        if (free) p.free_pages[place + __popcll(them & ((1ull << lane) - 1))] = (int32_t)(page0 + lane);
-        place += __popcll(them);
-    }
-    finish_list(p, all);
+    list_free(p, p.used, blockIdx.x * p.share, p.share, sums);
 }
 
+// Entries and pages up to which one launch, whose every workgroup reads the whole table, is the shorter way (three launches): 32 x 64 entries, 4096 pages 4.6 us (7.9);
+// 128 x 64, 65,536 pages 6.8 (9.1); 256 x 64, 65,536 pages 8.8 (9.2), 256 x 128 11.1 (9.1), replayed from a graph; called one by one, each launch costs the host 2.8.
+constexpr uint32_t SMALL_TABLE = 1u << 14, SMALL_POOL = 1u << 16;
 static bool small_release(uint32_t requests, uint32_t max_pages, uint32_t pages) { return (uint64_t)requests * max_pages <= SMALL_TABLE && pages <= SMALL_POOL; }
 size_t paged_release_workspace_bytes(uint32_t requests, uint32_t max_pages, uint32_t pages) { return small_release(requests, max_pages, pages) ? 0 : ((size_t)pages + 255) / 256 * 256; }
 
 int paged_release(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, uint32_t window, uint32_t sinks, uint32_t pages,
                   int32_t *table_out, int32_t *free_pages, int32_t *counts, void *workspace, hipStream_t st) {
     ReleaseDev p{page_table, lengths, table_out, free_pages, counts, (uint8_t *)workspace, requests, max_pages, page_size, window, sinks, pages, 0};
+    const uint32_t most = (uint32_t)std::min<uint64_t>(((uint64_t)pages + 2047) / 2048, 256);     // workgroups that list
+    p.share = (uint32_t)((((uint64_t)pages + most - 1) / most + 1023) / 1024 * 1024);
+    const dim3 blocks((uint32_t)(((uint64_t)pages + p.share - 1) / p.share));
     if (small_release(requests, max_pages, pages)) {
-        const uint32_t blocks = std::min(std::max(std::max(requests * max_pages, pages) / 8192, 1u), 32u);
-        hipLaunchKernelGGL(paged_release_small_kernel, dim3(blocks), dim3(1024), (pages + 31) / 32 * 4, st, p);
+        hipLaunchKernelGGL(paged_release_small_kernel, blocks, dim3(LIST_WAVES * 64), ((size_t)pages + 255) / 256 * 256, st, p);
         return check_launch("paged_release_small_kernel");
     }
     const uint32_t quads = (uint32_t)(((uint64_t)pages + 255) / 256 * 16);
@@ -291,9 +301,7 @@ int paged_release(const int32_t *page_table, const int32_t *lengths, uint32_t re
         hipLaunchKernelGGL(paged_release_mark_kernel, dim3((uint32_t)std::min<uint64_t>((uint64_t)requests * ((max_pages + 255) / 256), 1u << 16)), dim3(256), 0, st, p);
         if (int rc = check_launch("paged_release_mark_kernel")) return rc;
     }
-    const uint32_t most = (uint32_t)std::min<uint64_t>(((uint64_t)pages + 2047) / 2048, 256);
-    p.share = (uint32_t)((((uint64_t)pages + most - 1) / most + 1023) / 1024 * 1024);
-    hipLaunchKernelGGL(paged_release_list_kernel, dim3((uint32_t)(((uint64_t)pages + p.share - 1) / p.share)), dim3(LIST_WAVES * 64), 0, st, p);
+    hipLaunchKernelGGL(paged_release_list_kernel, blocks, dim3(LIST_WAVES * 64), 0, st, p);
     return check_launch("paged_release_list_kernel");
 }
 

@@ -4,7 +4,12 @@
 //   y_d = x_d w_d / sqrt(mean(x^2) + epsilon)
 // and, of its first R elements, the pairs (a, b) = (y_i, y_(i + R/2)), or neighbours (y_2i, y_(2i+1)), i < R/2,
 //   (a, b) -> m (a cos(p f_i) - b sin(p f_i), b cos(p f_i) + a sin(p f_i))
-// in fp32 and rounded once: to bf16, or, for keys of a BFLOAT8_B cache, from fp32 to its codes.
+// in fp32 and rounded once: to bf16, or, for keys of a BFLOAT8_B cache, from fp32 to its codes (by way of bf16 they would be off by up to 2^-9 more).
+//
+// Bound by memory, for few tokens by the launch and three loads that wait for each other (row starts, length, slot): 32 tokens of 32 heads of 128 elements
+// 4.6 us with the launch, with keys, values and norms 5.0.  8206 tokens of 71 heads of 64 elements: 33 us = 4.6 TB/s; 8183 tokens of 32 + 8 + 8 heads of 128 elements with
+// norms into BFLOAT8_B: 42 us = 4.4 TB/s, 43 without norms into bf16 (4.6 TB/s; a large copy moves 5.1).  The vector ALU is busy for 67 % of the former: 135 instructions
+// for two chunks of a head, 75 for each head's share of requests and angles.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -101,7 +106,9 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t shared, 
 }
 
 // An item is up to `each` heads of a few tokens.  LANES lanes share a token; each has two chunks of 8 elements of a head, chosen such that partners
-// of the rotation are in one lane: chunks k and k + R/16, or neighbours.  Angles are computed once for all heads of the item.
+// of the rotation are in one lane: chunks k and k + R/16, or neighbours.  Angles are computed once for all heads of the item.  Registers decide: with all
+// heads of a token in four lanes, 256 of them, the 8183 tokens took 136 us; now 82 to 120, four to six wavefronts per SIMD.  AHEAD heads are on their
+// way: two 58.7 us (with the read-back of the caches), three 57.7, four 59.4.
 template <int SLABS, bool NORM, bool INTERLEAVED, bool PACKED>
 __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
     constexpr uint32_t D = SLABS * 32, PAIRS = SLABS * 2, LANES = PAIRS <= 4 ? 4 : PAIRS <= 8 ? 8 : 16, ROWS = 64 / LANES, AHEAD = 3;
@@ -308,6 +315,8 @@ int paged_rotate(const PagedRotationArgs &x, hipStream_t st) {
     p.epsilon = x.epsilon; p.magnitude = x.magnitude;
     const uint32_t rows = x.head_dim == 64 ? 16 : x.head_dim == 256 ? 4 : 8;       // tokens of an item
     const uint64_t bands = ((uint64_t)p.out_rows + rows - 1) / rows, heads = (uint64_t)p.heads[0] + p.heads[1] + p.heads[2];
+    // Heads of an item: many share the angles, few leave enough items to fill the chip.  8183 tokens (with the read-back) and 8206: one 82 and 44 us,
+    // two 66 and 35, three 62 and 33, four 59 and 33, eight 60 and 35, sixteen 59 and 38
     p.each = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(bands * heads / 8192, 1), 4);
     for (int k = 0; k < 3; ++k) p.blocks[k] = (p.heads[k] + p.each - 1) / p.each;
     p.items = bands * (p.blocks[0] + p.blocks[1] + p.blocks[2]);
