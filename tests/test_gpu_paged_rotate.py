@@ -301,6 +301,60 @@ def test_a_graph_replayed_on_other_lengths_and_streams(device, dtype):
             assert torch.equal(a._buf.view(torch.uint8), b._buf.view(torch.uint8))
 
 
+def test_rows_past_4_gib(device):
+    """Activations whose bytes are more than 32 bits count, in both layouts; the last rows are turned as the first ones."""
+    from ttmi import capi
+
+    torch.manual_seed(11)
+    tokens, width, dim = 270016, 8192, 128
+    rows = torch.zeros(tokens, width, dtype=torch.bfloat16, device="cuda")
+    few = torch.randn(64, dim).bfloat16()
+    f = frequencies_of(dim)
+    put = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    cached, starts, freq = put([5, 900]), put([0, tokens - 40, tokens]), f.cuda()
+    want, bound = model.rotate(few, [(0, 5 + tokens - 64 + i) if i < 24 else (1, 900 + i - 24) for i in range(64)], 1, dim, f)
+    bound = model.as_bfloat16(want, bound)
+    for layout in (capi.ROW_MAJOR, capi.TILE):
+        rows.zero_()
+        if layout == capi.ROW_MAJOR:
+            rows[-64:, 8064:] = few.cuda()
+        else:
+            rows.view(-1, width // 32, 2, 2, 16, 16)[-2:, 252:].copy_(few.view(2, 2, 16, 4, 2, 16).permute(0, 3, 1, 4, 2, 5))
+        out = torch.empty(tokens, dim, dtype=torch.bfloat16, device="cuda")
+        capi.check(capi.lib().ttmi_rotate_heads(rows.data_ptr(), layout, tokens, width, 8064, 1, dim, cached.data_ptr(), starts.data_ptr(), 2, freq.data_ptr(), dim, 0, None, 0.0, 1.0, out.data_ptr(),
+                                                capi._stream()))
+        got = out[-64:].cpu() if layout == capi.ROW_MAJOR else out.view(-1, 4, 2, 2, 16, 16)[-2:].cpu().permute(0, 2, 4, 1, 3, 5).reshape(64, dim)
+        check(got.view(want.shape), want, bound)
+        assert not out[:1000].any()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "bfloat8_b"])
+def test_pages_past_4_gib(device, dtype):
+    """Keys and values into the last pages of large caches, and attention over a window there behind sinks in the first ones: the bits of the same pages in small caches."""
+    import ttnn
+
+    torch.manual_seed(12)
+    E, kv_heads, dim, page_size, heads, tokens = ttnn.experimental, 8, 128, 128, 16, 40
+    many = 20000 if dtype == "bfloat16" else 36000
+    wide = (heads + 2 * kv_heads) * dim
+    rows = activations(device, torch.randn(300, wide).bfloat16(), "TILE_LAYOUT")
+    chunk = activations(device, torch.randn(tokens, wide).bfloat16(), "TILE_LAYOUT")
+    f = floats(device, frequencies_of(dim))
+    answers = []
+    for pages, table in [(3, [0, 1, 2]), (many, [1, many - 2, many - 1])]:
+        caches = [E.allocate_paged_cache(pages, kv_heads, page_size, dim, dtype=getattr(ttnn, dtype), device=device) for _ in range(2)]
+        made = []
+        for given, n, cached in ((rows, 300, 0), (chunk, tokens, 300)):
+            slots = integers(device, [table[p // page_size] * page_size + p % page_size for p in range(cached, cached + n)])
+            lengths = integers(device, [cached]), integers(device, [0, n])
+            queries = E.rotate_write_paged_cache(given, *caches, slots, *lengths, f, num_heads=heads, key_column=heads * dim, value_column=(heads + kv_heads) * dim)
+            made.append(E.attend_paged_cache(queries, *caches, integers(device, [table]), *lengths, num_heads=heads, window=64, sinks=4)._buf.cpu())
+        answers.append(made)
+        del caches
+    for a, b in zip(*answers):
+        assert torch.equal(a, b) and not torch.isnan(a.float()).any()
+
+
 # ---- frequencies, refusals of the host layer --------------------------------------------------------------------------------------------
 def test_frequencies(device):
     import math
