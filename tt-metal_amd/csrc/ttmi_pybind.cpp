@@ -78,6 +78,10 @@ void bind_tensor_layer(py::module_ &m) {
         .def_property_readonly("data_ptr", [](const host::Tensor &t) { return (uintptr_t)t.buffer.data; })
         .def_property_readonly("offset", [](const host::Tensor &t) { return t.buffer.offset; }, "bytes between the start of `storage` and the tensor")
         .def_property_readonly("storage", &owner_of, "the object that owns the memory (a flat torch.uint8 tensor)")
+        .def_property_readonly("memory", [](const host::Tensor &t) {
+            const bool shaped = t.layout == host::Layout::ROW_MAJOR && !host::is_block_float(t.dtype) && t.padded.size() != 1;
+            return py::make_tuple(owner_of(t), t.buffer.offset, t.buffer.nbytes, (int)t.dtype, shaped ? py::object(py::tuple(py::cast(t.padded))) : py::object(py::none()));
+        }, "(storage, offset, nbytes, dtype, shape, or None where the elements are in one dimension) in one call")
         .def("volume", &host::Tensor::volume);
 
     m.def("set_runtime",

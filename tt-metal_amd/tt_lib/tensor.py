@@ -201,13 +201,11 @@ class Tensor:
     @property
     def _buf(self):
         """The buffer as a torch tensor of the storage element type (dense ROW_MAJOR data in the padded shape, else flat)."""
-        t = self._t
-        dtype = t.dtype
-        elements = _bytes_of(t).view(_TORCH[dtype])
-        if t.layout == Layout.ROW_MAJOR and dtype not in _BFP:
-            shape = t.padded_shape
-            return elements if len(shape) == 1 else elements.view(shape)
-        return elements
+        storage, offset, nbytes, dtype, shape = self._t.memory
+        if storage.numel() != nbytes:
+            storage = storage.narrow(0, offset, nbytes)
+        elements = storage.view(_TORCH[dtype])
+        return elements if shape is None else elements.view(shape)
 
     @property
     def shape(self):
