@@ -25,15 +25,16 @@ from tt_lib.tensor import DataType, Device, Tensor, _m, _wrap
 from .core import to_device
 
 
+def _handle(operation_name, name, t):
+    if not isinstance(t, Tensor):
+        raise RuntimeError(f"{operation_name}: {name} must be a ttnn.Tensor")
+    if t._t is None:
+        raise RuntimeError(f"{operation_name}: {name} has been deallocated")
+    return t._t
+
+
 def _handles(operation_name, **tensors):
-    handles = []
-    for name, t in tensors.items():
-        if not isinstance(t, Tensor):
-            raise RuntimeError(f"{operation_name}: {name} must be a ttnn.Tensor")
-        if t._t is None:
-            raise RuntimeError(f"{operation_name}: {name} has been deallocated")
-        handles.append(t._t)
-    return handles
+    return [_handle(operation_name, name, t) for name, t in tensors.items()]
 
 
 def _count(operation_name, name, value, least=0):
@@ -119,10 +120,6 @@ def rotary_frequencies(rotary_dim: int, *, theta: float = 10000.0, factor: float
     return to_device(Tensor((frequencies * (stays + (1.0 - stays) / factor)).float(), None), device)
 
 
-def _optional(operation_name, **tensors):
-    return [None if t is None else _handles(operation_name, **{name: t})[0] for name, t in tensors.items()]
-
-
 def rotate_heads(input_tensor: Tensor, cached_lengths: Tensor, row_starts: Tensor, frequencies: Tensor, *, num_heads: int, head_dim: int, column: int = 0,
                  interleaved: bool = False, norm: Optional[Tensor] = None, epsilon: float = 1e-6, magnitude: float = 1.0) -> Tensor:
     """The heads of the step's tokens, turned by their positions: token i of a request's new ones is at cached_lengths + i.
@@ -136,7 +133,7 @@ def rotate_heads(input_tensor: Tensor, cached_lengths: Tensor, row_starts: Tenso
     name = "ttnn.experimental.rotate_heads"
     handles = _handles(name, input_tensor=input_tensor, cached_lengths=cached_lengths, row_starts=row_starts, frequencies=frequencies)
     return _wrap(_m().rotate_heads(*handles, _count(name, "num_heads", num_heads, 1), _count(name, "head_dim", head_dim, 1), _count(name, "column", column), bool(interleaved),
-                                   *_optional(name, norm=norm), float(epsilon), float(magnitude), name))
+                                   None if norm is None else _handle(name, "norm", norm), float(epsilon), float(magnitude), name))
 
 
 def rotate_write_paged_cache(input_tensor: Tensor, key_cache: Tensor, value_cache: Tensor, slots: Tensor, cached_lengths: Tensor, row_starts: Tensor, frequencies: Tensor, *,
@@ -149,8 +146,8 @@ def rotate_write_paged_cache(input_tensor: Tensor, key_cache: Tensor, value_cach
     handles = _handles(name, input_tensor=input_tensor, key_cache=key_cache, value_cache=value_cache, slots=slots, cached_lengths=cached_lengths, row_starts=row_starts,
                        frequencies=frequencies)
     return _wrap(_m().paged_rotate_write(*handles, _count(name, "num_heads", num_heads, 1), _count(name, "key_column", key_column), _count(name, "value_column", value_column),
-                                         _count(name, "query_column", query_column), bool(interleaved), *_optional(name, query_norm=query_norm, key_norm=key_norm), float(epsilon),
-                                         float(magnitude), name))
+                                         _count(name, "query_column", query_column), bool(interleaved), None if query_norm is None else _handle(name, "query_norm", query_norm),
+                                         None if key_norm is None else _handle(name, "key_norm", key_norm), float(epsilon), float(magnitude), name))
 
 
 def fork_paged_tables(page_table: Tensor, lengths: Tensor, parents: Tensor, free_pages: Tensor, *, page_size: int) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
@@ -170,10 +167,7 @@ def copy_paged_pages(caches: Sequence[Tensor], sources: Tensor, targets: Tensor)
     """Page sources[i] to page targets[i] in every one of the caches, in place: the keys and the values of all layers, of one shape and dtype.
     Pairs in which either is no page are left out.  All are moved at once: a target may be named once, and is not a source."""
     name = "ttnn.experimental.copy_paged_pages"
-    for t in caches:
-        if not isinstance(t, Tensor) or t._t is None:
-            raise RuntimeError(f"{name}: caches must be ttnn.Tensors that have not been deallocated")
-    _m().paged_copy([t._t for t in caches], *_handles(name, sources=sources, targets=targets), name)
+    _m().paged_copy([_handle(name, "a cache", t) for t in caches], *_handles(name, sources=sources, targets=targets), name)
 
 
 def release_paged_pages(page_table: Tensor, lengths: Tensor, *, page_size: int, num_pages: int, window: Optional[int] = None, sinks: int = 0) -> Tuple[Tensor, Tensor, Tensor]:
