@@ -277,7 +277,8 @@ TTMI_API int ttmi_eltwise_bf16(int op, const void *a, const void *b, float scala
  * table[p / page_size] * page_size + p % page_size, with the request's row of the page table.  Lengths, tables, slots and row
  * starts are int32 in device memory and never come to the host, so a step can be captured into a graph and replayed on other
  * lengths.  Whatever they hold, no call reads or writes outside the buffers whose sizes it is told: page numbers outside
- * [0, pages), -1 among them, mean that there is no page, negative lengths count as 0.  Block floats in a cache are read as finite
+ * [0, pages), -1 among them, mean that there is no page, negative lengths count as 0.  They may not change while a call that reads them runs:
+ * that call's results may then be anything, those of later calls are right.  Block floats in a cache are read as finite
  * numbers: an exponent byte of 255 (infinities or NaN were written) as 254, one below 7 (all 16 numbers under 2^-119) as 7.  No
  * counterpart on the reference's block-float path.
  *

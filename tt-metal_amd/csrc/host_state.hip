@@ -18,7 +18,7 @@ namespace ttmi {
 // geometrically, so they add up to less than the live buffer).
 // ---------------------------------------------------------------------------------------------------------
 namespace {
-struct Buffer { void *ptr = nullptr; size_t bytes = 0; uint64_t generation = 0; };
+struct Buffer { void *ptr = nullptr; size_t bytes = 0; uint64_t generation = 0; uint32_t uses = 0; };
 struct Key {
     int kind, device; hipStream_t stream;
     bool operator<(const Key &o) const {
@@ -42,7 +42,7 @@ size_t scratch_grown_size(size_t have, size_t need) {
     return (want + 255) & ~(size_t)255;
 }
 
-int scratch_get(int kind, hipStream_t stream, size_t bytes, void **ptr, bool *fresh, size_t *capacity) {
+int scratch_get(int kind, hipStream_t stream, size_t bytes, void **ptr, bool *fresh, size_t *capacity, uint32_t *uses) {
     int dev = 0;
     if (int rc = check_hip(hipGetDevice(&dev), "hipGetDevice")) return rc;
     std::lock_guard<std::mutex> lock(g_guard);
@@ -63,8 +63,11 @@ int scratch_get(int kind, hipStream_t stream, size_t bytes, void **ptr, bool *fr
         *fresh = true;
     }
     if (b.generation != g_generation[kind]) { b.generation = g_generation[kind]; *fresh = true; }
+    if (*fresh) b.uses = 0;
     *ptr = b.ptr;
     if (capacity) *capacity = b.bytes;
+    if (uses) *uses = b.uses;
+    ++b.uses;
     return TTMI_OK;
 }
 
@@ -224,6 +227,17 @@ int ttmi_release_scratch(size_t *freed_bytes) {
 #ifdef TTMI_TEST_HOOKS
 // Test entry point: how many allocations (device scratch, the pinned error word) the library has made in this process.
 __attribute__((visibility("default"))) uint64_t ttmi_test_allocations(void) { return g_allocations.load(); }
+
+// Test entry point: the library's buffer for this purpose and stream on the current device, and how often it was handed out; null and 0 without one.
+__attribute__((visibility("default"))) void ttmi_test_scratch(int kind, void *stream, void **ptr, size_t *bytes, uint32_t *uses) {
+    int dev = 0;
+    *ptr = nullptr; *bytes = 0; *uses = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return;
+    std::lock_guard<std::mutex> lock(g_guard);
+    const auto it = g_live.find(Key{kind, dev, (hipStream_t)stream});
+    if (it == g_live.end()) return;
+    *ptr = it->second.ptr; *bytes = it->second.bytes; *uses = it->second.uses;
+}
 
 // Test entry point: the size a library buffer of `have` bytes grows to when `need` bytes are asked for.
 __attribute__((visibility("default"))) size_t ttmi_test_scratch_grown_size(size_t have, size_t need) { return scratch_grown_size(have, need); }

@@ -56,6 +56,7 @@ struct AttentionDev {
     uint32_t least_rows, most_rows;        // requests of that many rows per key head are this launch's
     uint32_t target, slots;                // about how many pieces the step is cut into; partial results that fit
     uint32_t *counters;                    // pieces of a unit that are done, by the unit's first slot; all zero between launches
+    uint32_t *spare;                       // counters of the stream's next call, which this one clears; null in a workspace of the caller's
     uint8_t *partial;
     float scale;                           // |scale| log2(e)
     uint32_t flip;                         // sign bits of the queries, for a negative scale
@@ -71,6 +72,13 @@ constexpr float LAZY = 8.f;                // how far (log2) a score may pass th
 constexpr int AHEAD = 2;
 // Reads of LDS and products stay in the order in which they are written; everything else may pass.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x476); }
+
+// Calls that use the library's buffer take two sets of counters in turn, and each clears the other's set.  A call leaves its own at zero, unless its lengths
+// changed while it ran: workgroups that cut different steps into pieces wait for counts that never come together.  What such a call leaves is cleared by
+// the next one, which counts in the other set.
+template <uint32_t THREADS> __device__ __forceinline__ void clear_spare(const AttentionDev &p) {
+    if (p.spare && blockIdx.x < COUNTERS / THREADS) p.spare[blockIdx.x * THREADS + threadIdx.x] = 0;
+}
 
 // ---- the work of a step ---------------------------------------------------------------------------------------------------------
 struct Request { uint32_t start, added, cached; };
@@ -790,6 +798,7 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
         }
         __syncthreads();                                        // LDS is the next piece's
     }
+    clear_spare<256>(p);
     if (p.zero_rows) clear_rows(p, D, plan.begin, plan.end);
 }
 
@@ -1283,6 +1292,7 @@ __global__ __launch_bounds__((TileShape<D, PACKED>::WAVES * 64)) void paged_atte
             }
         end_phase();                                            // LDS is the next piece's
     }
+    clear_spare<THREADS>(p);
     if (p.zero_rows) clear_rows(p, D, plan.begin, plan.end);
 }
 
@@ -1297,6 +1307,7 @@ struct Route {
     uint32_t target = 256, grid = 256;     // of the kernel for few rows: pieces to aim at, workgroups that are resident at once
     size_t slot_bytes = 0, slots = 0;
 };
+static_assert(2 * 512 <= NEXT_PIECE && 2 * TILE_TARGET <= NEXT_PIECE, "slots of either kernel are counted below the pieces asked for");
 Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCache &c) {
     Route r;
     const uint32_t group = heads / c.kv_heads;
@@ -1324,7 +1335,7 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
     // Two workgroups fit a CU up to 128 elements.  One piece for each CU fills the memory pipes of bf16, and is less to join than two: 32 users x 2000
     // tokens, 128 elements 44 us (two: 50), 64 elements 24 (30).  The expansion of block floats takes both: 8 users x 26000 tokens 102 us (one: 136).
     // The second workgroup stays for steps of more units than CUs: 64 users x 500 tokens 25 us (28 without it).
-    if (c.head_dim <= 128) r.grid = 512;
+    if (c.head_dim <= 128) r.grid = 512;       // at most: two slots each have counters
     if (c.head_dim <= 128 && packed) r.target = 512;
     if (r.mt) {
         const size_t cols = packed ? (c.head_dim + 63) / 64 * 4 : c.head_dim / 16;
@@ -1336,8 +1347,8 @@ Route route_of(uint32_t tokens, uint32_t requests, uint32_t heads, const PagedCa
 }
 
 __global__ void clear_counters_kernel(uint32_t *counters) { counters[blockIdx.x * 256 + threadIdx.x] = 0; }
-int clear_counters(void *at, hipStream_t st) {
-    hipLaunchKernelGGL(clear_counters_kernel, dim3(COUNTERS / 256), dim3(256), 0, st, (uint32_t *)at);
+int clear_counters(void *at, uint32_t count, hipStream_t st) {
+    hipLaunchKernelGGL(clear_counters_kernel, dim3(count / 256), dim3(256), 0, st, (uint32_t *)at);
     return check_launch("clear_counters_kernel");
 }
 
@@ -1385,22 +1396,27 @@ int paged_attention(const PagedAttentionArgs &x, hipStream_t st) {
     const Route route = route_of(p.tokens, p.requests, p.heads, c);
     // Without requests there are no pieces, hence no counters and no partial results: rows are cleared, and that needs no memory.
     uint8_t *memory = p.requests ? (uint8_t *)x.workspace : nullptr;
-    static std::mutex fresh_guard;         // another thread's launch on this stream stays behind the clearing of a new buffer
+    // held up to the last launch: what another thread launches on this stream stays behind the clearing of a new buffer, and has the other counters
+    static std::mutex scratch_guard;
+    std::unique_lock<std::mutex> launches(scratch_guard, std::defer_lock);
     if (memory) {
-        if (int rc = clear_counters(memory, st)) return rc;
-    } else if (p.requests) {
-        const size_t bytes = COUNTERS * 4 + route.slots;
-        std::lock_guard<std::mutex> lock(fresh_guard);
-        // what is recorded may be replayed on any stream beside any other call: the buffer of the stream that is captured is not its own
-        if (stream_is_capturing(st)) return fail(TTMI_ERR_UNSUPPORTED, "paged attention: a captured call takes no scratch of the library's, bring a workspace of %zu bytes", bytes);
-        bool fresh = false;
-        if (int rc = scratch_get(SCRATCH_PAGED, st, bytes, (void **)&memory, &fresh)) return rc;
-        if (fresh)
-            if (int rc = clear_counters(memory, st)) return rc;
-    }
-    if (memory) {
+        if (int rc = clear_counters(memory, COUNTERS, st)) return rc;
         p.counters = (uint32_t *)memory;
         p.partial = memory + COUNTERS * 4;
+    } else if (p.requests) {
+        const size_t bytes = 2 * COUNTERS * 4 + route.slots;
+        launches.lock();
+        // what is recorded may be replayed on any stream beside any other call: the buffer of the stream that is captured is not its own
+        if (stream_is_capturing(st))
+            return fail(TTMI_ERR_UNSUPPORTED, "paged attention: a captured call takes no scratch of the library's, bring a workspace of %zu bytes", COUNTERS * 4 + route.slots);
+        bool fresh = false;
+        uint32_t uses = 0;
+        if (int rc = scratch_get(SCRATCH_PAGED, st, bytes, (void **)&memory, &fresh, nullptr, &uses)) return rc;
+        if (fresh)
+            if (int rc = clear_counters(memory, 2 * COUNTERS, st)) return rc;
+        p.counters = (uint32_t *)memory + uses % 2 * COUNTERS;
+        p.spare = (uint32_t *)memory + (uses + 1) % 2 * COUNTERS;
+        p.partial = memory + 2 * COUNTERS * 4;
     }
     p.zero_rows = 1;
     if (route.mt) {

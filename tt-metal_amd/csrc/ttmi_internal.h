@@ -20,8 +20,9 @@ int check_hip(hipError_t e, const char *what);
 enum { SCRATCH_SLOTS = 0, SCRATCH_EXPANDED = 1, SCRATCH_PAGED = 2, SCRATCH_KINDS = 3 };
 // The library's own device buffer of at least `bytes` for this purpose on the current device and this stream.  *fresh is
 // set when the contents are undefined (a new buffer, or one invalidated since): the caller initialises ALL of it on `stream`
-// (*capacity bytes: buffers grow geometrically, so a later, larger request may be served without being fresh).
-int scratch_get(int kind, hipStream_t stream, size_t bytes, void **ptr, bool *fresh, size_t *capacity = nullptr);
+// (*capacity bytes: buffers grow geometrically, so a later, larger request may be served without being fresh).  *uses: how often it was
+// handed out before, 0 for a fresh one.
+int scratch_get(int kind, hipStream_t stream, size_t bytes, void **ptr, bool *fresh, size_t *capacity = nullptr, uint32_t *uses = nullptr);
 bool scratch_held(int kind, hipStream_t stream, size_t bytes);      // scratch_get would allocate nothing
 bool stream_is_capturing(hipStream_t stream);
 // Held from scratch_get(SCRATCH_EXPANDED) to the last launch that reads the buffer: one launch of a call fills it, the next ones
