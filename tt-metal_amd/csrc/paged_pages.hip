@@ -232,7 +232,7 @@ __global__ __launch_bounds__(LIST_WAVES * 64) void paged_release_small_kernel(co
     const uint32_t quads = (p.pages + 255) / 256 * 16;
     for (uint32_t i = threadIdx.x; i < quads; i += LIST_WAVES * 64) reinterpret_cast<u32x4 *>(in_use)[i] = u32x4{0, 0, 0, 0};
     __syncthreads();
-    // A wavefront has every 64th group of four rows: its lanes find what is kept of 16 groups, one row each, then the entries of four rows are on their way together
+    // A wavefront has every 16th group of four rows, 64 rows apart: its lanes find what is kept of 16 groups, one row each, then the entries of four rows are on their way together
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr uint32_t ROWS = 4, STRIDE = LIST_WAVES * ROWS;
     for (uint32_t base = wave * ROWS; base < p.requests; base += 16 * STRIDE) {
@@ -278,10 +278,15 @@ __global__ __launch_bounds__(LIST_WAVES * 64) void paged_release_list_kernel(con
     list_free(p, p.used, blockIdx.x * p.share, p.share, sums);
 }
 
-// Entries and pages up to which one launch, whose every workgroup reads the whole table, is the shorter way (three launches): 32 x 64 entries, 4096 pages 4.6 us (7.9);
-// 128 x 64, 65,536 pages 6.8 (9.1); 256 x 64, 65,536 pages 8.8 (9.2), 256 x 128 11.1 (9.1), replayed from a graph; called one by one, each launch costs the host 2.8.
-constexpr uint32_t SMALL_TABLE = 1u << 14, SMALL_POOL = 1u << 16;
-static bool small_release(uint32_t requests, uint32_t max_pages, uint32_t pages) { return (uint64_t)requests * max_pages <= SMALL_TABLE && pages <= SMALL_POOL; }
+// Where one launch, whose every workgroup reads the whole table, is the shorter way (three launches).  Entries and pages: 32 x 64 entries, 4096 pages 4.6 us (7.6);
+// 128 x 64, 65,536 pages 6.8 (9.1); 256 x 64, 65,536 pages 8.8 (9.1), 256 x 128 11.1 (9.1).  Turns of a wavefront, each four rows of 64 entries one after the other, whatever
+// the entries: 4096 pages, 4 x 512 (8 turns) 8.0 (7.7), 32 x 512 (8) 8.7 (7.7), 4 x 1024 (16) 12.1 (7.7), 1024 x 16 (16) 21.9 (7.8), 1 x 4096 (64) 16.2 (7.8), 1 x 16384 (256) 54
+// (7.6).  All replayed from a graph; called one by one, three launches cost the host 13.6 us, so that 8.7 are the shorter way there.
+constexpr uint32_t SMALL_TABLE = 1u << 14, SMALL_POOL = 1u << 16, SMALL_TURNS = 8;
+static bool small_release(uint32_t requests, uint32_t max_pages, uint32_t pages) {
+    const uint64_t turns = ((uint64_t)requests + 63) / 64 * std::max<uint64_t>(((uint64_t)max_pages + 63) / 64, 1);
+    return (uint64_t)requests * max_pages <= SMALL_TABLE && pages <= SMALL_POOL && turns <= SMALL_TURNS;
+}
 size_t paged_release_workspace_bytes(uint32_t requests, uint32_t max_pages, uint32_t pages) { return small_release(requests, max_pages, pages) ? 0 : ((size_t)pages + 255) / 256 * 256; }
 
 int paged_release(const int32_t *page_table, const int32_t *lengths, uint32_t requests, uint32_t max_pages, uint32_t page_size, uint32_t window, uint32_t sinks, uint32_t pages,
