@@ -62,3 +62,49 @@ def test_counters_that_an_earlier_call_left(test_library, heads, kv_heads, dim, 
         for _ in range(3):
             assert torch.equal(attend(), expected)
     capi.release_scratch()                                         # with what the last of them left
+
+
+def test_two_threads_on_one_stream():
+    """Steps of more pieces than workgroups and of rows in parts, called by two threads on a stream that they share: one buffer, whose counters go from call to call.  It grows meanwhile."""
+    import threading
+
+    page_size, dim = 64, 64
+    g = torch.Generator(device="cuda").manual_seed(5)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+    stream = torch.cuda.Stream()
+
+    def step(heads, kv_heads, cached, new):
+        width = max(-(-(c + n) // page_size) for c, n in zip(cached, new))
+        pages, tokens = len(new) * width, sum(new)
+        keys, values = (capi.tilize(torch.randn(pages, kv_heads, page_size, dim, device="cuda", generator=g).bfloat16()) for _ in range(2))
+        rows = torch.randn(tokens, heads * dim, device="cuda", generator=g).bfloat16()
+        return (tokens, heads, kv_heads, pages, width, rows, keys, values, ints(list(range(pages))), ints(cached), ints([sum(new[:r]) for r in range(len(new) + 1)]))
+
+    def attend(what, on):
+        tokens, heads, kv_heads, pages, width, rows, keys, values, table, cached, starts = what
+        out = torch.full((tokens, heads * dim), 7.0, device="cuda", dtype=torch.bfloat16)
+        on.wait_stream(torch.cuda.current_stream())
+        capi.check(capi.lib().ttmi_paged_attention(rows.data_ptr(), capi.ROW_MAJOR, tokens, heads * dim, 0, keys.data_ptr(), values.data_ptr(), capi.BFLOAT16, pages, kv_heads, page_size, dim,
+                                                   table.data_ptr(), cached.numel(), width, cached.data_ptr(), starts.data_ptr(), heads, dim ** -0.5, 0, out.data_ptr(), None, 0, on.cuda_stream))
+        return out
+
+    steps = [step(8, 2, [900], [1]), step(8, 2, [2100], [300]), step(16, 16, [0, 7], [1100, 1205]), step(8, 2, [900, 1800, 33], [1, 1, 1])]
+    expected = [attend(what, torch.cuda.current_stream()) for what in steps]
+    torch.cuda.synchronize()
+    results = [[], []]
+
+    def calls(mine):
+        for i in range(24):
+            n = (i + 2 * mine) % len(steps)
+            results[mine].append((n, attend(steps[n], stream)))
+
+    threads = [threading.Thread(target=calls, args=(mine,)) for mine in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert [len(r) for r in results] == [24, 24]
+    for got in results:
+        for n, out in got:
+            assert torch.equal(out, expected[n])
