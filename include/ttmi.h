@@ -340,7 +340,8 @@ TTMI_API int ttmi_paged_attention_sinks(const void *rows, int layout, uint32_t t
  *   y = norm * x / sqrt(mean(x^2) + epsilon)          where `norm` (head_dim values) is given, else y = x
  *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)  of the angle p * frequencies[i]
  * for the pairs i < rotary_dim / 2 of its first rotary_dim elements: (y[i], y[i + rotary_dim / 2]), or neighbours (y[2 i], y[2 i + 1]) where
- * `interleaved` is not 0.  The other elements are y.  fp32, rounded once; angles are reduced in 64 bits, positions count up to 2^32 - 1.
+ * `interleaved` is not 0.  The other elements are y.  fp32, rounded once (a sum of squares past 3e38 makes a head zeros; sine and cosine are up to 2^-22.9 off); angles are
+ * reduced in 64 bits, positions count up to 2^32 - 1.
  *   frequencies  rotary_dim / 2 floats, rotary_dim a multiple of 16 up to head_dim (0: nothing turns); norm: floats; both 16-byte aligned
  *   head_dim     64, 96, 128 or 256
  *   out          bf16 [tokens, heads * head_dim], layout as `rows`; rows of no request, padding rows among them, are zeros.  May not overlap `rows` */

@@ -11,12 +11,12 @@
 //   units      (request, key head, tile of ROWS rows).  A unit's tokens are cut into pieces of a common length, which is chosen from the
 //              lengths on the device so that the whole step comes to about `target` pieces: requests of any lengths, one long one among
 //              them, fill the chip evenly.  Every wavefront makes the same prefix sums over the requests (1 us for 64 of them) and
-//              takes pieces blockIdx, blockIdx + gridDim, ...  A unit of one piece is stored at once; the others leave (maximum, sum, fp32
+//              takes its pieces, by its number or as they come next (below).  A unit of one piece is stored at once; the others leave (maximum, sum, fp32
 //              accumulators) in memory, and whoever comes last joins them, in the order of the pieces: results do not depend on
 //              who that is.  The join costs 3 us for one row tile, 8 for five, 15 for 256 rows of 128 elements in four parts
 //   softmax    one pass: running maximum m and sum l per row in fp32, weights exp2(s - m).  m only moves when a score passes it
 //              by more than 2^8 in weight, so that the accumulators are hardly ever rescaled (two prompts of 5000 tokens, 32 heads on 8
-//              key heads, window 4096: 527 us, 566 where m always moves)
+//              key heads, window 4096: 7 % more time where m always moves)
 //   products   keys times queries and values times weights, both transposed: a lane's accumulators belong to one row, so m, l and the
 //              rescaling are the lane's own, and the weights leave the first product in the very lanes that the second one
 //              wants them in (the tokens of a k step are permuted alike on both sides).  Weights are rounded to bf16 for
@@ -25,7 +25,8 @@
 //              few tokens have no others for the roundings to cancel against: in the block where a row ends what the rounding
 //              took off is a second product.  Elsewhere it is left out: results are 2.0e-3 to 2.2e-3 off 64 bits (2-norm over 2-norm, scores
 //              with a spread of 2), with it everywhere 1.7e-3, the rounding of the result alone.  It would cost 32 users x 2000 tokens in bf16 63.0 us
-//              instead of 61.8, drafts of 5 tokens 69.0 (66.6), 8 users x 16000 in BFLOAT8_B 124 (98), 512 tokens behind 7680 114 (86), prompts 691 (527)
+//              instead of 61.8, drafts of 5 tokens 69.0 (66.6), 8 users x 16000 in BFLOAT8_B 124 (98), and
+//              the kernel for many rows 31 to 33 %
 //   masks      a score that does not count becomes -inf, its weight 0.  bf16 values that no row of the unit sees (behind the last token,
 //              before the window) are zeroed on their way into LDS: 0 x NaN is NaN.  Where rows of a unit see different tokens, or one
 //              ends (what a rounding took off may have either sign), values that are not finite are taken out as well, and two
@@ -67,7 +68,7 @@ constexpr uint32_t COUNTERS = 4096;        // at most 2 `target` slots, each cou
 constexpr uint32_t NEXT_PIECE = COUNTERS - 1;          // pieces that workgroups of the kernel for many rows have asked for
 constexpr float LAZY = 8.f;                // how far (log2) a score may pass the running maximum
 
-// Operands go from LDS through a ring of this many, so that a product finds its own in registers.  Four took 537 us where two take 527 (two prompts of
+// Operands go from LDS through a ring of this many, so that a product finds its own in registers.  Four took 2 % more time than two (two prompts of
 // 5000 tokens with a window of 4096): they are eight registers more, which are spilled.
 constexpr int AHEAD = 2;
 // Reads of LDS and products stay in the order in which they are written; everything else may pass.
@@ -354,7 +355,7 @@ __device__ __forceinline__ void clear_rows(const AttentionDev &p, uint32_t head_
 // The next block is asked for as soon as a block's keys are multiplied and its values are in LDS.  Nothing should spill in that loop: a reload
 // from scratch memory waits for all loads before it, the next block's among them (two row tiles of 128 elements in BFLOAT8_B with 66 spilled
 // registers: 185 us instead of 83).  Hence the scheduling barriers between products of different operands.  One and two row tiles have no spilled
-// registers; five row tiles of 64 elements do not fit: 46 are spilled for BFLOAT8_B, 12 for bf16, and some are reloaded in every block.
+// registers (with sinks, two of 128 elements one for BFLOAT8_B and four for bf16); five row tiles of 64 elements do not fit: 46 are spilled for BFLOAT8_B, 12 for bf16, and some are reloaded in every block.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int D, bool PACKED> struct StreamShape {
     static constexpr int SLABS = D / 32, TILE_BYTES = PACKED ? 1088 : 2048;
@@ -808,19 +809,23 @@ __global__ __launch_bounds__(256, (MT <= 2 && D <= 128) || D == 64 ? 2 : 1) void
 // once for all rows of the unit.  v_mfma_f32_32x32x16_bf16.
 //   phases   a step is a phase of vector work (masks, softmax, the next tokens into LDS) and one of matrix work (values of this step, then
 //            keys of the next).  The two wavefronts of a SIMD are a phase apart, kept there by a barrier after every phase: one has the
-//            matrix cores while the other has the vector ALU.  In step, both wait for the same unit: 615 us instead of 527 for two
-//            prompts of 5000 tokens (BFLOAT8_B cache, window 4096, 32 heads on 8 key heads), 106 instead of 94 for 512 tokens behind 7680
-//            (bf16).  With the wavefronts in their matrix phase not preferred (s_setprio): 560 and 97.  The additions of the
-//            weights belong into the matrix phase, although v_dot2_f32_bf16 takes 20 cycles beside products: 566 and 102 us in the other
+//            matrix cores while the other has the vector ALU.  In step, both wait for the same unit: 17 % more time for two
+//            prompts of 5000 tokens (BFLOAT8_B cache, window 4096, 32 heads on 8 key heads), 13 % for 512 tokens behind 7680
+//            (bf16).  With the wavefronts in their matrix phase not preferred (s_setprio): 6 and 3 %.  The additions of the
+//            weights belong into the matrix phase, although v_dot2_f32_bf16 takes 20 cycles beside products: 7 and 9 % more in the other
 //   pieces   workgroups ask a counter for what comes next: units of a prompt see different numbers of tokens, and every 256th piece for each came to 524 us
-//            for those prompts where it is 460 now (527 in the figures above and below, which are of the time before).  Bits of a mask are taken as signed
+//            for those prompts where it is 460.  A workgroup waits for the counter's answer before it may end, also the one for which nothing is left.  201 random
+//            steps of 257 to 800 pieces, against every 256th piece for each: 0.89 of the time in the middle, least 0.62, five of them more than 1.04, most 1.11; with a
+//            fixed order up to 512 pieces it would be 0.98 in the middle.  Bits of a mask are taken as signed
 //            fields and select -inf, two instructions for a score: with comparisons a step with a boundary in it took 7700 cycles, now 5700, others 4300.
 //            The last barrier of a piece waits for LDS only, not for the stores.  A piece of 38 blocks (a window of 1024, 100 sinks, BFLOAT8_B) is 90,000 cycles of steps and
 //            20,000 around them: 8200 until the first keys lie in LDS, 2000 for the second half's last phase, 5000 for stores
-//   rate     those prompts: 460 us = 0.94 PFLOP/s of what the masks leave (a tenth more or less from card to card, and more
-//            under a profiler), a large product reaches 1.22; with 527 us, the matrix cores busy 44 % of the time,
+//   rate     those prompts: 460 to 490 us = 0.94 to 0.88 PFLOP/s of what the masks leave (575 once the chip is hot), a large product reaches 1.2 to 1.4;
+//            4096 tokens of 32 heads on 8 key heads in bf16 0.96, of 16 heads of 256 elements 0.51, 8192 tokens 1.07 and 0.56.  With a fixed order of the pieces the matrix
+//            cores were busy 44 % of the time,
 //            vector ALU 66 %: an instruction takes it 8 cycles while the matrix cores work, and a step of 32 products (1024 cycles) has 300
 //            of them for each wavefront, 140 for expanding block floats, 32 exponentials among the rest
+//   spills   128 elements: 42 VGPRs (BFLOAT8_B), 48 or 49 (bf16); 256: 57 to 70, reloaded in every step; 96 in bf16: 10; others none (64 in bf16: 32 bytes of scratch memory)
 //   LDS      three buffers each for keys and values.  In vector phase i the keys of step i + 2 and the values of step i + 1 are written, read by
 //            either half of the workgroup until the end of the matrix phases i + 1, which are one phase apart
 //   keys     16-byte chunk (row r, half h) of a face lies at r * 32 + (h ^ (r / 8)) * 16: what a pass of a ds_read_b128 touches lies

@@ -8,7 +8,8 @@
 //
 // Bound by memory, for few tokens by the launch and three loads that wait for each other (row starts, length, slot): 32 tokens of 32 heads of 128 elements
 // 4.6 us with the launch, with keys, values and norms 5.0.  8206 tokens of 71 heads of 64 elements: 33 us = 4.6 TB/s; 8183 tokens of 32 + 8 + 8 heads of 128 elements with
-// norms into BFLOAT8_B: 42 us = 4.4 TB/s, 43 without norms into bf16 (4.6 TB/s; a large copy moves 5.1).  The vector ALU is busy for 67 % of the former: 135 instructions
+// norms into BFLOAT8_B: 42 us = 4.4 TB/s, 43 without norms into bf16 (4.6 TB/s; a large copy moves 5.1).  Queries alone, 8000 tokens,
+// TILE or rows: 16 heads of 256 elements 31 us = 4.2 TB/s, 32 of 128 the same, 32 of 96 25 = 3.9.  The vector ALU is busy for 67 % of the prompts into BFLOAT8_B: 135 instructions
 // for two chunks of a head, 75 for each head's share of requests and angles.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -38,6 +39,8 @@ struct RotateDev {
 
 // Position of row t0 + r, r < ROWS, false where it is no request's.  A row belongs to the request before the first start behind it, and
 // the request's rows begin at the largest start up to its own: row starts that do not ascend are read through their running maximum.
+// 64 requests at a time, from the first one on, in every item: 4096 tokens of 32 + 8 + 8 heads of 128 elements into a bf16 cache (slots in any order) 28 us as one request or
+// 64, 29 as 512, 34 as 2048, 44 as 4096 single tokens; 512 tokens 7.1 as one request, 8.5 as 512.
 template <uint32_t ROWS> __device__ __forceinline__ bool position_of(const RotateDev &p, uint32_t t0, uint32_t r, uint32_t &position) {
     const uint32_t lane = threadIdx.x & 63;
     uint32_t owner = 0xffffffffu, from = 0, top = 0, open = (1u << ROWS) - 1;      // rows whose request is still looked for
@@ -106,8 +109,9 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], uint32_t shared, 
 }
 
 // An item is up to `each` heads of a few tokens.  LANES lanes share a token; each has two chunks of 8 elements of a head, chosen such that partners
-// of the rotation are in one lane: chunks k and k + R/16, or neighbours.  Angles are computed once for all heads of the item.  Registers decide: with all
-// heads of a token in four lanes, 256 of them, the 8183 tokens took 136 us; now 82 to 120, four to six wavefronts per SIMD.  AHEAD heads are on their
+// of the rotation are in one lane: chunks k and k + R/16, or neighbours (heads of 96 elements: six of eight lanes).  Angles are computed once for all heads of the item.  Registers decide: with all
+// heads of a token in four lanes, 256 of them, the 8183 tokens took 136 us; now 82 to 128, four or five wavefronts per SIMD (64 elements into block floats
+// without norms: 36 bytes of scratch memory as well).  AHEAD heads are on their
 // way: two 58.7 us (with the read-back of the caches), three 57.7, four 59.4.
 template <int SLABS, bool NORM, bool INTERLEAVED, bool PACKED>
 __global__ __launch_bounds__(256) void paged_rotate_kernel(const RotateDev p) {
