@@ -11,8 +11,8 @@ No counterpart under these names in tt-metal.  A step of a decoder layer, the ta
 A model without rotary positions has write_paged_cache(qkv, ...) there, and its queries in qkv.  Between steps, requests fork (fork_paged_tables, copy_paged_pages), and
 pages come back (release_paged_pages).
 
-Lengths, tables and slots are uint32 tensors on the device (0xffffffff: no page, no slot) and stay there.  The shapes and the
-rules are checked by the C++ host layer; the kernels run on torch's current stream, behind ttmi_paged_* of include/ttmi.h."""
+Lengths, tables and slots are uint32 tensors on the device (0xffffffff: no page, no slot) and stay there; they may not change while a call that reads
+them runs (calls on one stream run one after the other).  The shapes and the rules are checked by the C++ host layer; the kernels run on torch's current stream, behind ttmi_paged_* of include/ttmi.h."""
 from __future__ import annotations
 
 import math
